@@ -9,7 +9,8 @@ CSRC = os.path.join(os.path.dirname(HERE), "csrc")
 INCLUDE = os.path.join(os.path.dirname(os.path.dirname(HERE)), "include")
 LIB = os.path.join(HERE, "libcapdec.so")
 LIB_TUNE = os.path.join(HERE, "libcapdec_tune.so")
-SOURCES = ["gemm.hip", "ops.hip", "lstm.hip", "engine.hip", "train_ops.hip", "decode_fused.hip"]
+SOURCES = ["gemm.hip", "ops.hip", "lstm.hip", "engine.hip", "train_ops.hip", "decode_fused.hip", "vocab_ce.hip",
+           "muon.hip"]
 
 # no packed fp32 arithmetic (v_pk_add_f32 and its kin): some of its forms have given wrong results now and then on these
 # GPUs; the host pass does not know the feature and says so

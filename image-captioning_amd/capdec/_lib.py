@@ -22,6 +22,7 @@ DECODE_FOLD_MEMORY = 2
 DECODE_NO_FUSED_LAYERS = 4
 VOCAB_STATIC_MAX_ELEMS = 1 << 20
 E2BIG = -7
+F32, BF16, F16 = 0, 1, 2
 
 
 class GemmGroup(Structure):
@@ -67,6 +68,20 @@ class RnnModel(Structure):
 class SattModel(Structure):
     _fields_ = [("E", c_int32), ("Hd", c_int32), ("A", c_int32), ("V", c_int32)] + \
                [(n, c_void_p) for n in ("emb", "w_ih", "w_hh", "b_ih", "b_hh", "att_h_w", "att_h_b", "att_v", "fc2_w", "fc2_b")]
+
+
+class VocabCE(Structure):
+    _fields_ = [("x", c_void_p), ("W", c_void_p), ("bias", c_void_p), ("targets", c_void_p), ("ldx", c_int64),
+                ("ldw", c_int64), ("ignore_index", c_int64), ("M", c_int32), ("V", c_int32), ("K", c_int32),
+                ("dtype", c_int32)]
+
+
+class Matrix(Structure):
+    _fields_ = [("src", c_void_p), ("dst", c_void_p), ("ld_src", c_int64), ("ld_dst", c_int64)]
+
+
+class MuonParam(Structure):
+    _fields_ = [("p", c_void_p), ("g", c_void_p), ("m", c_void_p), ("ldp", c_int64), ("ldg", c_int64), ("ldm", c_int64)]
 
 
 class Probe(Structure):
@@ -172,6 +187,17 @@ _SIGNATURES = {
                                               _P, _P, _P, _P]),
     "capdec_axpy_rows": (c_int, [_P, c_int, c_float, c_int, c_int, _P, c_int, _P]),
     "capdec_topk_rows": (c_int, [_P, c_int, c_int, c_int, _P, _P, _P]),
+    "capdec_vocab_ce_saved_bytes": (c_size_t, [POINTER(VocabCE)]),
+    "capdec_vocab_ce_forward_workspace_bytes": (c_size_t, [POINTER(VocabCE)]),
+    "capdec_vocab_ce_backward_workspace_bytes": (c_size_t, [POINTER(VocabCE)]),
+    "capdec_vocab_ce_forward": (c_int, [POINTER(VocabCE), _P, c_size_t, _P, c_size_t, _P, _P, _P]),
+    "capdec_vocab_ce_backward": (c_int, [POINTER(VocabCE), _P, c_size_t, _P, c_size_t, _P, _P, c_int, _P, c_int64, _P,
+                                         c_int64, _P, _P]),
+    "capdec_orthogonalize_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "capdec_orthogonalize": (c_int, [POINTER(Matrix), c_int, c_int, c_int, c_int, c_int, POINTER(c_float), c_float, _P,
+                                     c_size_t, _P]),
+    "capdec_muon_step": (c_int, [POINTER(MuonParam), c_int, c_int, c_int, c_float, _P, c_float, c_int, c_float, c_float,
+                                 c_float, c_int, POINTER(c_float), c_float, _P, c_size_t, _P]),
     "capdec_vocab_argmax_static": (c_int, [_P, c_int64, _P, _P, c_int, c_int, c_int, _P, _P, _P]),
 }
 

@@ -660,6 +660,38 @@ def _decoder_params(dec):
     return out
 
 
+class _VocabCrossEntropyFn(torch.autograd.Function):
+    """``ops.vocab_ce_forward`` / ``vocab_ce_backward`` as an autograd node; reduction "none", "sum" or "mean"."""
+
+    @staticmethod
+    def forward(ctx, x, W, b, targets, ignore_index, reduction):
+        ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        if x.shape[0] == 0:                       # no rows: the mean over none is NaN, every gradient zero
+            ctx.save_for_backward(x, W, b, targets, None)
+            return {"none": x.new_zeros(0, dtype=torch.float32), "sum": x.new_zeros((), dtype=torch.float32),
+                    "mean": x.new_full((), float("nan"), dtype=torch.float32)}[reduction]
+        nll, loss, saved = ops.vocab_ce_forward(x, W, b, targets, ignore_index, want_loss=reduction != "none")
+        ctx.save_for_backward(x, W, b, targets, saved)
+        return nll if reduction == "none" else loss[0 if reduction == "mean" else 1]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, W, b, targets, saved = ctx.saved_tensors
+        if saved is None:
+            return tuple(torch.zeros_like(t) if t is not None and n else None
+                         for t, n in zip((x, W, b), ctx.needs_input_grad)) + (None, None, None)
+        g = g.float().contiguous()
+        up = dict(row_grad=g) if ctx.reduction == "none" else dict(grad=g, mean=ctx.reduction == "mean")
+        dx, dW, db = ops.vocab_ce_backward(x, W, b, targets, saved, ignore_index=ctx.ignore_index,
+                                           need=ctx.needs_input_grad[:3], **up)
+        return dx, dW, db, None, None, None
+
+
+def vocab_cross_entropy(x, W, b, targets, ignore_index, reduction):
+    return _VocabCrossEntropyFn.apply(x, W, b, targets, ignore_index, reduction)
+
+
 class _DecoderLogitsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, dec, captions, enc, *params):

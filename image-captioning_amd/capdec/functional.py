@@ -59,3 +59,26 @@ def decoder_rnn_forward(rnn, features, captions):
     for t in range(T):
         h, c = ops.lstm_step(emb[:, t], h, c, *w, h_out=hs[:, t])   # h' lands in the [B,T,Hd] slab
     return ops.linear(hs.view(B * T, Hd), rnn.fc2.weight, rnn.fc2.bias).view(B, T, -1)
+
+
+def vocab_cross_entropy(x, weight, bias, targets, ignore_index=0, reduction="mean"):
+    """Cross entropy of a vocabulary projection, ``cross_entropy(x @ weight.T + bias, targets)``, without the logits: they
+    are formed tile by tile, in the forward pass and again, a piece of the vocabulary at a time, in the backward pass.
+
+    x [..., K], weight [V, K] and bias [V] (or None) share one type: float32, bfloat16 or float16; targets [...] int64.
+    Rows whose target is ``ignore_index`` have loss 0 and gradient 0 and are not read; any other target outside [0, V)
+    makes the loss NaN.  reduction: "mean" over the counted rows (NaN if there are none; the gradients are zero then),
+    "sum", or "none" (a loss per target).  The loss is float32; gradients flow to x, weight and bias in their own type.
+
+    A backward pass that is to be captured in a HIP graph must not run while an eager graph of the same leaves is alive:
+    drop the losses of earlier eager passes first."""
+    from . import autograd as AG
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"capdec: reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    if x.dim() < 1 or x.shape[:-1] != targets.shape:
+        raise RuntimeError(f"capdec: x {tuple(x.shape)} and targets {tuple(targets.shape)} do not fit")
+    x2, t = x.reshape(-1, x.shape[-1]), targets.reshape(-1)
+    if x2.stride(1) != 1 and x2.shape[1] > 1:
+        x2 = x2.contiguous()
+    loss = AG.vocab_cross_entropy(x2, weight, bias, t.contiguous(), ignore_index, reduction)
+    return loss.view(targets.shape) if reduction == "none" else loss

@@ -2,6 +2,7 @@
 
 PyTorch is used for device memory and the stream only; all arithmetic happens in libcapdec.so.
 """
+import ctypes
 import os
 from ctypes import byref
 
@@ -968,6 +969,203 @@ def adam_step_dev(p, g, m, v, state, beta1=0.9, beta2=0.999, eps=1e-8, grad_scal
     _lib.check(lib.capdec_adam_step_dev(_chk(p).data_ptr(), _chk(g).data_ptr(), _chk(m).data_ptr(), _chk(v).data_ptr(),
                                         p.numel(), beta1, beta2, eps, state.buf.data_ptr(), grad_scale, _stream()),
                "capdec_adam_step_dev")
+
+
+# ---------------------------------------------------------------------------------------------
+# vocabulary cross entropy without kept logits
+# ---------------------------------------------------------------------------------------------
+_DTYPE_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _same_device(what, *tensors):
+    """Every tensor on the current GPU (the wrappers launch on its current stream)."""
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != torch.cuda.current_device()):
+            raise RuntimeError(f"capdec {what}: every tensor must be on the current GPU (HIP device "
+                               f"{torch.cuda.current_device() if torch.cuda.is_available() else 'none'}), got {t.device}")
+
+
+def _bytes(n, device):
+    return torch.empty(int(n), device=device, dtype=torch.uint8)
+
+
+def _vocab_ce_args(x, W, b, targets, ignore_index):
+    for t, name in ((x, "x"), (W, "W"), (targets, "targets")) + (((b, "bias"),) if b is not None else ()):
+        if not isinstance(t, torch.Tensor):
+            raise RuntimeError(f"capdec vocab_ce: {name} must be a tensor")
+    _same_device("vocab_ce", x, W, b, targets)
+    if x.dtype not in _DTYPE_CODE or W.dtype != x.dtype or (b is not None and b.dtype != x.dtype):
+        raise RuntimeError("capdec vocab_ce: x, W and bias must share one type, float32, bfloat16 or float16; got "
+                           f"{x.dtype}, {W.dtype}" + (f", {b.dtype}" if b is not None else ""))
+    if x.dim() != 2 or W.dim() != 2 or x.shape[1] != W.shape[1] or min(x.shape + W.shape) < 1:
+        raise RuntimeError(f"capdec vocab_ce: x [M,K] and W [V,K] expected, got {tuple(x.shape)} and {tuple(W.shape)}")
+    if targets.dtype != torch.int64 or targets.dim() != 1 or targets.shape[0] != x.shape[0] or not targets.is_contiguous():
+        raise RuntimeError(f"capdec vocab_ce: targets must be {x.shape[0]} contiguous int64 values, got {targets.dtype} "
+                           f"{tuple(targets.shape)}")
+    if b is not None and (b.dim() != 1 or b.shape[0] != W.shape[0] or not b.is_contiguous()):
+        raise RuntimeError(f"capdec vocab_ce: bias must hold {W.shape[0]} contiguous values, got {tuple(b.shape)}")
+    a = _lib.VocabCE(x=x.data_ptr(), W=W.data_ptr(), bias=_ptr(b), targets=targets.data_ptr(), ldx=_row_stride(x, "x"),
+                     ldw=_row_stride(W, "W"), ignore_index=ignore_index, M=x.shape[0], V=W.shape[0], K=x.shape[1],
+                     dtype=_DTYPE_CODE[x.dtype])
+    return a
+
+
+def vocab_ce_forward(x, W, b, targets, ignore_index=0, want_loss=True):
+    """Cross entropy of the projection x W^T + b, no logits kept: x [M,K], W [V,K], b [V] or None, all float32, bfloat16
+    or float16 with unit column stride; targets [M] int64.  Returns (nll [M] fp32 with zeros for ignored rows,
+    loss [3] fp32 = (mean over the counted rows, sum, their number) or None, saved): ``saved`` goes to
+    ``vocab_ce_backward``."""
+    lib = _lib.load()
+    a = _vocab_ce_args(x, W, b, targets, ignore_index)
+    saved_bytes = lib.capdec_vocab_ce_saved_bytes(byref(a))
+    ws_bytes = lib.capdec_vocab_ce_forward_workspace_bytes(byref(a))
+    if not saved_bytes:
+        raise RuntimeError(f"capdec vocab_ce: unsupported sizes M={a.M} V={a.V} K={a.K}")
+    saved, ws = _bytes(saved_bytes, x.device), _bytes(ws_bytes, x.device)
+    out = torch.empty(a.M + 3, device=x.device, dtype=torch.float32)
+    nll, loss = out[:a.M], (out[a.M:] if want_loss else None)
+    _lib.check(lib.capdec_vocab_ce_forward(byref(a), saved.data_ptr(), saved_bytes, ws.data_ptr(), ws_bytes, nll.data_ptr(),
+                                           _ptr(loss), _stream()), "capdec_vocab_ce_forward")
+    return nll, loss, saved
+
+
+def vocab_ce_backward(x, W, b, targets, saved, grad=None, row_grad=None, mean=True, ignore_index=0, dx=None, dW=None, db=None,
+                      need=(True, True, True)):
+    """Gradients of ``vocab_ce_forward``.  The upstream gradient is ``row_grad`` [M] fp32 (of nll) or ``grad``, a one-element
+    fp32 tensor (of the mean, or with ``mean=False`` of the sum).  Returns (dx, dW, db) in the operands' type, written into
+    the tensors given for them, or None where ``need`` says so."""
+    lib = _lib.load()
+    a = _vocab_ce_args(x, W, b, targets, ignore_index)
+    if (grad is None) == (row_grad is None):
+        raise RuntimeError("capdec vocab_ce_backward: exactly one of grad and row_grad")
+    g = grad if grad is not None else row_grad
+    _same_device("vocab_ce_backward", _chk(g, name="upstream gradient"), saved)
+    if g.numel() != (1 if grad is not None else a.M) or not g.is_contiguous():
+        raise RuntimeError(f"capdec vocab_ce_backward: upstream gradient {tuple(g.shape)} does not fit {a.M} rows")
+    outs = []
+    for given, like, want, name in ((dx, x, need[0], "dx"), (dW, W, need[1], "dW"), (db, b, need[2], "db")):
+        if like is None or not want:
+            outs.append(None)
+            continue
+        if given is None:
+            given = torch.empty(like.shape, device=like.device, dtype=like.dtype)
+        elif given.dtype != like.dtype or given.shape != like.shape or given.device != like.device or given.stride(-1) != 1:
+            raise RuntimeError(f"capdec vocab_ce_backward: {name} must be {like.dtype} {tuple(like.shape)} on {like.device}")
+        outs.append(given)
+    dx, dW, db = outs
+    ws_bytes = lib.capdec_vocab_ce_backward_workspace_bytes(byref(a))
+    ws = _bytes(ws_bytes, x.device)
+    _lib.check(lib.capdec_vocab_ce_backward(byref(a), _chk(saved, torch.uint8, "saved").data_ptr(), saved.numel(),
+                                            ws.data_ptr(), ws_bytes, _ptr(row_grad), _ptr(grad), 1 if mean else 0, _ptr(dx),
+                                            0 if dx is None else _row_stride(dx, "dx"), _ptr(dW),
+                                            0 if dW is None else _row_stride(dW, "dW"), _ptr(db), _stream()),
+               "capdec_vocab_ce_backward")
+    return dx, dW, db
+
+
+# ---------------------------------------------------------------------------------------------
+# orthogonalised updates of weight matrices
+# ---------------------------------------------------------------------------------------------
+NS_COEFFS = (3.4445, -4.7750, 2.0315)
+
+
+def _ns_coeffs(coeffs):
+    if len(coeffs) != 3:
+        raise RuntimeError(f"capdec: three coefficients (a, b, c) expected, got {coeffs!r}")
+    return (ctypes.c_float * 3)(*coeffs)
+
+
+def _matrices(what, ts, dtypes):
+    """The 2-D matrices of a tensor [..., rows, cols] or of a list of 2-D tensors, unit column stride."""
+    if isinstance(ts, torch.Tensor):
+        if ts.dim() < 2:
+            raise RuntimeError(f"capdec {what}: a matrix or a batch of matrices expected, got shape {tuple(ts.shape)}")
+        ts = list(ts.unbind(0)) if ts.dim() == 3 else [ts] if ts.dim() == 2 else list(ts.flatten(0, -3).unbind(0))
+    ts = list(ts)
+    for t in ts:
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise RuntimeError(f"capdec {what}: tensors on the GPU (HIP) expected; there is no CPU path")
+        if t.dtype not in dtypes or t.dtype != ts[0].dtype:
+            raise RuntimeError(f"capdec {what}: one type of {[str(d) for d in dtypes]} expected, got {t.dtype}")
+        if t.dim() != 2 or min(t.shape) < 1:
+            raise RuntimeError(f"capdec {what}: non-empty matrices expected, got shape {tuple(t.shape)}")
+    return ts
+
+
+def _distinct(what, ts):
+    """Outputs of one call must not share memory."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.element_size() * (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1))
+                   for t in ts)
+    for (_, end), (start, _) in zip(spans, spans[1:]):
+        if start < end:
+            raise RuntimeError(f"capdec {what}: two of the matrices written overlap in memory")
+
+
+def orthogonalize(mats, steps=5, coeffs=NS_COEFFS, eps=1e-7, out=None):
+    """Newton-Schulz iteration of each matrix: X = G / (|G|_F + eps), then ``steps`` times X <- a X + (b A + c A^2) X with
+    A = X X^T (the shorter side's Gram matrix), (a, b, c) = ``coeffs``; it drives the singular values towards 1.
+
+    ``mats``: a matrix, a batch [..., rows, cols], or a list of matrices (shapes may differ), float32, bfloat16 or float16.
+    Returns the results in the same form and type, written to ``out`` if given (which may be ``mats``)."""
+    lib = _lib.load()
+    src = _matrices("orthogonalize", mats, tuple(_DTYPE_CODE))
+    if out is None:
+        out = torch.empty(mats.shape, device=mats.device, dtype=mats.dtype) if isinstance(mats, torch.Tensor) else \
+            [torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in src]
+    dst = _matrices("orthogonalize", out, tuple(_DTYPE_CODE))
+    if [(t.shape, t.dtype) for t in src] != [(t.shape, t.dtype) for t in dst]:
+        raise RuntimeError("capdec orthogonalize: out must match the matrices in shape and type")
+    _same_device("orthogonalize", *src, *dst)
+    if len(dst) > 1:
+        _distinct("orthogonalize", dst)
+    co = _ns_coeffs(coeffs)
+    for (rows, cols), idx in _by_shape(src).items():
+        arr = (_lib.Matrix * len(idx))()
+        for a, i in zip(arr, idx):
+            a.src, a.dst = src[i].data_ptr(), dst[i].data_ptr()
+            a.ld_src, a.ld_dst = _row_stride(src[i], "matrix"), _row_stride(dst[i], "out")
+        ws = _bytes(lib.capdec_orthogonalize_workspace_bytes(len(idx), rows, cols), src[0].device)
+        _lib.check(lib.capdec_orthogonalize(arr, len(idx), rows, cols, _DTYPE_CODE[src[0].dtype], steps, co, eps,
+                                            ws.data_ptr(), ws.numel(), _stream()), "capdec_orthogonalize")
+    return out
+
+
+def _by_shape(ts):
+    groups = {}
+    for i, t in enumerate(ts):
+        groups.setdefault(tuple(t.shape), []).append(i)
+    return groups
+
+
+def muon_step(params, grads, momenta, lr=None, state=None, momentum=0.95, nesterov=True, weight_decay=0.0,
+              update_scale=None, grad_scale=1.0, steps=5, coeffs=NS_COEFFS, eps=1e-7):
+    """One step of weight matrices along their orthogonalised momentum, in place: m <- momentum m + grad_scale g,
+    u = g + momentum m (``nesterov``) or m, p <- p (1 - lr weight_decay) - lr update_scale orthogonalize(u).
+
+    Lists of fp32 matrices (shapes may differ; one launch sequence per shape).  ``update_scale`` None: sqrt(max(1, rows /
+    cols)) of each shape, so that the update's entries have the same size whatever the aspect.  The learning rate is
+    ``lr``, or the device-resident one of ``state`` (``TrainState``), which a captured step reads at every replay."""
+    lib = _lib.load()
+    if (lr is None) == (state is None):
+        raise RuntimeError("capdec muon_step: exactly one of lr and state")
+    f32 = (torch.float32,)
+    p, g, m = (_matrices("muon_step", t, f32) for t in (params, grads, momenta))
+    if not ([t.shape for t in p] == [t.shape for t in g] == [t.shape for t in m]):
+        raise RuntimeError("capdec muon_step: params, grads and momenta must match in number and shape")
+    _same_device("muon_step", *p, *g, *m)
+    _distinct("muon_step", p + m)
+    co = _ns_coeffs(coeffs)
+    for (rows, cols), idx in _by_shape(p).items():
+        arr = (_lib.MuonParam * len(idx))()
+        for a, i in zip(arr, idx):
+            a.p, a.g, a.m = p[i].data_ptr(), g[i].data_ptr(), m[i].data_ptr()
+            a.ldp, a.ldg, a.ldm = _row_stride(p[i], "param"), _row_stride(g[i], "grad"), _row_stride(m[i], "momentum")
+        ws = _bytes(lib.capdec_orthogonalize_workspace_bytes(len(idx), rows, cols), p[0].device)
+        scale = max(1.0, rows / cols) ** 0.5 if update_scale is None else update_scale
+        _lib.check(lib.capdec_muon_step(arr, len(idx), rows, cols, 0.0 if lr is None else lr,
+                                        None if state is None else state.buf.data_ptr(), momentum, 1 if nesterov else 0,
+                                        weight_decay, scale, grad_scale, steps, co, eps, ws.data_ptr(), ws.numel(),
+                                        _stream()), "capdec_muon_step")
 
 
 # ---------------------------------------------------------------------------------------------

@@ -1,0 +1,261 @@
+// 16-bit MFMA contraction core for gfx950 (v_mfma_f32_32x32x16_{f16,bf16}, sums in fp32), shared by the vocabulary
+// cross entropy and the orthogonalised weight update.
+//
+//   D[i,j] = sum_k P(i,k) Q(j,k)        j on the lane, i in the registers of the 32x32 accumulators
+//
+// Each operand is stored either k-contiguous ([x][k], "N") or x-contiguous ([k][x], "T": the contraction runs over its
+// leading axis).  Tiles reach LDS by global_load_lds (1 KiB pieces, lane l at byte 16 l, XOR-swizzled through the source
+// address), in a ring of three buffers: two k-tiles are in flight while one is multiplied, one barrier per tile.  T
+// tiles are transposed by the LDS read itself (ds_read_b64_tr_b16).
+//
+// SPLIT operands carry 32-bit values as two fp16 numbers, v * s = hi + lo with s a power of two: 22 significant bits.
+// They are stored with twice the columns, [row][col / 16][hi, lo][16], which serves both orientations; a k-tile is then
+// 16 wide and feeds three products, lo*hi + hi*lo + hi*hi (lo*lo is below 2^-22 of the result).  Three MFMA passes
+// against sixteen for the fp32 matrix instruction at the same flops.
+//
+// Bounds: rows of an N operand past its end are copies of its last row, columns of a T operand past its end are copies
+// of its last 8 (both feed only outputs that are not stored); k-tiles are whole, so operands are padded to 32 columns
+// (16 k when SPLIT) by their producers; T operands may name a limit on their k rows, past which the last row is read
+// against zeros of the other operand.
+#pragma once
+#include "common.h"
+
+namespace mma16 {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+enum { F16 = 0, BF16 = 1 };
+
+// ---- element conversions (round to nearest even; 16-bit values as raw bits) ------------------------------------------
+template <int ELT>
+__device__ __forceinline__ short to_bits(float v) {
+    if (ELT == BF16) {
+        __bf16 b = (__bf16)v;
+        return __builtin_bit_cast(short, b);
+    }
+    _Float16 h = (_Float16)v;
+    return __builtin_bit_cast(short, h);
+}
+template <int ELT>
+__device__ __forceinline__ float from_bits(short b) {
+    if (ELT == BF16) return (float)__builtin_bit_cast(__bf16, b);
+    return (float)__builtin_bit_cast(_Float16, b);
+}
+// v = hi + lo in fp16; an infinite or not-a-number v stays that in hi
+__device__ __forceinline__ void split16(float v, short& hi, short& lo) {
+    const _Float16 h = (_Float16)v;
+    const _Float16 l = (_Float16)(v - (float)h);
+    hi = __builtin_bit_cast(short, h);
+    lo = __builtin_bit_cast(short, l);
+}
+// first of the two stored columns of logical column c of a SPLIT matrix (the other is 16 further on)
+__host__ __device__ __forceinline__ int64_t split_col(int64_t c) { return (c >> 4) * 32 + (c & 15); }
+
+template <int ELT>
+__device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
+    if (ELT == BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// accumulator register e of lane half h is row (e & 3) + 8 (e >> 2) + 4 h of the 32x32 tile
+__device__ __forceinline__ int acc_row(int e, int h) { return (e & 3) + 8 * (e >> 2) + 4 * h; }
+
+struct View {               // one operand
+    const short* p;
+    int64_t ld;             // stored elements between rows
+    int n;                  // extent of the i or j axis (logical)
+    int klim;               // T: number of k rows that exist
+};
+
+template <int NX, bool T, bool SPLIT>
+struct Operand {
+    static constexpr int PIECES = NX / 16;                    // 1 KiB each
+    static constexpr int NXS = NX * (SPLIT ? 2 : 1);          // T: stored columns per k row of the tile
+    static constexpr int KT = SPLIT ? 16 : 32;                // logical k per tile
+    static constexpr int CPR = NXS / 8, KPP = 512 / NXS;      // T: 16-byte chunks per k row, k rows per piece
+    static_assert(NX % 64 == 0 && NXS <= 512, "tile width not built");
+
+    // N: rows of four 16-byte slots.  The 16-lane groups of a ds_read_b128 read rows whose (row / 4) % 8 are
+    // {0,3,5,6} or {1,2,4,7} for each row % 4; this maps them to four different slots.
+    __device__ static int swz_n(int row) {
+        const int q = (row >> 2) & 7;
+        return (q & 3) ^ ((q >> 2) * 3);
+    }
+    // T: 32-byte granules (16 x of one k).  A half-wave reads two granules of each of four k rows: granules g, g+1
+    // (SPLIT: g, g+2, hi and lo alternate); the XOR spreads them over the eight granules of a 256-byte bank row.
+    __device__ static int swz_t(int k) {
+        if (SPLIT) return (k & 1) | ((k & 2) << 1);
+        return NXS >= 128 ? 2 * (k & 3) : (k & 2);
+    }
+    __device__ static const short* source(const View& v, int x0, int kt, int piece, int lane) {
+        if (!T) {
+            const int row = piece * 16 + (lane >> 2);
+            const int slot = (lane & 3) ^ swz_n(row);
+            return v.p + (int64_t)min(x0 + row, v.n - 1) * v.ld + (int64_t)kt * 32 + slot * 8;
+        }
+        const int kr = piece * KPP + lane / CPR;
+        const int chunk = (lane % CPR) ^ (swz_t(kr) << 1);
+        const int k = min(kt * KT + kr, v.klim - 1);
+        return v.p + (int64_t)k * v.ld + min(x0 * (SPLIT ? 2 : 1) + chunk * 8, v.n * (SPLIT ? 2 : 1) - 8);
+    }
+    // elements a source pointer moves per k-tile
+    __device__ static int64_t step(const View& v) { return T ? (int64_t)KT * v.ld : 32; }
+    // eight k values of row w0 + (lane & 31): k = 8 (lane >> 5) + 0..7 of k-chunk kc (SPLIT: kc is the plane)
+    __device__ static s16x8 frag(const short* img, int w0, int kc, int lane) {
+        const int h = lane >> 5;
+        if (!T) {
+            const int row = w0 + (lane & 31);
+            return *reinterpret_cast<const s16x8*>(img + row * 32 + (((kc * 2 + h) ^ swz_n(row)) * 8));
+        }
+        const int li = lane & 15;
+        const int k = (SPLIT ? 0 : kc * 16) + 8 * h + (li >> 2);
+        const int blk = (w0 >> 4) + ((lane >> 4) & 1);
+        const int gran = (SPLIT ? 2 * blk + kc : blk) ^ swz_t(k);
+        const short* a = img + k * NXS + gran * 16 + (li & 3) * 4;
+        typedef __attribute__((address_space(3))) s16x4* lp;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)a);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(a + 4 * NXS));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
+
+// A workgroup of 2 x 2 wavefronts, each holding TI x TJ accumulators of 32x32.
+template <int TI_, int TJ_>
+struct Tile {
+    static constexpr int TI = TI_, TJ = TJ_;
+    static constexpr int BI = 64 * TI, BJ = 64 * TJ;
+    static constexpr int THREADS = 256;
+    static constexpr int STAGE = (BI + BJ) * 32;              // 16-bit elements of one ring buffer
+    static constexpr int LDS_BYTES = 3 * STAGE * 2;
+};
+typedef Tile<4, 2> Big;        // 256 x 128: 72 KiB of LDS, two workgroups per CU
+typedef Tile<2, 2> Mid;        // 128 x 128: 48 KiB, three
+typedef Tile<1, 1> Small;      //  64 x  64: 24 KiB
+
+// Adds k-tiles [kt0, kt1) of the tile at (i0, j0) onto zero.  Ends behind a barrier: the caller may reuse `lds`.
+template <class C, int ELT, bool TP, bool TQ, bool SPLIT>
+__device__ __forceinline__ void contract(const View& P, const View& Q, int i0, int j0, int kt0, int kt1, short* lds,
+                                         f32x16 (&acc)[C::TI][C::TJ]) {
+    using OpP = Operand<C::BI, TP, SPLIT>;
+    using OpQ = Operand<C::BJ, TQ, SPLIT>;
+    constexpr int NPW = (OpP::PIECES + OpQ::PIECES) / 4;
+    static_assert(OpP::PIECES % 4 == 0 && OpQ::PIECES % 4 == 0, "pieces do not divide over the wavefronts");
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wi = wave >> 1, wj = wave & 1;
+#pragma unroll
+    for (int ti = 0; ti < C::TI; ++ti)
+#pragma unroll
+        for (int tj = 0; tj < C::TJ; ++tj)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[ti][tj][e] = 0.f;
+
+    const short* src[NPW];
+    auto seek = [&](int kt) {
+#pragma unroll
+        for (int i = 0; i < NPW; ++i) {
+            const int piece = i * 4 + wave;
+            src[i] = i * 4 < OpP::PIECES ? OpP::source(P, i0, kt, piece, lane)
+                                         : OpQ::source(Q, j0, kt, piece - OpP::PIECES, lane);
+        }
+    };
+    const int64_t stepP = OpP::step(P), stepQ = OpQ::step(Q);
+    // the first k-tile that reaches past a T operand's rows: its addresses are clamped one by one
+    const int ragged = min(TP ? P.klim / OpP::KT : kt1, TQ ? Q.klim / OpQ::KT : kt1);
+    auto issue = [&](short* buf, int kt) {
+        if ((TP || TQ) && kt >= ragged) seek(kt);
+#pragma unroll
+        for (int i = 0; i < NPW; ++i) {
+            const int piece = i * 4 + wave;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src[i],
+                                             (__attribute__((address_space(3))) void*)(buf + piece * 512), 16, 0, 0);
+            src[i] += i * 4 < OpP::PIECES ? stepP : stepQ;
+        }
+    };
+    auto compute = [&](const short* ip) {
+        const short* iq = ip + C::BI * 32;
+        if (SPLIT) {
+            s16x8 a[2][C::TI], b[2][C::TJ];
+#pragma unroll
+            for (int pl = 0; pl < 2; ++pl) {
+#pragma unroll
+                for (int ti = 0; ti < C::TI; ++ti) a[pl][ti] = OpP::frag(ip, (wi * C::TI + ti) * 32, pl, lane);
+#pragma unroll
+                for (int tj = 0; tj < C::TJ; ++tj) b[pl][tj] = OpQ::frag(iq, (wj * C::TJ + tj) * 32, pl, lane);
+            }
+#pragma unroll
+            for (int t = 0; t < 3; ++t)        // hi*hi first: its operands arrive first
+#pragma unroll
+                for (int ti = 0; ti < C::TI; ++ti)
+#pragma unroll
+                    for (int tj = 0; tj < C::TJ; ++tj)
+                        acc[ti][tj] = mfma<ELT>(a[t == 2][ti], b[t == 1][tj], acc[ti][tj]);
+        } else {
+#pragma unroll
+            for (int kc = 0; kc < 2; ++kc) {
+                s16x8 a[C::TI], b[C::TJ];
+#pragma unroll
+                for (int ti = 0; ti < C::TI; ++ti) a[ti] = OpP::frag(ip, (wi * C::TI + ti) * 32, kc, lane);
+#pragma unroll
+                for (int tj = 0; tj < C::TJ; ++tj) b[tj] = OpQ::frag(iq, (wj * C::TJ + tj) * 32, kc, lane);
+#pragma unroll
+                for (int ti = 0; ti < C::TI; ++ti)
+#pragma unroll
+                    for (int tj = 0; tj < C::TJ; ++tj) acc[ti][tj] = mfma<ELT>(a[ti], b[tj], acc[ti][tj]);
+            }
+        }
+    };
+    short* rd = lds;                          // the buffer of tile kt
+    short* wr = lds + 2 * C::STAGE;           // the buffer of tile kt + 2
+    if (kt0 < kt1) {
+        seek(kt0);
+        issue(rd, kt0);
+    }
+    if (kt0 + 1 < kt1) issue(rd + C::STAGE, kt0 + 1);
+    for (int kt = kt0; kt < kt1; ++kt) {
+        // this wavefront's pieces of tile kt have landed (those of kt + 1 may stay in flight, loads retire in order) and
+        // it is done reading the buffer that tile kt + 2 goes to; the barrier says so for all four
+        if (kt + 1 < kt1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NPW) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        if (kt + 2 < kt1) issue(wr, kt + 2);
+        __builtin_amdgcn_sched_barrier(0);
+        compute(rd);
+        __builtin_amdgcn_sched_barrier(0);
+        wr = rd;
+        rd = rd == lds + 2 * C::STAGE ? lds : rd + C::STAGE;
+    }
+    __syncthreads();
+}
+
+// Workgroup -> tile.  Workgroup ids go round-robin to the 8 XCDs, each with an L2 of its own: XCD x takes the x-th
+// eighth of the tile sequence, and the sequence walks blocks of eight i-tiles by all j, so that the workgroups that run
+// on one XCD at a time share operand rows.  A performance assumption only.
+struct Map {
+    int ni, nj, nz, per;       // per: tiles per XCD
+};
+inline unsigned make_map(Map& m, int ni, int nj, int nz) {
+    m.ni = ni; m.nj = nj; m.nz = nz;
+    const int64_t total = (int64_t)ni * nj * nz;
+    m.per = (int)((total + 7) / 8);
+    return (unsigned)m.per * 8u;
+}
+__device__ __forceinline__ bool tile_of(const Map& m, unsigned block, int& ti, int& tj, int& z) {
+    const int t = (int)(block & 7) * m.per + (int)(block >> 3);
+    const int plane = m.ni * m.nj;
+    z = t / plane;
+    if ((int)(block >> 3) >= m.per || z >= m.nz) return false;
+    int u = t - z * plane;
+    const int band = u / (8 * m.nj);
+    u -= band * 8 * m.nj;
+    const int rows = min(8, m.ni - band * 8);
+    ti = band * 8 + u % rows;
+    tj = u / rows;
+    return true;
+}
+
+}  // namespace mma16

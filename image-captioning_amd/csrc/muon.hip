@@ -1,0 +1,426 @@
+// Orthogonalised updates of weight matrices.
+//
+//   X_0 = U / (|U|_F + eps);   A = X X^T,  B = b A + c A^2,  X <- a X + B X     (steps times)
+//
+// on the shorter side: a tall matrix takes A = X^T X and X <- a X + X B, read through the transposing operand paths, so
+// nothing is transposed in memory.  Three products per step, 2 (2 m^2 n + m^3) flops, m <= n: bound by the matrix cores
+// from about 1000 x 1000 on, by launch and pipeline latency below.
+// The iterate, A and B are kept as pairs of fp16 numbers times a power of two (SPLIT in mma16.h) with fp32 sums: an error
+// made while r steps remain grows by up to a^r (3.4^r for the usual coefficients) in the directions whose singular
+// values are still small, so the early steps need all of fp32's digits whatever the matrices' type.  The powers of two
+// come from the exact maxima of the polynomials on the interval that the singular values can be in.
+#include "mma16.h"
+#include <math.h>
+
+using namespace mma16;
+
+namespace {
+
+constexpr int MAX_BATCH = 32;             // matrices per launch (their descriptors are kernel arguments)
+constexpr size_t BATCH_BYTES = (size_t)1 << 30;
+constexpr int NORM_BLOCKS = 64;           // partial sums of squares per matrix
+
+struct Item {
+    const void* src;                      // orthogonalize: the matrix;  update: the gradient
+    void* dst;                            // orthogonalize: the result;  update: the parameter
+    float* mom;                           // update: the momentum
+    int64_t lds, ldd, ldm;
+};
+struct Batch {
+    Item it[MAX_BATCH];
+};
+
+struct Dims {
+    int rows, cols, rp, cp, m;            // rp, cp: rounded up to 32; m: the shorter of the two
+    bool tall;
+    size_t x_elems, a_elems;              // 16-bit elements of one matrix
+    size_t per, norm;                     // workspace bytes per matrix, and of the partial sums of a batch
+    int batch;
+};
+
+bool make_dims(int count, int rows, int cols, Dims& d) {
+    if (count < 1 || rows < 1 || cols < 1 || rows > (1 << 20) || cols > (1 << 20)) return false;
+    if ((int64_t)rows * cols > (int64_t)1 << 31) return false;
+    d.rows = rows; d.cols = cols;
+    d.rp = (rows + 31) / 32 * 32;
+    d.cp = (cols + 31) / 32 * 32;
+    d.tall = rows > cols;
+    d.m = d.tall ? d.cp : d.rp;
+    d.x_elems = (size_t)d.rp * d.cp * 2;
+    d.a_elems = (size_t)d.m * d.m * 2;
+    d.per = (2 * d.x_elems + 2 * d.a_elems) * 2;
+    size_t b = BATCH_BYTES / d.per;
+    d.batch = b < 1 ? 1 : b > MAX_BATCH ? MAX_BATCH : (int)b;
+    if (d.batch > count) d.batch = count;
+    d.norm = (size_t)d.batch * NORM_BLOCKS * 8;
+    return true;
+}
+
+__device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int dtype) {
+    if (dtype == CAPDEC_F32) return ((const float*)p)[i];
+    const short b = ((const short*)p)[i];
+    return dtype == CAPDEC_BF16 ? from_bits<BF16>(b) : from_bits<F16>(b);
+}
+__device__ __forceinline__ void store_as(void* p, int64_t i, float v, int dtype) {
+    if (dtype == CAPDEC_F32) ((float*)p)[i] = v;
+    else ((short*)p)[i] = dtype == CAPDEC_BF16 ? to_bits<BF16>(v) : to_bits<F16>(v);
+}
+
+struct Momentum {                         // update only (on != 0)
+    int on, nesterov;
+    float mu, grad_scale;
+};
+
+// Sums of squares of U in double (no square over- or underflows), one partial per block in a fixed order; an update
+// advances its momentum here.  A wavefront per row.
+__global__ __launch_bounds__(256) void norm_kernel(Batch b, int rows, int cols, int dtype, Momentum mo, double* __restrict__ part) {
+    const Item& it = b.it[blockIdx.y];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    double s = 0.0;
+    for (int r = blockIdx.x * 4 + wave; r < rows; r += NORM_BLOCKS * 4)
+        for (int c = lane; c < cols; c += 64) {
+            float u = load_as_f32(it.src, (int64_t)r * it.lds + c, dtype);
+            if (mo.on) {
+                u *= mo.grad_scale;
+                float* q = it.mom + (int64_t)r * it.ldm + c;
+                const float m = fmaf(mo.mu, *q, u);
+                *q = m;
+                u = mo.nesterov ? fmaf(mo.mu, m, u) : m;
+            }
+            s += (double)u * (double)u;
+        }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    __shared__ double ws[4];
+    if (lane == 0) ws[wave] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) part[blockIdx.y * NORM_BLOCKS + blockIdx.x] = (ws[0] + ws[1]) + (ws[2] + ws[3]);
+}
+
+// X_0 2^sx = U 2^sx / (|U| + eps) into the padded two-number layout
+__global__ __launch_bounds__(256) void normalise_kernel(Batch b, int rows, int cols, int rp, int cp, int dtype, Momentum mo,
+                                                        const double* __restrict__ part, float eps, float scale, int split,
+                                                        short* __restrict__ X, int64_t x_elems) {
+    const Item& it = b.it[blockIdx.y];
+    double s = part[blockIdx.y * NORM_BLOCKS + (threadIdx.x & 63)];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    const float inv = (float)((double)scale / (sqrt(s) + (double)eps));
+    short* x = X + blockIdx.y * x_elems;
+    const int cpr = cp / 8;
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < (int64_t)rp * cpr; t += (int64_t)gridDim.x * 256) {
+        const int r = (int)(t / cpr), c = (int)(t - (int64_t)r * cpr) * 8;
+        s16x8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float u = 0.f;
+            if (r < rows && c + e < cols) {
+                u = load_as_f32(it.src, (int64_t)r * it.lds + c + e, dtype);
+                if (mo.on) {
+                    const float m = it.mom[(int64_t)r * it.ldm + c + e];
+                    u = mo.nesterov ? fmaf(mo.mu, m, u * mo.grad_scale) : m;
+                }
+                u *= inv;
+            }
+            short h, l;
+            split16(u, h, l);
+            hi[e] = h;
+            lo[e] = l;
+        }
+        short* d = x + (split ? (int64_t)r * cp * 2 + split_col(c) : (int64_t)r * cp + c);
+        *reinterpret_cast<s16x8*>(d) = hi;
+        if (split) *reinterpret_cast<s16x8*>(d + 16) = lo;
+    }
+}
+
+// One product of a step for a batch of matrices: out = alpha P Q^T + beta R.
+struct StepArgs {
+    View P, Q;
+    int64_t strideP, strideQ, strideR, strideO;   // 16-bit elements between the batch's matrices
+    const short* R;                // stored like the operands, [i][j]; nullable
+    int64_t ldr;
+    float alpha, beta;
+    int I, J, kt;
+    Map map;
+    short* out; int64_t ldo; int out_split;       // inner products
+    // last product of the last step
+    Batch b; int dtype;
+    float lr, decay, scale;        // update: p <- p (1 - lr decay) - lr scale out
+    const capdec_train_state* st;  // nullable: lr is read from it
+};
+enum { INNER = 0, RESULT = 1, UPDATE = 2 };
+
+template <class C, bool TP, bool TQ, bool SPLIT, int OUT>
+__global__ __launch_bounds__(256, 2) void step_kernel(StepArgs a) {
+    extern __shared__ __attribute__((aligned(16))) short lds[];
+    int ti_, tj_, z;
+    if (!tile_of(a.map, blockIdx.x, ti_, tj_, z)) return;
+    const int i0 = ti_ * C::BI, j0 = tj_ * C::BJ;
+    View P = a.P, Q = a.Q;
+    P.p += z * a.strideP;
+    Q.p += z * a.strideQ;
+    f32x16 acc[C::TI][C::TJ];
+    contract<C, F16, TP, TQ, SPLIT>(P, Q, i0, j0, 0, a.kt, lds, acc);
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, wave = tid >> 6, wi = wave >> 1, wj = wave & 1, h = lane >> 5;
+    const short* R = a.R ? a.R + z * a.strideR : nullptr;
+    float lr = a.lr;
+    if (OUT == UPDATE && a.st) lr = a.st->lr;
+#pragma unroll
+    for (int tj = 0; tj < C::TJ; ++tj) {
+        const int j = j0 + (wj * C::TJ + tj) * 32 + (lane & 31);
+        if (j >= a.J) continue;
+        const int64_t js = SPLIT ? split_col(j) : j;
+        const int64_t jo = a.out_split ? split_col(j) : j;
+#pragma unroll
+        for (int ti = 0; ti < C::TI; ++ti) {
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int i = i0 + (wi * C::TI + ti) * 32 + acc_row(e, h);
+                v[e] = a.alpha * acc[ti][tj][e];
+                if (R && i < a.I) {
+                    const short* q = R + (int64_t)i * a.ldr + js;
+                    float x = from_bits<F16>(q[0]);
+                    if (SPLIT) x += from_bits<F16>(q[16]);
+                    v[e] = fmaf(a.beta, x, v[e]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int i = i0 + (wi * C::TI + ti) * 32 + acc_row(e, h);
+                if (i >= a.I) continue;
+                if (OUT == INNER) {
+                    short* d = a.out + z * a.strideO + (int64_t)i * a.ldo + jo;
+                    short p, r;
+                    split16(v[e], p, r);
+                    d[0] = p;
+                    if (a.out_split) d[16] = r;
+                } else {
+                    const Item& it = a.b.it[z];
+                    const int64_t at = (int64_t)i * it.ldd + j;
+                    if (OUT == RESULT) {
+                        store_as(it.dst, at, v[e], a.dtype);
+                    } else {
+                        float* p = (float*)it.dst + at;
+                        *p = fmaf(-lr * a.scale, v[e], *p * (1.f - lr * a.decay));
+                    }
+                }
+            }
+        }
+    }
+}
+
+template <class C, bool TP, bool TQ, bool SPLIT, int OUT>
+int launch(const StepArgs& a0, int nz, hipStream_t s) {
+    StepArgs a = a0;
+    const unsigned grid = make_map(a.map, (a.I + C::BI - 1) / C::BI, (a.J + C::BJ - 1) / C::BJ, nz);
+    if (C::LDS_BYTES > 64 * 1024)
+        CAPDEC_TRY((int)hipFuncSetAttribute(reinterpret_cast<const void*>(step_kernel<C, TP, TQ, SPLIT, OUT>),
+                                            hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS_BYTES));
+    step_kernel<C, TP, TQ, SPLIT, OUT><<<grid, 256, C::LDS_BYTES, s>>>(a);
+    CAPDEC_LAUNCH_CHECK();
+    return 0;
+}
+
+// 256x128 tiles when they give every CU one, else 128x128, else 64x64
+template <bool TP, bool TQ, bool SPLIT, int OUT>
+int launch_sized(const StepArgs& a, int nz, hipStream_t s) {
+    auto tiles = [&](int bi, int bj) { return (int64_t)((a.I + bi - 1) / bi) * ((a.J + bj - 1) / bj) * nz; };
+    if (tiles(256, 128) >= 256) return launch<Big, TP, TQ, SPLIT, OUT>(a, nz, s);
+    if (tiles(128, 128) >= 256) return launch<Mid, TP, TQ, SPLIT, OUT>(a, nz, s);
+    return launch<Small, TP, TQ, SPLIT, OUT>(a, nz, s);
+}
+template <bool TP, bool TQ, int OUT>
+int launch_split(const StepArgs& a, bool split, int nz, hipStream_t s) {
+    return split ? launch_sized<TP, TQ, true, OUT>(a, nz, s) : launch_sized<TP, TQ, false, OUT>(a, nz, s);
+}
+
+// Largest |p(x)| on [0, top] of a x + b x^3 + c x^5 (odd) or b x + c x^2: ends and stationary points.
+double top_of_step(double a, double b, double c, double top) {
+    auto f = [&](double x) { return fabs(x * (a + x * x * (b + x * x * c))); };
+    double best = f(top);
+    auto root = [&](double y) {                   // y = x^2 of a stationary point: a + 3 b y + 5 c y^2 = 0
+        if (y > 0 && y < top * top) best = fmax(best, f(sqrt(y)));
+    };
+    if (c != 0) {
+        const double q = 9 * b * b - 20 * a * c;
+        if (q >= 0) {
+            root((-3 * b + sqrt(q)) / (10 * c));
+            root((-3 * b - sqrt(q)) / (10 * c));
+        }
+    } else if (b != 0) {
+        root(-a / (3 * b));
+    }
+    return best;
+}
+double top_of_poly(double b, double c, double top) {
+    double best = fabs(top * (b + c * top));
+    if (c != 0) {
+        const double x = -b / (2 * c);
+        if (x > 0 && x < top) best = fmax(best, fabs(x * (b + c * x)));
+    }
+    return best;
+}
+// power of two that brings values up to `top` below 2^15 (fp16 ends at 65504), with room for rounding
+int exponent_for(double top) {
+    if (!(top > 0)) return 14;
+    int e;
+    frexp(top * 1.01, &e);                        // top < 2^e
+    return 15 - e;
+}
+
+struct Iteration {
+    int steps, exact_steps;                       // the first exact_steps keep two numbers per value
+    float a, b, c, eps;
+};
+
+int run_batch(const Batch& b, int nz, const Dims& d, const Iteration& n, int dtype, const Momentum& mo, char* ws,
+              const StepArgs& last, hipStream_t s) {
+    double* part = (double*)ws;
+    short* X[2];
+    X[0] = (short*)(ws + ((d.norm + 255) & ~(size_t)255));
+    X[1] = X[0] + (size_t)d.batch * d.x_elems;
+    short* A = X[1] + (size_t)d.batch * d.x_elems;
+    short* B = A + (size_t)d.batch * d.a_elems;
+    double sigma = 1.0;                           // bound of the iterate's singular values
+    int sx = exponent_for(sigma);
+    bool split = n.exact_steps > 0;
+    norm_kernel<<<dim3(NORM_BLOCKS, nz), 256, 0, s>>>(b, d.rows, d.cols, dtype, mo, part);
+    const int64_t items = (int64_t)d.rp * (d.cp / 8);
+    const unsigned blocks = (unsigned)(items / 256 + 1 < 1024 ? items / 256 + 1 : 1024);
+    normalise_kernel<<<dim3(blocks, nz), 256, 0, s>>>(b, d.rows, d.cols, d.rp, d.cp, dtype, mo, part, n.eps, ldexpf(1.f, sx),
+                                                      split, X[0], (int64_t)d.x_elems);
+    CAPDEC_LAUNCH_CHECK();
+    for (int k = 0; k < n.steps; ++k) {
+        const int pl = split ? 2 : 1, kdiv = split ? 16 : 32;
+        const double lambda = sigma * sigma;
+        const int sa = exponent_for(lambda), sb = exponent_for(top_of_poly(n.b, n.c, lambda));
+        const int64_t ldx = (int64_t)d.cp * pl, lda = (int64_t)d.m * pl;
+        StepArgs g{};
+        g.strideP = g.strideQ = (int64_t)d.x_elems;
+        g.P = g.Q = View{X[k & 1], ldx, d.m, d.rp};
+        g.alpha = ldexpf(1.f, sa - 2 * sx);
+        g.I = g.J = d.m; g.kt = (d.tall ? d.rp : d.cp) / kdiv;
+        g.out = A; g.ldo = lda; g.out_split = split; g.strideO = (int64_t)d.a_elems;
+        if (d.tall) CAPDEC_TRY((launch_split<true, true, INNER>(g, split, nz, s)));
+        else CAPDEC_TRY((launch_split<false, false, INNER>(g, split, nz, s)));
+
+        g.strideP = g.strideQ = g.strideR = (int64_t)d.a_elems;
+        g.P = g.Q = View{A, lda, d.m, d.m};
+        g.R = A; g.ldr = lda;
+        g.alpha = (float)ldexp((double)n.c, sb - 2 * sa);
+        g.beta = (float)ldexp((double)n.b, sb - sa);
+        g.kt = d.m / kdiv;
+        g.out = B;
+        CAPDEC_TRY((launch_split<false, false, INNER>(g, split, nz, s)));
+
+        const bool end = k + 1 == n.steps;
+        const double next = top_of_step(n.a, n.b, n.c, sigma);
+        const int sn = end ? 0 : exponent_for(next);
+        const bool next_split = k + 1 < n.exact_steps;
+        StepArgs h = end ? last : StepArgs{};
+        h.b = b;
+        const View vx{X[k & 1], ldx, d.cp, d.rp}, vb{B, lda, d.m, d.m};
+        h.alpha = ldexpf(1.f, sn - sb - sx);
+        h.beta = (float)ldexp((double)n.a, sn - sx);
+        h.R = X[k & 1]; h.ldr = ldx; h.strideR = (int64_t)d.x_elems;
+        h.I = end ? d.rows : d.rp;
+        h.J = end ? d.cols : d.cp;
+        h.kt = d.m / kdiv;
+        h.out = X[~k & 1]; h.ldo = (int64_t)d.cp * (next_split ? 2 : 1); h.out_split = next_split; h.strideO = (int64_t)d.x_elems;
+        if (d.tall) {
+            h.P = View{X[k & 1], ldx, d.rp, d.rp}; h.strideP = (int64_t)d.x_elems;
+            h.Q = vb; h.strideQ = (int64_t)d.a_elems;
+            if (!end) CAPDEC_TRY((launch_split<false, false, INNER>(h, split, nz, s)));
+            else if (mo.on) CAPDEC_TRY((launch_split<false, false, UPDATE>(h, split, nz, s)));
+            else CAPDEC_TRY((launch_split<false, false, RESULT>(h, split, nz, s)));
+        } else {
+            h.P = vb; h.strideP = (int64_t)d.a_elems;
+            h.Q = vx; h.strideQ = (int64_t)d.x_elems;
+            if (!end) CAPDEC_TRY((launch_split<false, true, INNER>(h, split, nz, s)));
+            else if (mo.on) CAPDEC_TRY((launch_split<false, true, UPDATE>(h, split, nz, s)));
+            else CAPDEC_TRY((launch_split<false, true, RESULT>(h, split, nz, s)));
+        }
+        sigma = next;
+        sx = sn;
+        split = next_split;
+    }
+    return 0;
+}
+
+// the iterate's bound must leave the powers of two in fp32's and fp16's range
+bool iteration_fits(const float* coeffs, int steps) {
+    if (!coeffs || steps < 1 || steps > 32) return false;
+    double sigma = 1.0;
+    for (int k = 0; k < 3; ++k)
+        if (!(fabs((double)coeffs[k]) <= 1e3)) return false;
+    for (int k = 0; k < steps; ++k) {
+        sigma = top_of_step(coeffs[0], coeffs[1], coeffs[2], sigma);
+        if (!(sigma <= 64.0)) return false;
+    }
+    return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t capdec_orthogonalize_workspace_bytes(int count, int rows, int cols) {
+    Dims d;
+    if (!make_dims(count, rows, cols, d)) return 0;
+    return ((d.norm + 255) & ~(size_t)255) + d.per * d.batch;
+}
+
+int capdec_orthogonalize(const capdec_matrix* mats, int count, int rows, int cols, int dtype, int steps, const float* coeffs,
+                         float eps, void* workspace, size_t workspace_bytes, void* stream) {
+    Dims d;
+    CAPDEC_REQUIRE(mats && make_dims(count, rows, cols, d) && dtype >= 0 && dtype <= 2 && iteration_fits(coeffs, steps));
+    CAPDEC_REQUIRE(workspace && eps >= 0.f);
+    for (int k = 0; k < count; ++k)
+        CAPDEC_REQUIRE(mats[k].src && mats[k].dst && (rows == 1 || (mats[k].ld_src >= cols && mats[k].ld_dst >= cols)));
+    if (!capdec_aligned16(workspace)) return CAPDEC_EALIGN;
+    if (workspace_bytes < capdec_orthogonalize_workspace_bytes(count, rows, cols)) return CAPDEC_ENOMEM;
+    const Iteration n{steps, steps, coeffs[0], coeffs[1], coeffs[2], eps};
+    for (int k = 0; k < count; k += d.batch) {
+        const int nz = count - k < d.batch ? count - k : d.batch;
+        Batch b{};
+        for (int e = 0; e < nz; ++e)
+            b.it[e] = Item{mats[k + e].src, mats[k + e].dst, nullptr, mats[k + e].ld_src, mats[k + e].ld_dst, 0};
+        StepArgs last{};
+        last.dtype = dtype;
+        CAPDEC_TRY(run_batch(b, nz, d, n, dtype, Momentum{}, (char*)workspace, last, (hipStream_t)stream));
+    }
+    return 0;
+}
+
+int capdec_muon_step(const capdec_muon_param* params, int count, int rows, int cols, float lr, const capdec_train_state* st,
+                     float momentum, int nesterov, float weight_decay, float update_scale, float grad_scale, int steps,
+                     const float* coeffs, float eps, void* workspace, size_t workspace_bytes, void* stream) {
+    Dims d;
+    CAPDEC_REQUIRE(params && make_dims(count, rows, cols, d) && iteration_fits(coeffs, steps));
+    CAPDEC_REQUIRE(workspace && eps >= 0.f);
+    for (int k = 0; k < count; ++k) {
+        const capdec_muon_param& q = params[k];
+        CAPDEC_REQUIRE(q.p && q.g && q.m && (rows == 1 || (q.ldp >= cols && q.ldg >= cols && q.ldm >= cols)));
+    }
+    if (!capdec_aligned16(workspace)) return CAPDEC_EALIGN;
+    if (workspace_bytes < capdec_orthogonalize_workspace_bytes(count, rows, cols)) return CAPDEC_ENOMEM;
+    const Iteration n{steps, steps, coeffs[0], coeffs[1], coeffs[2], eps};
+    const Momentum mo{1, nesterov, momentum, grad_scale};
+    for (int k = 0; k < count; k += d.batch) {
+        const int nz = count - k < d.batch ? count - k : d.batch;
+        Batch b{};
+        for (int e = 0; e < nz; ++e) {
+            const capdec_muon_param& q = params[k + e];
+            b.it[e] = Item{q.g, q.p, q.m, q.ldg, q.ldp, q.ldm};
+        }
+        StepArgs last{};
+        last.lr = lr; last.st = st; last.decay = weight_decay; last.scale = update_scale;
+        CAPDEC_TRY(run_batch(b, nz, d, n, CAPDEC_F32, mo, (char*)workspace, last, (hipStream_t)stream));
+    }
+    return 0;
+}
+
+}  // extern "C"

@@ -1,0 +1,853 @@
+// Softmax cross entropy of a vocabulary projection without keeping the logits, and its gradients.
+//
+//   z = x W^T + b;  nll_r = log(sum_v exp z_rv) - z_rt;  G_rv = (exp(z_rv - lse_r) - [v = t_r]) g_r
+//   dx = G W,  dW = G^T x,  db = sum_r G_r
+//
+// Forward: rows with a counted target are compacted, the product runs tile by tile on the matrix cores and each tile
+// leaves (max, sum of exp) per row.  Backward: G is rebuilt for one piece of the vocabulary at a time from x, W and the
+// rows' log-sum-exp, and contracted with W and x while it is in the caches.  Four products of 2 M V K flops in all for
+// loss and gradients, bound by the matrix cores at large sizes and by reading W at few rows.
+// fp32 operands are split into two fp16 numbers (mma16.h); 16-bit operands are multiplied as they are.  Sums, softmax
+// statistics and the partial sums of the gradients are fp32.  G takes the operands' 16-bit type (scaled by 2^14, so
+// that probabilities down to 2^-28 stay normal in fp16): its rounding is that of the gradients themselves, and averages
+// out in sums over rows or words.
+// Every sum has a fixed order: results repeat bit for bit.
+#include "mma16.h"
+#include <math.h>
+
+using namespace mma16;
+
+namespace {
+
+constexpr float L2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr int G_EXP = 14;                        // G is stored times 2^14
+constexpr size_t PIECE_BYTES = (size_t)512 << 20;
+
+// ---- memory plan (host and device agree through it) ------------------------------------------------------------------
+struct Plan {
+    int M, V, K, Mp, Vp, Kp, split, elt;         // Mp: rows rounded up to 128, Vp: words to 256, Kp: width to 32
+    int xs;                                      // stored columns of the packed operands: Kp, or 2 Kp when split
+    bool pack_w;
+    int piece, pieces;                           // vocabulary words per piece (a multiple of 256)
+    int sx, sw;                                  // contraction splits of dx and dW
+    size_t o_order, o_slot, o_tgt, o_lse, o_dlt, o_b2, o_x, o_w, saved;
+    size_t o_part, fwd;
+    size_t o_rw, o_g, o_dx, o_dw, o_db, bwd;
+};
+
+size_t take(size_t& at, size_t bytes) {
+    const size_t o = at;
+    at += (bytes + 255) & ~(size_t)255;
+    return o;
+}
+
+int splits_for(int64_t tiles, int kt) {
+    // enough workgroups for two on each of 256 CUs, at least 8 k-tiles each
+    int s = 1;
+    while (s < 16 && tiles * (s + 1) <= 512 && kt / (s + 1) >= 8) ++s;
+    return s;
+}
+
+bool make_plan(const capdec_vocab_ce* a, Plan& p) {
+    if (!a || a->M < 1 || a->V < 1 || a->K < 1 || a->dtype < 0 || a->dtype > 2) return false;
+    if (a->M > (1 << 24) || a->V > (1 << 24) || a->K > (1 << 20)) return false;
+    p = Plan{};
+    p.M = a->M; p.V = a->V; p.K = a->K;
+    p.Mp = (a->M + 127) / 128 * 128;
+    p.Vp = (a->V + 255) / 256 * 256;
+    p.Kp = (a->K + 31) / 32 * 32;
+    p.split = a->dtype == CAPDEC_F32;
+    p.elt = a->dtype == CAPDEC_BF16 ? BF16 : F16;
+    p.xs = p.Kp * (p.split ? 2 : 1);
+    // 16-bit weights are read where they are when their rows are made of whole k-tiles of aligned vectors
+    p.pack_w = p.split || a->K % 32 != 0 || a->ldw % 8 != 0 || !capdec_aligned16(a->W);
+    size_t at = 256;
+    p.o_order = take(at, (size_t)p.M * 4);
+    p.o_slot = take(at, (size_t)p.M * 4);
+    p.o_tgt = take(at, (size_t)p.Mp * 4);
+    p.o_lse = take(at, (size_t)p.Mp * 4);
+    p.o_dlt = take(at, (size_t)p.Mp * 4);
+    p.o_b2 = take(at, (size_t)p.Vp * 4);
+    p.o_x = take(at, (size_t)p.Mp * p.xs * 2);
+    p.o_w = p.pack_w ? take(at, (size_t)p.V * p.xs * 2) : 0;
+    p.saved = at;
+
+    at = 256;
+    p.o_part = take(at, (size_t)(p.Vp / 256) * p.Mp * 8);
+    p.fwd = at;
+
+    const int es = p.split ? 4 : 2;
+    int64_t most = (int64_t)(PIECE_BYTES / ((size_t)p.Mp * es)) / 256 * 256;
+    if (most < 256) most = 256;
+    p.pieces = (int)((p.Vp + most - 1) / most);
+    p.piece = ((p.Vp + p.pieces - 1) / p.pieces + 255) / 256 * 256;
+    p.pieces = (p.Vp + p.piece - 1) / p.piece;
+    const int kt = p.split ? 16 : 32;
+    p.sx = splits_for((int64_t)((p.M + 255) / 256) * ((p.Kp + 127) / 128), p.piece / kt);
+    p.sw = splits_for((int64_t)(p.piece / 256) * ((p.Kp + 127) / 128), p.Mp / kt);
+    at = 256;
+    p.o_rw = take(at, (size_t)p.Mp * 4);
+    p.o_g = take(at, (size_t)p.Mp * p.piece * es);
+    p.o_dx = take(at, (size_t)p.sx * p.Mp * p.Kp * 4);
+    p.o_dw = p.sw > 1 ? take(at, (size_t)p.sw * p.piece * p.Kp * 4) : 0;
+    p.o_db = a->bias ? take(at, (size_t)(p.Mp / 128) * p.piece * 4) : 0;
+    p.bwd = at;
+    return true;
+}
+
+struct Head {               // first 256 bytes of the saved buffer
+    int count;              // rows with a counted target
+    unsigned amax_x, amax_w;   // bits of the largest finite magnitude (split operands)
+};
+struct BwdHead {            // first 256 bytes of the backward workspace
+    float factor;           // what dx, dW and db are to be multiplied by
+};
+
+// power of two that brings amax to [2^14, 2^15); the operands' scales are undone in fp32
+__device__ __forceinline__ int scale_exp(unsigned amax_bits) {
+    const int e = (int)(amax_bits >> 23) - 127;        // floor(log2), denormals count as 2^-127
+    if (amax_bits == 0) return 0;
+    return min(14 - e, 60);
+}
+__device__ __forceinline__ float pow2(int e) { return ldexpf(1.f, e); }
+
+// ---- rows with a counted target -------------------------------------------------------------------------------------
+// One workgroup: stable compaction, 4096 targets per round.
+__global__ __launch_bounds__(1024) void compact_kernel(const int64_t* __restrict__ targets, int M, int V, int64_t ignore,
+                                                       Head* __restrict__ head, int* __restrict__ order,
+                                                       int* __restrict__ slot, int* __restrict__ tgt) {
+    __shared__ int wsum[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int done = 0;
+    for (int base = 0; base < M; base += 4096) {
+        int64_t t[4];
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = base + threadIdx.x * 4 + k;
+            t[k] = r < M ? targets[r] : ignore;
+            n += t[k] != ignore;
+        }
+        int pre = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(pre, o, 64);
+            if (lane >= o) pre += v;
+        }
+        if (lane == 63) wsum[wave] = pre;
+        __syncthreads();
+        int before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            if (w < wave) before += wsum[w];
+            all += wsum[w];
+        }
+        int s = done + before + pre - n;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = base + threadIdx.x * 4 + k;
+            if (r >= M) break;
+            if (t[k] != ignore) {
+                order[s] = r;
+                tgt[s] = (t[k] >= 0 && t[k] < V) ? (int)t[k] : -1;    // -1: outside the vocabulary, the row's loss is NaN
+                slot[r] = s++;
+            } else {
+                slot[r] = -1;
+            }
+        }
+        done += all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        head->count = done;
+        head->amax_x = head->amax_w = 0;
+    }
+}
+
+__device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int dtype) {
+    if (dtype == CAPDEC_F32) return ((const float*)p)[i];
+    const short b = ((const short*)p)[i];
+    return dtype == CAPDEC_BF16 ? from_bits<BF16>(b) : from_bits<F16>(b);
+}
+
+// largest finite magnitude of x (counted rows) and W; blockIdx.y picks the operand.  atomicMax of non-negative floats'
+// bits: the order does not matter.
+__global__ __launch_bounds__(256) void amax_kernel(const float* __restrict__ x, int64_t ldx, const float* __restrict__ W,
+                                                   int64_t ldw, int V, int K, Head* __restrict__ head,
+                                                   const int* __restrict__ order, int vec) {
+    const bool isw = blockIdx.y != 0;
+    const int rows = isw ? V : head->count;
+    float m = 0.f;
+    const int wave = (blockIdx.x * 256 + threadIdx.x) >> 6, nw = gridDim.x * 4, lane = threadIdx.x & 63;
+    auto see = [&](float v) {
+        v = fabsf(v);
+        if (v < INFINITY) m = fmaxf(m, v);
+    };
+    for (int r = wave; r < rows; r += nw) {
+        const float* row = isw ? W + (int64_t)r * ldw : x + (int64_t)order[r] * ldx;
+        if (vec) {
+            for (int c = lane * 4; c < K; c += 256) {
+                const f32x4 v = *reinterpret_cast<const f32x4*>(row + c);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) see(v[e]);
+            }
+        } else {
+            for (int c = lane; c < K; c += 64) see(row[c]);
+        }
+    }
+    m = wave_max(m);
+    __shared__ float wm[4];
+    if (lane == 0) wm[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        m = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+        if (m > 0.f) atomicMax(isw ? &head->amax_w : &head->amax_x, __float_as_uint(m));
+    }
+}
+
+// Packed operands: rows of whole k-tiles, zero beyond the width; x by slot (zero rows up to the next multiple of 32
+// behind the last), W by word, and the bias times log2(e) with -inf behind the vocabulary.  A thread makes 8 columns.
+struct PackArgs {
+    const void* x; int64_t ldx;
+    const void* W; int64_t ldw;
+    const void* bias;
+    int M, V, K, Kp, xs, dtype, split, Vp, pack_w, vec;
+    Head* head;
+    const int* order;
+    short* px; short* pw; float* b2;
+    int64_t nx, nw;           // 8-column chunks of x and W
+};
+__global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
+    const int64_t total = a.nx + a.nw + a.Vp;
+    const int cpr = a.Kp / 8;
+    const int count = a.head->count;
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+        if (t >= a.nx + a.nw) {
+            const int v = (int)(t - a.nx - a.nw);
+            a.b2[v] = v >= a.V ? -INFINITY : a.bias ? load_as_f32(a.bias, v, a.dtype) * L2E : 0.f;
+            continue;
+        }
+        const bool isw = t >= a.nx;
+        const int64_t u = isw ? t - a.nx : t;
+        const int row = (int)(u / cpr), c = (int)(u - (int64_t)row * cpr) * 8;
+        if (!isw && row >= ((count + 31) & ~31)) continue;
+        const bool zero = !isw && row >= count;
+        const int64_t base = isw ? (int64_t)row * a.ldw : zero ? 0 : (int64_t)a.order[row] * a.ldx;
+        const void* src = isw ? a.W : a.x;
+        short* dst = (isw ? a.pw : a.px) + (int64_t)row * a.xs;
+        if (!a.split) {
+            s16x8 o;
+            if (!zero && a.vec && c + 8 <= a.K) {
+                o = *reinterpret_cast<const s16x8*>((const short*)src + base + c);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = (!zero && c + e < a.K) ? ((const short*)src)[base + c + e] : (short)0;
+            }
+            *reinterpret_cast<s16x8*>(dst + c) = o;
+        } else {
+            const float s = pow2(scale_exp(isw ? a.head->amax_w : a.head->amax_x));
+            float v[8];
+            if (!zero && a.vec && c + 8 <= a.K) {
+                const f32x4* q = reinterpret_cast<const f32x4*>((const float*)src + base + c);
+                const f32x4 p0 = q[0], p1 = q[1];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = p0[e], v[4 + e] = p1[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = (!zero && c + e < a.K) ? ((const float*)src)[base + c + e] : 0.f;
+            }
+            s16x8 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                short h, l;
+                split16(v[e] * s, h, l);
+                hi[e] = h;
+                lo[e] = l;
+            }
+            short* d = dst + split_col(c);
+            *reinterpret_cast<s16x8*>(d) = hi;
+            *reinterpret_cast<s16x8*>(d + 16) = lo;
+        }
+    }
+}
+
+// ---- (max, sum of exp) of every row over each tile of 256 words; values in units of log 2 ---------------------------
+struct LogitArgs {
+    View W, X;
+    const float* b2;
+    const Head* head;
+    int kt, Mp;
+    Map map;
+    float2* part;                                // forward: [tile][slot]
+    // dlogits
+    const float *lse, *dlt, *rw;
+    const int* tgt;
+    short* g; int64_t ldg;                       // [slot][word of the piece]
+    float* dbp;                                  // [row tile][word of the piece], nullable
+    int v0, piece;
+};
+
+template <bool SPLIT>
+__device__ __forceinline__ float logit_scale(const Head* head) {
+    return SPLIT ? pow2(-scale_exp(head->amax_x)) * pow2(-scale_exp(head->amax_w)) * L2E : L2E;
+}
+
+template <class C, int ELT, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void lse_kernel(LogitArgs a) {
+    extern __shared__ __attribute__((aligned(16))) short lds[];
+    int ti_, tj_, z;
+    if (!tile_of(a.map, blockIdx.x, ti_, tj_, z)) return;
+    const int count = a.head->count;
+    const int i0 = ti_ * C::BI, j0 = tj_ * C::BJ;
+    if (j0 >= count) return;
+    f32x16 acc[C::TI][C::TJ];
+    contract<C, ELT, false, false, SPLIT>(a.W, a.X, i0, j0, 0, a.kt, lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave >> 1, wj = wave & 1, h = lane >> 5;
+    const float c1 = logit_scale<SPLIT>(a.head);
+    float2* red = reinterpret_cast<float2*>(lds);
+#pragma unroll
+    for (int tj = 0; tj < C::TJ; ++tj) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int ti = 0; ti < C::TI; ++ti)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 b = *reinterpret_cast<const f32x4*>(a.b2 + i0 + (wi * C::TI + ti) * 32 + 8 * q + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float v = fmaf(acc[ti][tj][4 * q + e], c1, b[e]);
+                    acc[ti][tj][4 * q + e] = v;
+                    m = fmaxf(m, v);
+                }
+            }
+        const float m0 = m == -INFINITY ? 0.f : m;          // a tile whose words are all masked by the bias
+        float s = 0.f;
+#pragma unroll
+        for (int ti = 0; ti < C::TI; ++ti)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(acc[ti][tj][e] - m0);
+        // the other half of the words, then the other pair of wavefronts
+        const float mo = __shfl_xor(m, 32, 64), so = __shfl_xor(s, 32, 64);
+        const float mm = fmaxf(m, mo), mz = mm == -INFINITY ? 0.f : mm;
+        s = s * __builtin_amdgcn_exp2f(m - mz) + so * __builtin_amdgcn_exp2f(mo - mz);
+        if (h == 0) red[wi * C::BJ + (wj * C::TJ + tj) * 32 + lane] = make_float2(mm, s);
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < C::BJ; j += 256) {
+        const float2 u = red[j], v = red[C::BJ + j];
+        const float mm = fmaxf(u.x, v.x), mz = mm == -INFINITY ? 0.f : mm;
+        a.part[(int64_t)ti_ * a.Mp + j0 + j] =
+            make_float2(mm, u.y * __builtin_amdgcn_exp2f(u.x - mz) + v.y * __builtin_amdgcn_exp2f(v.x - mz));
+    }
+}
+
+// Per slot: the tiles' statistics joined, the target's logit (a dot product of the original operands), and the loss.
+// A wavefront per row of the batch; rows that are not counted get loss 0.
+__global__ __launch_bounds__(256) void nll_kernel(const float2* __restrict__ part, int ntiles, int Mp, const void* x,
+                                                  int64_t ldx, const void* W, int64_t ldw, const void* bias, int dtype,
+                                                  int M, int K, const int* __restrict__ slot, const int* __restrict__ tgt,
+                                                  float* __restrict__ lse, float* __restrict__ dlt, float* __restrict__ nll) {
+    const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (r >= M) return;
+    const int s = slot[r];
+    if (s < 0) {
+        if (lane == 0) nll[r] = 0.f;
+        return;
+    }
+    float m = -INFINITY, sum = 0.f;
+    for (int t = lane; t < ntiles; t += 64) {
+        const float2 v = part[(int64_t)t * Mp + s];
+        const float mm = fmaxf(m, v.x), mz = mm == -INFINITY ? 0.f : mm;
+        sum = sum * __builtin_amdgcn_exp2f(m - mz) + v.y * __builtin_amdgcn_exp2f(v.x - mz);
+        m = mm;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const float mo = __shfl_xor(m, o, 64), so = __shfl_xor(sum, o, 64);
+        const float mm = fmaxf(m, mo), mz = mm == -INFINITY ? 0.f : mm;
+        sum = sum * __builtin_amdgcn_exp2f(m - mz) + so * __builtin_amdgcn_exp2f(mo - mz);
+        m = mm;
+    }
+    const int t = tgt[s];
+    float dot = 0.f;
+    if (t >= 0)
+        for (int c = lane; c < K; c += 64)
+            dot = fmaf(load_as_f32(x, (int64_t)r * ldx + c, dtype), load_as_f32(W, (int64_t)t * ldw + c, dtype), dot);
+    dot = wave_sum(dot);
+    if (lane == 0) {
+        const float l2 = t >= 0 ? m + __log2f(sum) : NAN;
+        const float zt = t < 0 ? NAN : dot + (bias ? load_as_f32(bias, t, dtype) : 0.f);
+        const float d = fmaf(-l2, LN2, zt);            // log of the target's probability
+        lse[s] = l2;
+        dlt[s] = d;
+        nll[r] = -d;
+    }
+}
+
+// loss[0] = mean over the counted rows, loss[1] = sum, loss[2] = number of counted rows; one workgroup, fixed order
+__global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ nll, int M, const Head* __restrict__ head,
+                                                    float* __restrict__ loss) {
+    double s = 0.0;
+    for (int r = threadIdx.x; r < M; r += 1024) s += (double)nll[r];
+    __shared__ double part[16];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = 0.0;
+        for (int w = 0; w < 16; ++w) s += part[w];
+        loss[0] = (float)(s / (double)head->count);    // no counted row: 0 / 0, as torch has it
+        loss[1] = (float)s;
+        loss[2] = (float)head->count;
+    }
+}
+
+// ---- backward -----------------------------------------------------------------------------------------------------
+// What each row of G is multiplied by, brought to [2^13, 2^14] at most by a power of two, and the factor that undoes it.
+// row_grad: the rows' own upstream gradients; else one scalar for all of them (divided by the count when `mean`).
+__global__ __launch_bounds__(1024) void weights_kernel(const float* __restrict__ row_grad, const float* __restrict__ grad,
+                                                       int mean, const Head* __restrict__ head,
+                                                       const int* __restrict__ order, int Mp, float* __restrict__ rw,
+                                                       BwdHead* __restrict__ bh) {
+    const int count = head->count;
+    float scale = pow2(G_EXP);
+    __shared__ float wm[16];
+    if (row_grad) {
+        float m = 0.f;
+        for (int s = threadIdx.x; s < count; s += 1024) {
+            const float v = fabsf(row_grad[order[s]]);
+            if (v < INFINITY) m = fmaxf(m, v);
+        }
+        m = wave_max(m);
+        if ((threadIdx.x & 63) == 0) wm[threadIdx.x >> 6] = m;
+        __syncthreads();
+        m = 0.f;
+        for (int w = 0; w < 16; ++w) m = fmaxf(m, wm[w]);
+        // amax * scale in [2^13, 2^14)
+        const int e = (int)(__float_as_uint(m) >> 23) - 127;
+        scale = m > 0.f ? pow2(min(G_EXP - 1 - e, 126)) : 1.f;
+    }
+    for (int s = threadIdx.x; s < Mp; s += 1024)
+        rw[s] = s >= count ? 0.f : row_grad ? row_grad[order[s]] * scale : scale;
+    if (threadIdx.x == 0) {
+        float f = 1.f / scale;
+        if (!row_grad) f *= grad[0] / (mean ? (float)count : 1.f);
+        bh->factor = count > 0 ? f : 0.f;
+    }
+}
+
+// G of one piece of the vocabulary.  The tile is turned through LDS (a wavefront's 64 rows x 128 words at a time), so
+// that rows are stored 256 contiguous bytes at a time; on the way the targets' entries are put in, (p_t - 1) g as
+// expm1(log p_t) g, and each word's column is summed for the bias gradient.
+template <class C, int ELT, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void dlogits_kernel(LogitArgs a) {
+    extern __shared__ __attribute__((aligned(16))) short lds[];
+    int ti_, tj_, z;
+    if (!tile_of(a.map, blockIdx.x, ti_, tj_, z)) return;
+    const int count = a.head->count;
+    const int i0 = a.v0 + ti_ * C::BI, j0 = tj_ * C::BJ;
+    if (j0 >= count) return;
+    f32x16 acc[C::TI][C::TJ];
+    contract<C, ELT, false, false, SPLIT>(a.W, a.X, i0, j0, 0, a.kt, lds, acc);
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));       // the addresses below are made here, not ahead of the contraction (72 spills)
+    const int lane = tid & 63, wave = tid >> 6, wi = wave >> 1, wj = wave & 1, h = lane >> 5;
+    const float c1 = logit_scale<SPLIT>(a.head);
+    constexpr int WORDS = 32 * C::TI;                     // of a wavefront
+    constexpr int PL = SPLIT ? 2 : 1;
+    constexpr int LD = WORDS * PL + 8;                    // 16-bit elements per row of the turned tile
+    // one 32-row block of the wavefront at a time
+    short* tile = lds + wave * 32 * LD;
+    float* colsum = reinterpret_cast<float*>(lds + 4 * 32 * LD);      // [2 (wj)][BI]
+    float sums[2] = {0.f, 0.f};
+#pragma unroll
+    for (int tj = 0; tj < C::TJ; ++tj) {
+        const int s = j0 + (wj * C::TJ + tj) * 32 + (lane & 31);
+        const bool live = s < count;
+        const float l2 = live ? a.lse[s] : 0.f;
+        const float w = live ? a.rw[s] : 0.f;
+        const float* b2 = a.b2 + i0 + wi * WORDS;
+#pragma unroll
+        for (int ti = 0; ti < C::TI; ++ti) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int wd = ti * 32 + 8 * q + 4 * h;       // word inside the wavefront's range
+                const f32x4 b = *reinterpret_cast<const f32x4*>(b2 + wd);
+                s16x4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float v = __builtin_amdgcn_exp2f(fmaf(acc[ti][tj][4 * q + e], c1, b[e]) - l2) * w;
+                    if (!live) v = 0.f;
+                    if (SPLIT) {
+                        short p, r;
+                        split16(v, p, r);
+                        hi[e] = p;
+                        lo[e] = r;
+                    } else {
+                        hi[e] = to_bits<ELT>(v);
+                    }
+                }
+                short* d = tile + (lane & 31) * LD + (SPLIT ? (int)split_col(wd) : wd);
+                *reinterpret_cast<s16x4*>(d) = hi;
+                if (SPLIT) *reinterpret_cast<s16x4*>(d + 16) = lo;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // (the tile belongs to this wavefront alone: LDS operations of a wavefront complete in order)
+        if (h == 0 && live) {
+            const int t = a.tgt[s] - (i0 + wi * WORDS);
+            if (t >= 0 && t < WORDS) {
+                const float v = expm1f(a.dlt[s]) * w;
+                short* d = tile + lane * LD + (SPLIT ? (int)split_col(t) : t);
+                if (SPLIT) {
+                    short p, r;
+                    split16(v, p, r);
+                    d[0] = p;
+                    d[16] = r;
+                } else {
+                    d[0] = to_bits<ELT>(v);
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        constexpr int CH = WORDS * PL / 8;                     // 16-byte chunks per row
+        constexpr int RPP = 64 / CH;                           // rows per pass
+        static_assert(64 % CH == 0, "row does not divide over the wavefront");
+        const int row0 = j0 + (wj * C::TJ + tj) * 32;
+        short* gp = a.g + (int64_t)(ti_ * C::BI + wi * WORDS) * PL;
+#pragma unroll 4
+        for (int r = lane / CH; r < 32; r += RPP) {
+            const s16x8 v = *reinterpret_cast<const s16x8*>(tile + r * LD + (lane % CH) * 8);
+            *reinterpret_cast<s16x8*>(gp + (int64_t)(row0 + r) * a.ldg + (lane % CH) * 8) = v;
+        }
+        if (a.dbp) {
+#pragma unroll
+            for (int k = 0; k < WORDS / 64; ++k) {
+                const int wd = lane + 64 * k;
+                const short* d = tile + (SPLIT ? (int)split_col(wd) : wd);
+                float sum = 0.f;
+#pragma unroll 8
+                for (int r = 0; r < 32; ++r) {
+                    sum += from_bits<ELT>(d[r * LD]);
+                    if (SPLIT) sum += from_bits<ELT>(d[r * LD + 16]);
+                }
+                sums[k] += sum;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    if (a.dbp) {
+#pragma unroll
+        for (int k = 0; k < WORDS / 64; ++k) colsum[wj * C::BI + wi * WORDS + lane + 64 * k] = sums[k];
+        __syncthreads();
+        for (int i = threadIdx.x; i < C::BI; i += 256)
+            a.dbp[(int64_t)tj_ * a.piece + ti_ * C::BI + i] = colsum[i] + colsum[C::BI + i];
+    }
+}
+
+// dx and dW of one piece.  OUT 0: fp32 partial sums [split][i][j], added onto what earlier pieces left when `add`;
+// OUT 1: times the factor, in the weights' type.
+struct GradArgs {
+    View P, Q;
+    const Head* head;
+    const BwdHead* bh;
+    int I, J;                      // rows and columns stored
+    int rows_live;                 // dx: only the first count rows exist
+    int k_live;                    // dW: the contraction runs over the counted rows; else over kt k-tiles
+    int kt, nsplit;
+    Map map;
+    float* part; int64_t ldp, plane; int add;
+    void* out; int64_t ldo; int dtype;
+};
+__device__ __forceinline__ void store_as(void* p, int64_t i, float v, int dtype) {
+    if (dtype == CAPDEC_F32) ((float*)p)[i] = v;
+    else ((short*)p)[i] = dtype == CAPDEC_BF16 ? to_bits<BF16>(v) : to_bits<F16>(v);
+}
+
+template <class C, int ELT, bool TP, bool SPLIT, int OUT>
+__global__ __launch_bounds__(256, 2) void grad_kernel(GradArgs a) {
+    extern __shared__ __attribute__((aligned(16))) short lds[];
+    int ti_, tj_, z;
+    if (!tile_of(a.map, blockIdx.x, ti_, tj_, z)) return;
+    const int count = a.head->count;
+    const int i0 = ti_ * C::BI, j0 = tj_ * C::BJ;
+    const int nI = a.rows_live ? min(a.I, count) : a.I;
+    if (i0 >= nI) return;
+    constexpr int KT = SPLIT ? 16 : 32;
+    const int kt = a.k_live ? (count + KT - 1) / KT : a.kt;
+    const int per = (kt + a.nsplit - 1) / a.nsplit;
+    f32x16 acc[C::TI][C::TJ];
+    contract<C, ELT, TP, true, SPLIT>(a.P, a.Q, i0, j0, z * per, min(kt, (z + 1) * per), lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave >> 1, wj = wave & 1, h = lane >> 5;
+    float f = 1.f;
+    if (OUT == 1) {
+        f = a.bh->factor;
+        if (SPLIT) f *= pow2(-scale_exp(a.head->amax_x));
+    }
+#pragma unroll
+    for (int tj = 0; tj < C::TJ; ++tj) {
+        const int j = j0 + (wj * C::TJ + tj) * 32 + (lane & 31);
+        if (j >= a.J) continue;
+#pragma unroll
+        for (int ti = 0; ti < C::TI; ++ti)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int i = i0 + (wi * C::TI + ti) * 32 + acc_row(e, h);
+                if (i >= nI) continue;
+                if (OUT == 0) {
+                    float* d = a.part + (int64_t)z * a.plane + (int64_t)i * a.ldp + j;
+                    *d = a.add ? *d + acc[ti][tj][e] : acc[ti][tj][e];
+                } else {
+                    store_as(a.out, (int64_t)i * a.ldo + j, acc[ti][tj][e] * f, a.dtype);
+                }
+            }
+    }
+}
+
+// dx[r] = factor * sum of the partial sums of r's slot; zero for rows that are not counted
+__global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part, int64_t plane, int nsplit, int Kp, int M,
+                                                 int K, const int* __restrict__ slot, const Head* __restrict__ head,
+                                                 const BwdHead* __restrict__ bh, int split, void* out, int64_t ldo, int dtype) {
+    const float f = bh->factor * (split ? pow2(-scale_exp(head->amax_w)) : 1.f);
+    const int cpr = (K + 3) / 4;
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < (int64_t)M * cpr; t += (int64_t)gridDim.x * 256) {
+        const int r = (int)(t / cpr), c = (int)(t - (int64_t)r * cpr) * 4;
+        const int s = slot[r];
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (s >= 0) {
+            for (int k = 0; k < nsplit; ++k) v += *reinterpret_cast<const f32x4*>(part + k * plane + (int64_t)s * Kp + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= f;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < K) store_as(out, (int64_t)r * ldo + c + e, v[e], dtype);
+    }
+}
+
+// dW of one piece from its partial sums, and db from the row tiles' column sums
+__global__ __launch_bounds__(256) void dw_kernel(const float* __restrict__ part, int64_t plane, int nsplit, int Kp, int rows,
+                                                 int K, const Head* __restrict__ head, const BwdHead* __restrict__ bh,
+                                                 int split, void* dW, int64_t ldw, int dtype, const float* __restrict__ dbp,
+                                                 int piece, void* db, int v0) {
+    const float fb = bh->factor;
+    const float f = fb * (split ? pow2(-scale_exp(head->amax_x)) : 1.f);
+    const int cpr = (K + 3) / 4;
+    const int64_t nw = nsplit > 1 ? (int64_t)rows * cpr : 0;
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < nw + (dbp ? rows : 0); t += (int64_t)gridDim.x * 256) {
+        if (t >= nw) {
+            const int v = (int)(t - nw), tiles = (head->count + 127) / 128;
+            float s = 0.f;
+            for (int k = 0; k < tiles; ++k) s += dbp[(int64_t)k * piece + v];
+            store_as(db, v0 + v, s * fb, dtype);
+            continue;
+        }
+        const int r = (int)(t / cpr), c = (int)(t - (int64_t)r * cpr) * 4;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < nsplit; ++k) v += *reinterpret_cast<const f32x4*>(part + k * plane + (int64_t)r * Kp + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < K) store_as(dW, (int64_t)(v0 + r) * ldw + c + e, v[e] * f, dtype);
+    }
+}
+
+unsigned blocks_for(int64_t items, int64_t per, unsigned most) {
+    int64_t b = (items + per - 1) / per;
+    return (unsigned)(b < 1 ? 1 : b > (int64_t)most ? (int64_t)most : b);
+}
+
+template <class K>
+int allow_lds(K kernel, int bytes) {
+    if (bytes <= 64 * 1024) return 0;
+    return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+template <class C, int ELT, bool SPLIT>
+int launch_lse(const LogitArgs& a, unsigned grid, hipStream_t s) {
+    CAPDEC_TRY(allow_lds(lse_kernel<C, ELT, SPLIT>, C::LDS_BYTES));
+    lse_kernel<C, ELT, SPLIT><<<grid, 256, C::LDS_BYTES, s>>>(a);
+    CAPDEC_LAUNCH_CHECK();
+    return 0;
+}
+template <class C, int ELT, bool SPLIT>
+int launch_dlogits(const LogitArgs& a, unsigned grid, hipStream_t s) {
+    constexpr int turned = (4 * 32 * (32 * C::TI * (SPLIT ? 2 : 1) + 8)) * 2 + 2 * C::BI * 4;
+    constexpr int bytes = turned > C::LDS_BYTES ? turned : C::LDS_BYTES;
+    CAPDEC_TRY(allow_lds(dlogits_kernel<C, ELT, SPLIT>, bytes));
+    dlogits_kernel<C, ELT, SPLIT><<<grid, 256, bytes, s>>>(a);
+    CAPDEC_LAUNCH_CHECK();
+    return 0;
+}
+template <class C, int ELT, bool TP, bool SPLIT, int OUT>
+int launch_grad(const GradArgs& a, unsigned grid, hipStream_t s) {
+    CAPDEC_TRY(allow_lds(grad_kernel<C, ELT, TP, SPLIT, OUT>, C::LDS_BYTES));
+    grad_kernel<C, ELT, TP, SPLIT, OUT><<<grid, 256, C::LDS_BYTES, s>>>(a);
+    CAPDEC_LAUNCH_CHECK();
+    return 0;
+}
+
+#define BY_TYPE(p, CALL)                                    \
+    ((p).split ? CALL(F16, true) : (p).elt == BF16 ? CALL(BF16, false) : CALL(F16, false))
+
+bool valid(const capdec_vocab_ce* a) {
+    if (!a || !a->x || !a->W || !a->targets) return false;
+    const bool rows = a->M > 1 ? a->ldx >= a->K : a->ldx >= 0;
+    return rows && (a->V > 1 ? a->ldw >= a->K : a->ldw >= 0);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t capdec_vocab_ce_saved_bytes(const capdec_vocab_ce* a) {
+    Plan p;
+    return make_plan(a, p) ? p.saved : 0;
+}
+size_t capdec_vocab_ce_forward_workspace_bytes(const capdec_vocab_ce* a) {
+    Plan p;
+    return make_plan(a, p) ? p.fwd : 0;
+}
+size_t capdec_vocab_ce_backward_workspace_bytes(const capdec_vocab_ce* a) {
+    Plan p;
+    return make_plan(a, p) ? p.bwd : 0;
+}
+
+int capdec_vocab_ce_forward(const capdec_vocab_ce* a, void* saved, size_t saved_bytes, void* workspace,
+                            size_t workspace_bytes, float* nll, float* loss, void* stream) {
+    Plan p;
+    CAPDEC_REQUIRE(valid(a) && make_plan(a, p) && saved && workspace && nll);
+    if (!capdec_aligned16(saved) || !capdec_aligned16(workspace)) return CAPDEC_EALIGN;
+    if (saved_bytes < p.saved || workspace_bytes < p.fwd) return CAPDEC_ENOMEM;
+    hipStream_t s = (hipStream_t)stream;
+    char* sv = (char*)saved;
+    Head* head = (Head*)sv;
+    int* order = (int*)(sv + p.o_order);
+    int* slot = (int*)(sv + p.o_slot);
+    int* tgt = (int*)(sv + p.o_tgt);
+    compact_kernel<<<1, 1024, 0, s>>>(a->targets, a->M, a->V, a->ignore_index, head, order, slot, tgt);
+    const int esz = p.split ? 4 : 2;
+    const int vec = capdec_aligned16(a->x) && capdec_aligned16(a->W) && a->ldx * esz % 16 == 0 && a->ldw * esz % 16 == 0;
+    if (p.split) {
+        const unsigned bx = blocks_for((int64_t)(p.V > p.M ? p.V : p.M), 4, 2048);
+        amax_kernel<<<dim3(bx, 2), 256, 0, s>>>((const float*)a->x, a->ldx, (const float*)a->W, a->ldw, p.V, p.K, head, order,
+                                                vec && p.K % 4 == 0);
+    }
+    PackArgs k{};
+    k.x = a->x; k.ldx = a->ldx; k.W = a->W; k.ldw = a->ldw; k.bias = a->bias;
+    k.M = p.M; k.V = p.V; k.K = p.K; k.Kp = p.Kp; k.xs = p.xs; k.dtype = a->dtype; k.split = p.split; k.Vp = p.Vp;
+    k.pack_w = p.pack_w; k.vec = vec;
+    k.head = head; k.order = order;
+    k.px = (short*)(sv + p.o_x); k.pw = (short*)(sv + p.o_w); k.b2 = (float*)(sv + p.o_b2);
+    k.nx = (int64_t)p.Mp * (p.Kp / 8);
+    k.nw = p.pack_w ? (int64_t)p.V * (p.Kp / 8) : 0;
+    pack_kernel<<<blocks_for(k.nx + k.nw + p.Vp, 256, 8192), 256, 0, s>>>(k);
+    CAPDEC_LAUNCH_CHECK();
+
+    LogitArgs g{};
+    g.W = View{p.pack_w ? k.pw : (const short*)a->W, p.pack_w ? (int64_t)p.xs : a->ldw, p.V, 0};
+    g.X = View{k.px, (int64_t)p.xs, p.Mp, 0};
+    g.b2 = k.b2; g.head = head; g.kt = p.xs / 32; g.Mp = p.Mp;
+    g.part = (float2*)((char*)workspace + p.o_part);
+    const unsigned grid = make_map(g.map, p.Vp / Big::BI, p.Mp / Big::BJ, 1);
+#define LSE(E, S) launch_lse<Big, E, S>(g, grid, s)
+    CAPDEC_TRY(BY_TYPE(p, LSE));
+#undef LSE
+    nll_kernel<<<(p.M + 3) / 4, 256, 0, s>>>(g.part, p.Vp / 256, p.Mp, a->x, a->ldx, a->W, a->ldw, a->bias, a->dtype, p.M, p.K,
+                                             slot, tgt, (float*)(sv + p.o_lse), (float*)(sv + p.o_dlt), nll);
+    if (loss) loss_kernel<<<1, 1024, 0, s>>>(nll, p.M, head, loss);
+    CAPDEC_LAUNCH_CHECK();
+    return 0;
+}
+
+int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t saved_bytes, void* workspace,
+                             size_t workspace_bytes, const float* row_grad, const float* grad, int mean, void* dx,
+                             int64_t lddx, void* dW, int64_t lddw, void* dbias, void* stream) {
+    Plan p;
+    CAPDEC_REQUIRE(valid(a) && make_plan(a, p) && saved && workspace && (row_grad || grad));
+    CAPDEC_REQUIRE(!dx || p.M == 1 || lddx >= p.K);
+    CAPDEC_REQUIRE(!dW || p.V == 1 || lddw >= p.K);
+    CAPDEC_REQUIRE(!dbias || a->bias);
+    if (!capdec_aligned16(saved) || !capdec_aligned16(workspace)) return CAPDEC_EALIGN;
+    if (saved_bytes < p.saved || workspace_bytes < p.bwd) return CAPDEC_ENOMEM;
+    if (!dx && !dW && !dbias) return 0;
+    hipStream_t s = (hipStream_t)stream;
+    const char* sv = (const char*)saved;
+    char* ws = (char*)workspace;
+    const Head* head = (const Head*)sv;
+    const int* order = (const int*)(sv + p.o_order);
+    const int* slot = (const int*)(sv + p.o_slot);
+    BwdHead* bh = (BwdHead*)ws;
+    float* rw = (float*)(ws + p.o_rw);
+    weights_kernel<<<1, 1024, 0, s>>>(row_grad, grad, mean, head, order, p.Mp, rw, bh);
+    CAPDEC_LAUNCH_CHECK();
+    const short* px = (const short*)(sv + p.o_x);
+    const short* W = p.pack_w ? (const short*)(sv + p.o_w) : (const short*)a->W;
+    const int64_t ldw = p.pack_w ? p.xs : a->ldw;
+    const int kt = p.split ? 16 : 32, pl = p.split ? 2 : 1;
+    short* G = (short*)(ws + p.o_g);
+    float* dxp = (float*)(ws + p.o_dx);
+    for (int v0 = 0; v0 < p.V; v0 += p.piece) {
+        const int words = p.Vp - v0 < p.piece ? p.Vp - v0 : p.piece;      // a multiple of 256
+        const int real = p.V - v0 < words ? p.V - v0 : words;
+        LogitArgs g{};
+        g.W = View{W, ldw, p.V, 0};
+        g.X = View{px, (int64_t)p.xs, p.Mp, 0};
+        g.b2 = (const float*)(sv + p.o_b2); g.head = head; g.kt = p.xs / 32; g.Mp = p.Mp;
+        g.lse = (const float*)(sv + p.o_lse); g.dlt = (const float*)(sv + p.o_dlt); g.rw = rw; g.tgt = (const int*)(sv + p.o_tgt);
+        g.g = G; g.ldg = (int64_t)p.piece * pl; g.dbp = dbias ? (float*)(ws + p.o_db) : nullptr; g.v0 = v0; g.piece = p.piece;
+        unsigned grid = make_map(g.map, words / Big::BI, p.Mp / Big::BJ, 1);
+#define DL(E, S) launch_dlogits<Big, E, S>(g, grid, s)
+        CAPDEC_TRY(BY_TYPE(p, DL));
+#undef DL
+        if (dx) {
+            GradArgs d{};
+            d.P = View{G, g.ldg, p.Mp, 0};
+            d.Q = View{W + (int64_t)v0 * ldw, ldw, p.Kp, real};
+            d.head = head; d.bh = bh; d.I = p.Mp; d.J = p.Kp; d.rows_live = 1; d.kt = words / kt; d.nsplit = p.sx;
+            d.part = dxp; d.ldp = p.Kp; d.plane = (int64_t)p.Mp * p.Kp; d.add = v0 > 0;
+            grid = make_map(d.map, (p.Mp + Big::BI - 1) / Big::BI, (p.Kp + Big::BJ - 1) / Big::BJ, p.sx);
+#define DX(E, S) launch_grad<Big, E, false, S, 0>(d, grid, s)
+            CAPDEC_TRY(BY_TYPE(p, DX));
+#undef DX
+        }
+        if (dW) {
+            GradArgs d{};
+            d.P = View{G, g.ldg, words, p.Mp};
+            d.Q = View{px, (int64_t)p.xs, p.Kp, p.Mp};
+            d.head = head; d.bh = bh; d.k_live = 1; d.nsplit = p.sw;
+            grid = make_map(d.map, words / Big::BI, (p.Kp + Big::BJ - 1) / Big::BJ, p.sw);
+            if (p.sw == 1) {
+                d.I = real; d.J = p.K;
+                d.out = (char*)dW + (int64_t)v0 * lddw * (p.split ? 4 : 2); d.ldo = lddw; d.dtype = a->dtype;
+#define DW(E, S) launch_grad<Big, E, true, S, 1>(d, grid, s)
+                CAPDEC_TRY(BY_TYPE(p, DW));
+#undef DW
+            } else {
+                d.I = real; d.J = p.Kp;
+                d.part = (float*)(ws + p.o_dw); d.ldp = p.Kp; d.plane = (int64_t)p.piece * p.Kp;
+#define DW(E, S) launch_grad<Big, E, true, S, 0>(d, grid, s)
+                CAPDEC_TRY(BY_TYPE(p, DW));
+#undef DW
+            }
+        }
+        const int slabs = dW ? p.sw : 1;
+        if (slabs > 1 || dbias) {
+            const int64_t items = (slabs > 1 ? (int64_t)real * ((p.K + 3) / 4) : 0) + (dbias ? real : 0);
+            dw_kernel<<<blocks_for(items, 256, 8192), 256, 0, s>>>((const float*)(ws + p.o_dw), (int64_t)p.piece * p.Kp, slabs,
+                                                                   p.Kp, real, p.K, head, bh, p.split, dW, lddw, a->dtype,
+                                                                   g.dbp, p.piece, dbias, v0);
+            CAPDEC_LAUNCH_CHECK();
+        }
+    }
+    if (dx) {
+        dx_kernel<<<blocks_for((int64_t)p.M * ((p.K + 3) / 4), 256, 8192), 256, 0, s>>>(
+            dxp, (int64_t)p.Mp * p.Kp, p.sx, p.Kp, p.M, p.K, slot, head, bh, p.split, dx, lddx, a->dtype);
+        CAPDEC_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+}  // extern "C"

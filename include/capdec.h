@@ -615,6 +615,74 @@ int capdec_satt_greedy_decode(const capdec_satt_model* m, const float* enc, cons
                               const float* c0, int B, int S, int max_len, int sos, int eos, void* workspace,
                               size_t workspace_bytes, int64_t* out_ids, int32_t* out_len, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Softmax cross entropy of a vocabulary projection without kept logits, with its gradients (no counterpart in the
+ * reference, which materialises [B,T,V] logits: transformer.py:137 + train.py:216,254-256).
+ *   z = x W^T + bias;  nll[r] = log(sum_v exp z[r,v]) - z[r, targets[r]], 0 where targets[r] == ignore_index
+ * x [M,K] and W [V,K] have unit column stride and row strides ldx, ldw (elements); x, W, bias and their gradients share
+ * one type.  Rows whose target is ignore_index are not read at all.  A counted target outside [0, V) makes its loss and
+ * the gradients it enters NaN.  M, V <= 2^24, K <= 2^20.
+ * `saved` (capdec_vocab_ce_saved_bytes) carries packed operands and row statistics from the forward call to the backward
+ * call, which reads W again: neither W nor `saved` may change in between.  `workspace` is scratch of one call.  Both are
+ * 16-byte aligned.  Sums run in fixed orders: results repeat bit for bit.
+ * forward: nll [M] fp32; loss (nullable) [3] fp32 = (mean over the counted rows, NaN without any; sum; their number).
+ * backward: the upstream gradient is row_grad [M] (fp32, d/d nll) or, where that is NULL, grad[0] for the sum of nll
+ * (mean == 0) or for its mean (mean != 0); dx, dW, dbias are written (not added to), any of them may be NULL.
+ * ------------------------------------------------------------------------------------------ */
+#define CAPDEC_F32 0
+#define CAPDEC_BF16 1
+#define CAPDEC_F16 2
+typedef struct capdec_vocab_ce {
+    const void* x;
+    const void* W;
+    const void* bias;             /* [V], nullable */
+    const int64_t* targets;       /* [M] */
+    int64_t ldx, ldw;
+    int64_t ignore_index;
+    int32_t M, V, K;
+    int32_t dtype;                /* CAPDEC_F32 / CAPDEC_BF16 / CAPDEC_F16 */
+} capdec_vocab_ce;
+size_t capdec_vocab_ce_saved_bytes(const capdec_vocab_ce* a /*host*/);
+size_t capdec_vocab_ce_forward_workspace_bytes(const capdec_vocab_ce* a /*host*/);
+size_t capdec_vocab_ce_backward_workspace_bytes(const capdec_vocab_ce* a /*host*/);
+int capdec_vocab_ce_forward(const capdec_vocab_ce* a /*host*/, void* saved, size_t saved_bytes, void* workspace,
+                            size_t workspace_bytes, float* nll, float* loss, void* stream);
+int capdec_vocab_ce_backward(const capdec_vocab_ce* a /*host*/, const void* saved, size_t saved_bytes, void* workspace,
+                             size_t workspace_bytes, const float* row_grad, const float* grad, int mean, void* dx,
+                             int64_t lddx, void* dW, int64_t lddw, void* dbias, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Orthogonalised updates of weight matrices (no counterpart in the reference, whose optimizer is Adam, train.py:217).
+ *   X = U / (|U|_F + eps);  steps times:  A = X X^T, X <- a X + (b A + c A^2) X      (coeffs = {a, b, c}, host)
+ * which drives the singular values of U towards 1.  `count` matrices of one shape per call, rows x cols with unit column
+ * stride, rows * cols <= 2^31, any of 16 bits or fp32; sums and intermediate values carry fp32's precision.  Coefficients
+ * under which singular values in [0, 1] could grow beyond 64 within the steps are refused (CAPDEC_EINVAL), as are more
+ * than 32 steps.  A zero matrix stays zero.  Sums run in fixed orders: results repeat bit for bit.
+ * capdec_orthogonalize: dst = the last X; dst may be src.
+ * capdec_muon_step: g <- grad_scale g;  m <- momentum m + g;  U = nesterov ? g + momentum m : m;
+ *   p <- p (1 - lr weight_decay) - lr update_scale X.   fp32; g itself is not written.  lr comes from st->lr (device) when st
+ *   is given.  No two of the call's p and m buffers may overlap.
+ * workspace: capdec_orthogonalize_workspace_bytes(count, rows, cols), 16-byte aligned.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct capdec_matrix {
+    const void* src;
+    void* dst;
+    int64_t ld_src, ld_dst;
+} capdec_matrix;
+typedef struct capdec_muon_param {
+    float* p;
+    const float* g;
+    float* m;
+    int64_t ldp, ldg, ldm;
+} capdec_muon_param;
+size_t capdec_orthogonalize_workspace_bytes(int count, int rows, int cols);
+int capdec_orthogonalize(const capdec_matrix* mats /*host*/, int count, int rows, int cols, int dtype, int steps,
+                         const float* coeffs /*host [3]*/, float eps, void* workspace, size_t workspace_bytes, void* stream);
+int capdec_muon_step(const capdec_muon_param* params /*host*/, int count, int rows, int cols, float lr,
+                     const capdec_train_state* st /*device, nullable*/, float momentum, int nesterov, float weight_decay,
+                     float update_scale, float grad_scale, int steps, const float* coeffs /*host [3]*/, float eps,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,346 @@
+"""Vocabulary cross entropy without kept logits: loss and gradients against the definition in 64 bits.
+
+Tolerances.  Let u be half a step of the operands' type (2^-24, 2^-8 for bfloat16, 2^-11 for float16).
+  logits: every product of the split fp32 operands is off by at most 3 * 2^-22 of itself (both low parts rounded, their
+  product left out; 16-bit products are exact) and a sum of K + 1 terms in fp32 by at most (K + 1) 2^-24 of the sum of
+  magnitudes S = |x| |W|^T + |b|: dz = (3 * 2^-22 + (K + 1) 2^-24) S.
+  softmax: exp2 in fp32 of a number of size Z = max |z| log2(e), rounded three times, over a sum of V terms added in a tree of
+  depth < 200:  dp / p <= 2 dz + (3 Z + 200) 2^-23.
+  gradients: G is rounded once to the operands' type (fp32: to 22 bits), its contraction's sum again in fp32 and the result
+  to the type:  |d| <= (dp/p + g + n 2^-24) sum |G| |other| + u |result|, with g = u (fp32: 2^-22) and n the length of the sum.
+  expm1 at the target adds 4 * 2^-24 + dz, which the bound of dp / p covers.  There G is p - 1, and an error dp of p (or of
+  log p) stays dp while the difference may vanish (a vocabulary of one word): the dp term is of p, not of |G|, so it is
+  taken over  H = p + [v = t] >= |G|:  |d| <= (dp/p) sum H |other| + (g + n 2^-24) sum |G| |other| + u |result|.
+  fp16 numbers (also the pairs that fp32 takes) end in steps of 2^-24: G, stored times at least 2^13 / max |w|, is off by
+  half a step, 2^-38 max |w|, however small it is; over a sum that is 2^-38 max |w| sum |other|.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TYPES = list(U)
+
+
+def make(M, V, K, dt, seed=0, bias=True, ignored=0.25, ignore=0):
+    g = torch.Generator("cuda").manual_seed(1000 * seed + M + V + K)
+    x = torch.randn(M, K, device="cuda", generator=g).to(dt)
+    W = (torch.randn(V, K, device="cuda", generator=g) * 1.5 / math.sqrt(K)).to(dt)
+    b = torch.randn(V, device="cuda", generator=g).to(dt) if bias else None
+    t = torch.randint(0, V, (M,), device="cuda", generator=g)
+    if ignored:
+        t[torch.rand(M, device="cuda", generator=g) < ignored] = ignore
+    return x, W, b, t
+
+
+def definition(x, W, b, t, w, ignore=0):
+    """nll, dx, dW, db for the upstream gradients ``w`` of the rows, and the error bounds of the module's docstring."""
+    K, V = x.shape[1], W.shape[0]
+    u = U[x.dtype]
+    x, W = x.double(), W.double()
+    bb = torch.zeros(V, device=x.device, dtype=torch.float64) if b is None else b.double()
+    live = t != ignore
+    z = x @ W.T + bb
+    lse = torch.logsumexp(z, 1)
+    at = torch.where(live, t, 0)
+    nll = torch.where(live, lse - z.gather(1, at[:, None])[:, 0], 0.0)
+    G = torch.softmax(z, 1)
+    H = G.clone()
+    G[torch.arange(len(t), device=t.device), at] -= 1.0
+    H[torch.arange(len(t), device=t.device), at] += 1.0
+    G, H = G * (w.double() * live)[:, None], H * (w.double().abs() * live)[:, None]
+    S = x.abs() @ W.abs().T + torch.where(bb.isfinite(), bb.abs(), 0.0)
+    S, Z = S[live].max().item() if live.any() else 0.0, z[live][z[live].isfinite()].abs().max().item() if live.any() else 0.0
+    dz = (3 * 2.0 ** -22 + (K + 1) * 2.0 ** -24) * S
+    dp = 2 * dz + (3 * Z * 1.4427 + 200) * 2.0 ** -23
+    g = 2.0 ** -22 if u == 2.0 ** -24 else u
+
+    floor = 0.0 if u == 2.0 ** -8 else 2.0 ** -38 * float(w.abs().max())
+
+    def bound(A, H, B, n):
+        return floor * B.abs().sum(0) + dp * (H @ B.abs()) + (g + n * 2.0 ** -24) * (A.abs() @ B.abs()) + u * (A @ B).abs()
+    n_live = int(live.sum())
+    res = [nll, G @ W, G.T @ x, G.sum(0)]
+    tol = [dz * 2 + (3 * Z + 200) * 2.0 ** -23, bound(G, H, W, V), bound(G.T, H.T, x, n_live),
+           floor * n_live + dp * H.sum(0) + (g + n_live * 2.0 ** -24) * G.abs().sum(0) + u * G.sum(0).abs()]
+    return res, tol
+
+
+def near(got, want, tol, what, subnormal=0.0):
+    err = (got.double() - want).abs()
+    assert got.shape == want.shape, what
+    assert bool((err <= tol + subnormal).all()), f"{what}: {float((err - tol).max()):.3e} over the bound, error {float(err.max()):.3e}"
+
+
+def run(x, W, b, t, reduction, w, ignore=0):
+    from capdec import functional as F
+    x, W = x.detach().requires_grad_(), W.detach().requires_grad_()
+    b = None if b is None else b.detach().requires_grad_()
+    loss = F.vocab_cross_entropy(x, W, b, t, ignore_index=ignore, reduction=reduction)
+    ins = [v for v in (x, W, b) if v is not None]
+    grads = torch.autograd.grad(loss, ins, w if reduction == "none" else None)
+    return loss.detach(), grads
+
+
+def check(x, W, b, t, reduction="mean", ignore=0, w=None):
+    n = max(1, int((t != ignore).sum()))
+    if reduction == "none":
+        w = torch.rand(len(t), device=x.device) + 0.1 if w is None else w
+        rows = w
+    else:
+        rows = torch.full((len(t),), 1.0 / n if reduction == "mean" else 1.0, device=x.device)
+    loss, grads = run(x, W, b, t, reduction, w, ignore)
+    (nll, *want), (tn, *tol) = definition(x, W, b, t, rows, ignore)
+    if reduction == "none":
+        near(loss, nll, torch.full_like(nll, tn), "loss")
+    else:
+        total = nll.sum() / (n if reduction == "mean" else 1)
+        near(loss, total, (tn * n + 2.0 ** -22 * nll.abs().sum()) / (n if reduction == "mean" else 1), "loss")
+    sub = 2.0 ** -25 if x.dtype == torch.float16 else 0.0          # half a step of fp16's smallest numbers
+    for got, ref, bound, name in zip(grads, want, tol, ("dx", "dW", "db")):
+        assert got.dtype == x.dtype
+        near(got, ref, bound, name, sub)
+    return loss, grads
+
+
+SIZES = [(1, 1, 1), (1, 2, 3), (1, 5, 32), (3, 257, 33), (31, 300, 40), (64, 255, 64), (65, 256, 31), (128, 1000, 96),
+         (129, 513, 333), (500, 2049, 128), (1030, 777, 512), (2000, 5000, 65)]
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("size", SIZES)
+def test_loss_and_gradients(size, dt):
+    x, W, b, t = make(*size, dt)
+    t[0] = size[1] - 1 if size[1] > 1 else 0
+    check(x, W, b if size[0] % 2 else None, t, "mean", ignore=0 if size[1] > 1 else -100)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_reductions_and_ignored_rows(reduction, dt):
+    for ignored in (0.0, 0.5, 0.95):
+        x, W, b, t = make(300, 1100, 96, dt, seed=1, ignored=ignored, ignore=-100)
+        check(x, W, b, t, reduction, ignore=-100)
+
+
+def test_row_weights_of_any_size():
+    """Upstream gradients of the rows over many orders of magnitude, zero among them."""
+    x, W, b, t = make(200, 600, 64, torch.float32, seed=2)
+    w = torch.rand(200, device="cuda") * 1e-12
+    w[3] = 0.0
+    check(x, W, b, t, "none", w=w)
+    w[5] = 1.0
+    check(x, W, b, t, "none", w=w * 1e20)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_no_counted_row(dt):
+    x, W, b, t = make(70, 300, 64, dt)
+    t[:] = 0
+    loss, grads = run(x, W, b, t, "mean", None)
+    assert math.isnan(loss.item()) and all(int(g.count_nonzero()) == 0 for g in grads)
+    loss, grads = run(x, W, b, t, "sum", None)
+    assert loss.item() == 0.0 and all(int(g.count_nonzero()) == 0 for g in grads)
+
+
+def test_empty_batch():
+    x, W, b, t = make(4, 300, 64, torch.float32)
+    loss, grads = run(x[:0], W, b, t[:0], "mean", None)
+    assert math.isnan(loss.item()) and grads[0].shape == (0, 64) and all(int(g.count_nonzero()) == 0 for g in grads)
+    assert run(x[:0], W, b, t[:0], "sum", None)[0].item() == 0.0
+
+
+def test_ignored_rows_are_not_read():
+    """Rows behind an ignored target may hold anything: infinities, NaN, uninitialised memory."""
+    x, W, b, t = make(300, 500, 64, torch.float32, seed=3)
+    want = run(x, W, b, t, "mean", None)
+    y = x.clone()
+    y[t == 0] = float("nan")
+    y[(t == 0).nonzero()[0]] = float("inf")
+    got = run(y, W, b, t, "mean", None)
+    assert torch.equal(got[0], want[0]) and all(torch.equal(a, c) for a, c in zip(got[1], want[1]))
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_masked_words(dt):
+    """Words masked by a bias of -inf or of the type's lowest value: whole tiles of them, and all but one."""
+    x, W, b, t = make(100, 700, 64, dt, seed=4, ignored=0.0)
+    b[:300] = float("-inf")
+    b[300:400] = torch.finfo(dt).min
+    t[:] = torch.randint(400, 700, (100,), device="cuda")
+    loss, grads = check(x, W, b, t, "mean", ignore=-1)
+    assert int(grads[1][:400].count_nonzero()) == 0 and int(grads[2][:400].count_nonzero()) == 0
+    b[:] = float("-inf")
+    b[650] = 0.5
+    t[:] = 650
+    loss, grads = run(x, W, b, t, "mean", None, ignore=-1)
+    assert abs(loss.item()) < 1e-5 and all(bool(g.isfinite().all()) for g in grads)
+
+
+def test_nan_stays_in_its_row():
+    x, W, b, t = make(200, 400, 64, torch.float32, seed=5, ignored=0.0)
+    want, _ = run(x, W, b, t, "none", torch.ones(200, device="cuda"), ignore=-1)
+    x[7, 3] = float("nan")
+    x[11, 3] = float("inf")
+    got, grads = run(x, W, b, t, "none", torch.ones(200, device="cuda"), ignore=-1)
+    bad = torch.zeros(200, dtype=torch.bool, device="cuda")
+    bad[[7, 11]] = True
+    assert bool(got[7].isnan()) and not bool(got[11].isfinite()) and torch.equal(got[~bad], want[~bad])
+    assert bool(grads[0][7].isnan().all()) and bool(grads[0][~bad].isfinite().all())
+
+
+def test_target_outside_the_vocabulary_is_nan():
+    for bad in (-5, 400, 2 ** 40):
+        x, W, b, t = make(50, 400, 64, torch.float32, seed=6)
+        t[9] = bad
+        loss, grads = run(x, W, b, t, "mean", None)
+        assert math.isnan(loss.item()) and bool(grads[0][9].isnan().all())
+        assert bool(grads[0][torch.arange(50) != 9].isfinite().all())
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_strides_and_alignment(dt):
+    x, W, b, t = make(130, 520, 96, dt, seed=7)
+    want = run(x, W, b, t, "sum", None)
+    for off in (1, 8):
+        wide_x = torch.full((130, 120), float("nan"), device="cuda", dtype=dt)
+        wide_w = torch.full((520, 130), float("nan"), device="cuda", dtype=dt)
+        wide_x[:, off:off + 96], wide_w[:, off:off + 96] = x, W
+        got = run(wide_x[:, off:off + 96], wide_w[:, off:off + 96], b, t, "sum", None)
+        assert torch.equal(got[0], want[0]) and all(torch.equal(a, c) for a, c in zip(got[1], want[1]))
+    # x whose columns are not contiguous is copied by the call; targets of any shape
+    from capdec import functional as F
+    got = F.vocab_cross_entropy(x.t().contiguous().t().view(10, 13, 96), W, b, t.view(10, 13), reduction="none")
+    assert got.shape == (10, 13) and torch.equal(got.sum(), F.vocab_cross_entropy(x, W, b, t, reduction="none").view(10, 13).sum())
+
+
+def test_gradients_written_into_given_buffers_with_strides():
+    from capdec import ops
+    x, W, b, t = make(130, 520, 96, torch.float32, seed=8)
+    nll, loss, saved = ops.vocab_ce_forward(x, W, b, t)
+    one = torch.ones(1, device="cuda")
+    want = ops.vocab_ce_backward(x, W, b, t, saved, grad=one)
+    bx, bw = torch.full((130, 100), 7.0, device="cuda"), torch.full((520, 101), 7.0, device="cuda")
+    got = ops.vocab_ce_backward(x, W, b, t, saved, grad=one, dx=bx[:, :96], dW=bw[:, :96])
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    assert bool((bx[:, 96:] == 7).all()) and bool((bw[:, 96:] == 7).all())
+    only = ops.vocab_ce_backward(x, W, b, t, saved, grad=one, need=(False, False, True))
+    assert only[0] is None and only[1] is None and torch.equal(only[2], want[2])
+    only = ops.vocab_ce_backward(x, W, b, t, saved, grad=one, need=(False, True, False))
+    assert torch.equal(only[1], want[1])
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_large_and_tiny_values(dt):
+    """Logits of hundreds, and operands at the ends of the type's range (fp32 operands are scaled by their largest)."""
+    x, W, b, t = make(100, 300, 64, dt, seed=9)
+    check((x.float() * 12).to(dt), W, b, t, "mean")
+    if dt == torch.float32:
+        check(x * 1e-18, W * 1e18, b, t, "mean")
+        check(x * 1e15, W * 1e-15, None, t, "mean")
+        check(x * 0, W, b, t, "mean")
+
+
+def test_gradient_against_differences():
+    """Central differences of the fp32 loss along random directions.  The loss of size L is known to about 2^-22 L, so a
+    step h leaves 2^-22 L / h of noise and h^2 / 6 of the third derivative (below |d|^3, |d| = the logits' change)."""
+    from capdec import functional as F
+    x, W, b, t = make(60, 200, 32, torch.float32, seed=10)
+    loss, (dx, dW, db) = run(x, W, b, t, "mean", None)
+    g = torch.Generator("cuda").manual_seed(3)
+    for k, (v, dv) in enumerate(((x, dx), (W, dW), (b, db))):
+        d = torch.randn(v.shape, device="cuda", generator=g)
+        d /= d.norm()
+        h = 0.02
+        ins = [x, W, b]
+
+        def at(s):
+            ins[k] = v + s * d
+            return F.vocab_cross_entropy(*ins, t).double().item()
+        diff = (at(h) - at(-h)) / (2 * h)
+        reach = max(1.0, float(W.norm(dim=1).max()), float(x.norm(dim=1).max()))
+        assert abs(diff - float((dv * d).sum())) <= 2.0 ** -20 * float(loss) / h + h * h * min(reach, 8.0) ** 3 / 6
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_repeats_bit_for_bit_and_on_another_stream(dt):
+    x, W, b, t = make(700, 3000, 160, dt, seed=11)
+    want = run(x, W, b, t, "mean", None)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        got = run(x, W, b, t, "mean", None)
+    s.synchronize()
+    again = run(x, W, b, t, "mean", None)
+    for r in (got, again):
+        assert torch.equal(r[0], want[0]) and all(torch.equal(a, c) for a, c in zip(r[1], want[1]))
+
+
+def test_captured_and_replayed():
+    """Forward and backward in one HIP graph, replayed with new inputs, other work in between; two graphs side by side."""
+    from capdec import ops
+    graphs = []
+    one = torch.ones(1, device="cuda")
+    for n in range(2):
+        x, W, b, t = make(260, 900, 96, torch.float32, seed=20 + n)
+
+        def step(x=x, W=W, b=b, t=t):
+            nll, loss, saved = ops.vocab_ce_forward(x, W, b, t)
+            return (loss,) + ops.vocab_ce_backward(x, W, b, t, saved, grad=one)
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        graphs.append((graph, outs, (x, W, b, t), step))
+    for r in range(3):
+        for n, (graph, outs, ins, step) in enumerate(graphs):
+            fresh = make(260, 900, 96, torch.float32, seed=30 + 2 * r + n, ignored=0.2 * r)
+            for dst, src in zip(ins, fresh):
+                dst.copy_(src)
+        for graph, *_ in graphs:
+            graph.replay()
+        got = [[o.clone() for o in outs] for _, outs, _, _ in graphs]
+        torch.cuda.synchronize()
+        for have, (_, _, _, step) in zip(got, graphs):
+            assert all(torch.equal(a, c) for a, c in zip(have, step()))
+
+
+def test_pieces_of_the_vocabulary():
+    """A batch and vocabulary whose gradient matrix takes more than one piece (512 MiB each)."""
+    M, V, K = 30000, 10007, 32
+    for dt in (torch.bfloat16, torch.float32):
+        x, W, b, t = make(M, V, K, dt, seed=12)
+        check(x, W, b, t, "mean")
+
+
+def test_offsets_past_32_bits():
+    """A vocabulary matrix of more than 2^31 elements: loss, and the gradients of the words at its end."""
+    V, K, M = 1100001, 2048, 40
+    g = torch.Generator("cuda").manual_seed(5)
+    W = torch.empty(V, K, device="cuda", dtype=torch.bfloat16)
+    for i in range(0, V, 100000):
+        W[i:i + 100000] = torch.randn(min(100000, V - i), K, device="cuda", generator=g) * 0.03
+    x = torch.randn(M, K, device="cuda", generator=g).bfloat16()
+    t = torch.randint(V - 1000, V, (M,), device="cuda", generator=g)
+    loss, (dx, dW) = run(x, W, None, t, "mean", None)
+    z = torch.cat([x.double() @ W[i:i + 100000].double().T for i in range(0, V, 100000)], 1)
+    lse = torch.logsumexp(z, 1)
+    want = (lse - z.gather(1, t[:, None])[:, 0]).mean()
+    assert abs(loss.item() - want.item()) <= 1e-5 * abs(want.item())
+    G = torch.softmax(z, 1)
+    G[torch.arange(M), t] -= 1
+    G /= M
+    u = U[torch.bfloat16]
+    end = G[:, -1000:].T @ x.double()
+    # twice u: G's rounding and the result's, plus a sixteenth for the fp32 sums
+    near(dW[-1000:], end, (1 + 1 / 16) * u * (G[:, -1000:].abs().T @ x.double().abs() + end.abs()), "dW")
+    ref, mag = torch.zeros(M, K, device="cuda", dtype=torch.float64), torch.zeros(M, K, device="cuda", dtype=torch.float64)
+    for i in range(0, V, 100000):
+        w = W[i:i + 100000].double()
+        ref += G[:, i:i + 100000] @ w
+        mag += G[:, i:i + 100000].abs() @ w.abs()
+    near(dx, ref, (1 + 1 / 16) * u * (mag + ref.abs()), "dx")
