@@ -5,7 +5,7 @@
 //
 // Each operand is stored either k-contiguous ([x][k], "N") or x-contiguous ([k][x], "T": the contraction runs over its
 // leading axis).  Tiles reach LDS by global_load_lds (1 KiB pieces, lane l at byte 16 l, XOR-swizzled through the source
-// address), in a ring of three buffers: two k-tiles are in flight while one is multiplied, one barrier per tile.  T
+// address), in a ring of three or four buffers: the other tiles are in flight while one is multiplied, one barrier per tile.  T
 // tiles are transposed by the LDS read itself (ds_read_b64_tr_b16).
 //
 // SPLIT operands carry 32-bit values as two fp16 numbers, v * s = hi + lo with s a power of two: 22 significant bits.
@@ -63,6 +63,14 @@ __device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
 
 // accumulator register e of lane half h is row (e & 3) + 8 (e >> 2) + 4 h of the 32x32 tile
 __device__ __forceinline__ int acc_row(int e, int h) { return (e & 3) + 8 * (e >> 2) + 4 * h; }
+
+// 16 bytes per lane from `src` to 1 KiB of LDS at `dst` (wave-uniform), asynchronously.  Written as assembly because the
+// compiler, where it knows of such loads, waits for all of them before every transposing LDS read; it has no output
+// registers, and contract() waits for it by count.
+__device__ __forceinline__ void dma16(const short* src, short* dst) {
+    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) short*)dst);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src) : "memory");
+}
 
 struct View {               // one operand
     const short* p;
@@ -123,18 +131,23 @@ struct Operand {
     }
 };
 
-// A workgroup of 2 x 2 wavefronts, each holding TI x TJ accumulators of 32x32.
-template <int TI_, int TJ_>
+// A workgroup of WI x WJ wavefronts, each holding TI x TJ accumulators of 32x32, with a ring of STAGES k-tiles.
+// SPREAD: the loads of a later k-tile are issued between the matrix instructions, at raised priority, which suits
+// workgroups that share a CU (256 x 128: 223 against 243 us for 7424 x 10000 x 512 in fp32); else ahead of them, with the
+// LDS reads spread instead (256 x 256: 1076 against 1090 us for 8192 x 32768 x 2048 in bf16, gradients 941 against 1041).
+template <int WI_, int WJ_, int TI_, int TJ_, int STAGES_, bool SPREAD_>
 struct Tile {
-    static constexpr int TI = TI_, TJ = TJ_;
-    static constexpr int BI = 64 * TI, BJ = 64 * TJ;
-    static constexpr int THREADS = 256;
+    static constexpr int WI = WI_, WJ = WJ_, TI = TI_, TJ = TJ_, STAGES = STAGES_;
+    static constexpr bool SPREAD = SPREAD_;
+    static constexpr int BI = 32 * WI * TI, BJ = 32 * WJ * TJ;
+    static constexpr int WAVES = WI * WJ, THREADS = 64 * WAVES;
     static constexpr int STAGE = (BI + BJ) * 32;              // 16-bit elements of one ring buffer
-    static constexpr int LDS_BYTES = 3 * STAGE * 2;
+    static constexpr int LDS_BYTES = STAGES * STAGE * 2;
 };
-typedef Tile<4, 2> Big;        // 256 x 128: 72 KiB of LDS, two workgroups per CU
-typedef Tile<2, 2> Mid;        // 128 x 128: 48 KiB, three
-typedef Tile<1, 1> Small;      //  64 x  64: 24 KiB
+typedef Tile<2, 4, 4, 2, 4, false> Wide;    // 256 x 256: 128 KiB of LDS, one workgroup per CU
+typedef Tile<2, 2, 4, 2, 3, true> Big;     // 256 x 128: 72 KiB, two workgroups per CU
+typedef Tile<2, 2, 2, 2, 3, true> Mid;     // 128 x 128: 48 KiB, three
+typedef Tile<2, 2, 1, 1, 3, false> Small;   //  64 x  64: 24 KiB
 
 // Adds k-tiles [kt0, kt1) of the tile at (i0, j0) onto zero.  Ends behind a barrier: the caller may reuse `lds`.
 template <class C, int ELT, bool TP, bool TQ, bool SPLIT>
@@ -142,11 +155,12 @@ __device__ __forceinline__ void contract(const View& P, const View& Q, int i0, i
                                          f32x16 (&acc)[C::TI][C::TJ]) {
     using OpP = Operand<C::BI, TP, SPLIT>;
     using OpQ = Operand<C::BJ, TQ, SPLIT>;
-    constexpr int NPW = (OpP::PIECES + OpQ::PIECES) / 4;
-    static_assert(OpP::PIECES % 4 == 0 && OpQ::PIECES % 4 == 0, "pieces do not divide over the wavefronts");
+    constexpr int W = C::WAVES, S = C::STAGES, NPW = (OpP::PIECES + OpQ::PIECES) / W;
+    static_assert(S == 3 || S == 4, "the waits below count for these ring depths");
+    static_assert(OpP::PIECES % W == 0 && OpQ::PIECES % W == 0, "pieces do not divide over the wavefronts");
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wi = wave >> 1, wj = wave & 1;
+    const int wi = wave / C::WJ, wj = wave % C::WJ;
 #pragma unroll
     for (int ti = 0; ti < C::TI; ++ti)
 #pragma unroll
@@ -158,76 +172,94 @@ __device__ __forceinline__ void contract(const View& P, const View& Q, int i0, i
     auto seek = [&](int kt) {
 #pragma unroll
         for (int i = 0; i < NPW; ++i) {
-            const int piece = i * 4 + wave;
-            src[i] = i * 4 < OpP::PIECES ? OpP::source(P, i0, kt, piece, lane)
+            const int piece = i * W + wave;
+            src[i] = i * W < OpP::PIECES ? OpP::source(P, i0, kt, piece, lane)
                                          : OpQ::source(Q, j0, kt, piece - OpP::PIECES, lane);
         }
     };
     const int64_t stepP = OpP::step(P), stepQ = OpQ::step(Q);
     // the first k-tile that reaches past a T operand's rows: its addresses are clamped one by one
     const int ragged = min(TP ? P.klim / OpP::KT : kt1, TQ ? Q.klim / OpQ::KT : kt1);
+    // one of this wavefront's pieces of k-tile kt
+    auto issue_piece = [&](short* buf, int i) {
+        const int piece = i * W + wave;
+        if (TP || TQ)
+            dma16(src[i], buf + piece * 512);
+        else
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src[i],
+                                             (__attribute__((address_space(3))) void*)(buf + piece * 512), 16, 0, 0);
+        src[i] += i * W < OpP::PIECES ? stepP : stepQ;
+    };
     auto issue = [&](short* buf, int kt) {
         if ((TP || TQ) && kt >= ragged) seek(kt);
 #pragma unroll
-        for (int i = 0; i < NPW; ++i) {
-            const int piece = i * 4 + wave;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src[i],
-                                             (__attribute__((address_space(3))) void*)(buf + piece * 512), 16, 0, 0);
-            src[i] += i * 4 < OpP::PIECES ? stepP : stepQ;
-        }
+        for (int i = 0; i < NPW; ++i) issue_piece(buf, i);
     };
-    auto compute = [&](const short* ip) {
+    // Two halves (k-chunks; SPLIT: planes) of fragments, the products over them, and between the products the loads of a
+    // later tile when `more`.
+    auto compute = [&](const short* ip, short* buf, bool more) {
         const short* iq = ip + C::BI * 32;
-        if (SPLIT) {
-            s16x8 a[2][C::TI], b[2][C::TJ];
+        s16x8 a[2][C::TI], b[2][C::TJ];
 #pragma unroll
-            for (int pl = 0; pl < 2; ++pl) {
+        for (int hf = 0; hf < 2; ++hf) {
 #pragma unroll
-                for (int ti = 0; ti < C::TI; ++ti) a[pl][ti] = OpP::frag(ip, (wi * C::TI + ti) * 32, pl, lane);
+            for (int tj = 0; tj < C::TJ; ++tj) b[hf][tj] = OpQ::frag(iq, (wj * C::TJ + tj) * 32, hf, lane);
 #pragma unroll
-                for (int tj = 0; tj < C::TJ; ++tj) b[pl][tj] = OpQ::frag(iq, (wj * C::TJ + tj) * 32, pl, lane);
-            }
+            for (int ti = 0; ti < C::TI; ++ti) a[hf][ti] = OpP::frag(ip, (wi * C::TI + ti) * 32, hf, lane);
+        }
+        if (C::SPREAD) __builtin_amdgcn_sched_barrier(0);
+        constexpr int TERMS = SPLIT ? 3 : 2, N = TERMS * C::TI * C::TJ, EVERY = N / NPW > 0 ? N / NPW : 1;
+        static_assert(!C::SPREAD || N >= NPW, "not every piece would be issued");
 #pragma unroll
-            for (int t = 0; t < 3; ++t)        // hi*hi first: its operands arrive first
-#pragma unroll
-                for (int ti = 0; ti < C::TI; ++ti)
-#pragma unroll
-                    for (int tj = 0; tj < C::TJ; ++tj)
-                        acc[ti][tj] = mfma<ELT>(a[t == 2][ti], b[t == 1][tj], acc[ti][tj]);
-        } else {
-#pragma unroll
-            for (int kc = 0; kc < 2; ++kc) {
-                s16x8 a[C::TI], b[C::TJ];
-#pragma unroll
-                for (int ti = 0; ti < C::TI; ++ti) a[ti] = OpP::frag(ip, (wi * C::TI + ti) * 32, kc, lane);
-#pragma unroll
-                for (int tj = 0; tj < C::TJ; ++tj) b[tj] = OpQ::frag(iq, (wj * C::TJ + tj) * 32, kc, lane);
-#pragma unroll
-                for (int ti = 0; ti < C::TI; ++ti)
-#pragma unroll
-                    for (int tj = 0; tj < C::TJ; ++tj) acc[ti][tj] = mfma<ELT>(a[ti], b[tj], acc[ti][tj]);
+        for (int n = 0; n < N; ++n) {
+            const int t = n / (C::TI * C::TJ), ti = n / C::TJ % C::TI, tj = n % C::TJ;
+            // SPLIT: hi*hi, hi*lo, lo*hi
+            acc[ti][tj] = mfma<ELT>(a[SPLIT ? t == 2 : t][ti], b[SPLIT ? t == 1 : t][tj], acc[ti][tj]);
+            if (C::SPREAD && n % EVERY == 0 && n / EVERY < NPW) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (more) issue_piece(buf, n / EVERY);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     };
     short* rd = lds;                          // the buffer of tile kt
-    short* wr = lds + 2 * C::STAGE;           // the buffer of tile kt + 2
-    if (kt0 < kt1) {
-        seek(kt0);
-        issue(rd, kt0);
-    }
-    if (kt0 + 1 < kt1) issue(rd + C::STAGE, kt0 + 1);
+    short* wr = lds + (S - 1) * C::STAGE;     // the buffer of tile kt + S - 1
+#pragma unroll
+    for (int t = 0; t < S - 1; ++t)
+        if (kt0 + t < kt1) {
+            if (t == 0) seek(kt0);
+            issue(lds + t * C::STAGE, kt0 + t);
+        }
     for (int kt = kt0; kt < kt1; ++kt) {
-        // this wavefront's pieces of tile kt have landed (those of kt + 1 may stay in flight, loads retire in order) and
-        // it is done reading the buffer that tile kt + 2 goes to; the barrier says so for all four
-        if (kt + 1 < kt1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NPW) : "memory");
+        // this wavefront's pieces of tile kt have landed (those of later tiles may stay in flight, loads retire in order)
+        // and it is done reading the buffer that tile kt + S - 1 goes to; the barrier says so for all wavefronts
+        if (kt + S - 2 < kt1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * NPW) : "memory");
+        else if (S > 3 && kt + S - 3 < kt1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 3) * NPW) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
-        if (kt + 2 < kt1) issue(wr, kt + 2);
-        __builtin_amdgcn_sched_barrier(0);
-        compute(rd);
+        const bool more = kt + S - 1 < kt1;
+        if (C::SPREAD) {
+            if ((TP || TQ) && more && kt + S - 1 >= ragged) seek(kt + S - 1);
+            __builtin_amdgcn_s_setprio(1);
+            compute(rd, wr, more);
+            __builtin_amdgcn_s_setprio(0);
+        } else {
+            if (more) issue(wr, kt + S - 1);
+            __builtin_amdgcn_sched_barrier(0);
+            compute(rd, wr, more);
+            // the first half's LDS reads, then one read between matrix instructions
+            constexpr int READS = C::TI * (TP ? 2 : 1) + C::TJ * (TQ ? 2 : 1);
+            __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+            for (int i = 0; i < READS; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, (SPLIT ? 3 : 2) * C::TI * C::TJ - READS, 0);
+        }
         __builtin_amdgcn_sched_barrier(0);
         wr = rd;
-        rd = rd == lds + 2 * C::STAGE ? lds : rd + C::STAGE;
+        rd = rd == lds + (S - 1) * C::STAGE ? lds : rd + C::STAGE;
     }
     __syncthreads();
 }

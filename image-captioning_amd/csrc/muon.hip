@@ -151,7 +151,7 @@ struct StepArgs {
 enum { INNER = 0, RESULT = 1, UPDATE = 2 };
 
 template <class C, bool TP, bool TQ, bool SPLIT, int OUT>
-__global__ __launch_bounds__(256, 2) void step_kernel(StepArgs a) {
+__global__ __launch_bounds__(C::THREADS, 2) void step_kernel(StepArgs a) {
     extern __shared__ __attribute__((aligned(16))) short lds[];
     int ti_, tj_, z;
     if (!tile_of(a.map, blockIdx.x, ti_, tj_, z)) return;
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(256, 2) void step_kernel(StepArgs a) {
     contract<C, F16, TP, TQ, SPLIT>(P, Q, i0, j0, 0, a.kt, lds, acc);
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));
-    const int lane = tid & 63, wave = tid >> 6, wi = wave >> 1, wj = wave & 1, h = lane >> 5;
+    const int lane = tid & 63, wave = tid >> 6, wi = wave / C::WJ, wj = wave % C::WJ, h = lane >> 5;
     const short* R = a.R ? a.R + z * a.strideR : nullptr;
     float lr = a.lr;
     if (OUT == UPDATE && a.st) lr = a.st->lr;
@@ -219,15 +219,16 @@ int launch(const StepArgs& a0, int nz, hipStream_t s) {
     if (C::LDS_BYTES > 64 * 1024)
         CAPDEC_TRY((int)hipFuncSetAttribute(reinterpret_cast<const void*>(step_kernel<C, TP, TQ, SPLIT, OUT>),
                                             hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS_BYTES));
-    step_kernel<C, TP, TQ, SPLIT, OUT><<<grid, 256, C::LDS_BYTES, s>>>(a);
+    step_kernel<C, TP, TQ, SPLIT, OUT><<<grid, C::THREADS, C::LDS_BYTES, s>>>(a);
     CAPDEC_LAUNCH_CHECK();
     return 0;
 }
 
-// 256x128 tiles when they give every CU one, else 128x128, else 64x64
+// the largest tiles that give every CU one, from 256x256 to 64x64
 template <bool TP, bool TQ, bool SPLIT, int OUT>
 int launch_sized(const StepArgs& a, int nz, hipStream_t s) {
     auto tiles = [&](int bi, int bj) { return (int64_t)((a.I + bi - 1) / bi) * ((a.J + bj - 1) / bj) * nz; };
+    if (tiles(256, 256) >= 256) return launch<Wide, TP, TQ, SPLIT, OUT>(a, nz, s);
     if (tiles(256, 128) >= 256) return launch<Big, TP, TQ, SPLIT, OUT>(a, nz, s);
     if (tiles(128, 128) >= 256) return launch<Mid, TP, TQ, SPLIT, OUT>(a, nz, s);
     return launch<Small, TP, TQ, SPLIT, OUT>(a, nz, s);

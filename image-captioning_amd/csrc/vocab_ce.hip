@@ -25,11 +25,12 @@ constexpr size_t PIECE_BYTES = (size_t)512 << 20;
 
 // ---- memory plan (host and device agree through it) ------------------------------------------------------------------
 struct Plan {
-    int M, V, K, Mp, Vp, Kp, split, elt;         // Mp: rows rounded up to 128, Vp: words to 256, Kp: width to 32
+    int M, V, K, Mp, Vp, Kp, split, elt;         // Mp: rows and Vp: words rounded up to 256, Kp: width to 32
     int xs;                                      // stored columns of the packed operands: Kp, or 2 Kp when split
     bool pack_w;
     int piece, pieces;                           // vocabulary words per piece (a multiple of 256)
     int sx, sw;                                  // contraction splits of dx and dW
+    bool wide_z, wide_dx, wide_dw;               // tiles of 256 x 256 for the logits, dx and dW
     size_t o_order, o_slot, o_tgt, o_lse, o_dlt, o_b2, o_x, o_w, saved;
     size_t o_part, fwd;
     size_t o_rw, o_g, o_dx, o_dw, o_db, bwd;
@@ -41,19 +42,28 @@ size_t take(size_t& at, size_t bytes) {
     return o;
 }
 
-int splits_for(int64_t tiles, int kt) {
-    // enough workgroups for two on each of 256 CUs, at least 8 k-tiles each
-    int s = 1;
-    while (s < 16 && tiles * (s + 1) <= 512 && kt / (s + 1) >= 8) ++s;
-    return s;
+// Contractions with few output tiles and a long sum are cut into s parts.  Workgroups run in rounds of `slots`; a part takes
+// 1 / s of the time, and each part costs about 6 k-tiles of time for its start, its partial sums and their addition.
+int splits_for(int64_t tiles, int kt, int slots) {
+    int best = 1;
+    double least = 1e300;
+    for (int s = 1; s <= 16 && kt / s >= 8; ++s) {
+        const double t = (double)((tiles * s + slots - 1) / slots) * ((kt + s - 1) / s + 6);
+        if (t < least * 0.97) least = t, best = s;
+    }
+    return best;
 }
+
+// Tiles of 256 x 256 when the contraction is long enough to make up for an epilogue that nothing overlaps (from 48 k-tiles
+// on: 1076 against 1213 us at 64, 243 against 223 at 32) and there is one for every CU; else 256 x 128, two to a CU.
+bool wide_pays(int64_t wide_tiles, int kt) { return kt >= 48 && wide_tiles >= 256; }
 
 bool make_plan(const capdec_vocab_ce* a, Plan& p) {
     if (!a || a->M < 1 || a->V < 1 || a->K < 1 || a->dtype < 0 || a->dtype > 2) return false;
     if (a->M > (1 << 24) || a->V > (1 << 24) || a->K > (1 << 20)) return false;
     p = Plan{};
     p.M = a->M; p.V = a->V; p.K = a->K;
-    p.Mp = (a->M + 127) / 128 * 128;
+    p.Mp = (a->M + 255) / 256 * 256;
     p.Vp = (a->V + 255) / 256 * 256;
     p.Kp = (a->K + 31) / 32 * 32;
     p.split = a->dtype == CAPDEC_F32;
@@ -83,8 +93,16 @@ bool make_plan(const capdec_vocab_ce* a, Plan& p) {
     p.piece = ((p.Vp + p.pieces - 1) / p.pieces + 255) / 256 * 256;
     p.pieces = (p.Vp + p.piece - 1) / p.piece;
     const int kt = p.split ? 16 : 32;
-    p.sx = splits_for((int64_t)((p.M + 255) / 256) * ((p.Kp + 127) / 128), p.piece / kt);
-    p.sw = splits_for((int64_t)(p.piece / 256) * ((p.Kp + 127) / 128), p.Mp / kt);
+    const int64_t row_tiles = p.Mp / 256, word_tiles = p.piece / 256;
+    p.wide_z = wide_pays(row_tiles * word_tiles, p.xs / 32);
+    auto grad = [&](int64_t tiles, int n, int& split) {      // tiles of 256 along the first axis
+        const int s2 = splits_for(tiles * ((p.Kp + 127) / 128), n, 512), s1 = splits_for(tiles * ((p.Kp + 255) / 256), n, 256);
+        const bool wide = p.Kp % 256 == 0 && wide_pays(tiles * (p.Kp / 256) * s1, n / s1);
+        split = wide ? s1 : s2;
+        return wide;
+    };
+    p.wide_dx = grad(row_tiles, p.piece / kt, p.sx);
+    p.wide_dw = grad(word_tiles, p.Mp / kt, p.sw);
     at = 256;
     p.o_rw = take(at, (size_t)p.Mp * 4);
     p.o_g = take(at, (size_t)p.Mp * p.piece * es);
@@ -293,7 +311,7 @@ __device__ __forceinline__ float logit_scale(const Head* head) {
 }
 
 template <class C, int ELT, bool SPLIT>
-__global__ __launch_bounds__(256, 2) void lse_kernel(LogitArgs a) {
+__global__ __launch_bounds__(C::THREADS, 2) void lse_kernel(LogitArgs a) {
     extern __shared__ __attribute__((aligned(16))) short lds[];
     int ti_, tj_, z;
     if (!tile_of(a.map, blockIdx.x, ti_, tj_, z)) return;
@@ -302,7 +320,7 @@ __global__ __launch_bounds__(256, 2) void lse_kernel(LogitArgs a) {
     if (j0 >= count) return;
     f32x16 acc[C::TI][C::TJ];
     contract<C, ELT, false, false, SPLIT>(a.W, a.X, i0, j0, 0, a.kt, lds, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave >> 1, wj = wave & 1, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave / C::WJ, wj = wave % C::WJ, h = lane >> 5;
     const float c1 = logit_scale<SPLIT>(a.head);
     float2* red = reinterpret_cast<float2*>(lds);
 #pragma unroll
@@ -333,7 +351,7 @@ __global__ __launch_bounds__(256, 2) void lse_kernel(LogitArgs a) {
         if (h == 0) red[wi * C::BJ + (wj * C::TJ + tj) * 32 + lane] = make_float2(mm, s);
     }
     __syncthreads();
-    for (int j = threadIdx.x; j < C::BJ; j += 256) {
+    for (int j = threadIdx.x; j < C::BJ; j += C::THREADS) {
         const float2 u = red[j], v = red[C::BJ + j];
         const float mm = fmaxf(u.x, v.x), mz = mm == -INFINITY ? 0.f : mm;
         a.part[(int64_t)ti_ * a.Mp + j0 + j] =
@@ -441,7 +459,7 @@ __global__ __launch_bounds__(1024) void weights_kernel(const float* __restrict__
 // that rows are stored 256 contiguous bytes at a time; on the way the targets' entries are put in, (p_t - 1) g as
 // expm1(log p_t) g, and each word's column is summed for the bias gradient.
 template <class C, int ELT, bool SPLIT>
-__global__ __launch_bounds__(256, 2) void dlogits_kernel(LogitArgs a) {
+__global__ __launch_bounds__(C::THREADS, 2) void dlogits_kernel(LogitArgs a) {
     extern __shared__ __attribute__((aligned(16))) short lds[];
     int ti_, tj_, z;
     if (!tile_of(a.map, blockIdx.x, ti_, tj_, z)) return;
@@ -452,14 +470,14 @@ __global__ __launch_bounds__(256, 2) void dlogits_kernel(LogitArgs a) {
     contract<C, ELT, false, false, SPLIT>(a.W, a.X, i0, j0, 0, a.kt, lds, acc);
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));       // the addresses below are made here, not ahead of the contraction (72 spills)
-    const int lane = tid & 63, wave = tid >> 6, wi = wave >> 1, wj = wave & 1, h = lane >> 5;
+    const int lane = tid & 63, wave = tid >> 6, wi = wave / C::WJ, wj = wave % C::WJ, h = lane >> 5;
     const float c1 = logit_scale<SPLIT>(a.head);
     constexpr int WORDS = 32 * C::TI;                     // of a wavefront
     constexpr int PL = SPLIT ? 2 : 1;
     constexpr int LD = WORDS * PL + 8;                    // 16-bit elements per row of the turned tile
     // one 32-row block of the wavefront at a time
     short* tile = lds + wave * 32 * LD;
-    float* colsum = reinterpret_cast<float*>(lds + 4 * 32 * LD);      // [2 (wj)][BI]
+    float* colsum = reinterpret_cast<float*>(lds + C::WAVES * 32 * LD);      // [WJ][BI]
     float sums[2] = {0.f, 0.f};
 #pragma unroll
     for (int tj = 0; tj < C::TJ; ++tj) {
@@ -543,8 +561,12 @@ __global__ __launch_bounds__(256, 2) void dlogits_kernel(LogitArgs a) {
 #pragma unroll
         for (int k = 0; k < WORDS / 64; ++k) colsum[wj * C::BI + wi * WORDS + lane + 64 * k] = sums[k];
         __syncthreads();
-        for (int i = threadIdx.x; i < C::BI; i += 256)
-            a.dbp[(int64_t)tj_ * a.piece + ti_ * C::BI + i] = colsum[i] + colsum[C::BI + i];
+        for (int i = threadIdx.x; i < C::BI; i += C::THREADS) {
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < C::WJ; ++w) sum += colsum[w * C::BI + i];
+            a.dbp[(int64_t)tj_ * a.piece + ti_ * C::BI + i] = sum;
+        }
     }
 }
 
@@ -568,7 +590,7 @@ __device__ __forceinline__ void store_as(void* p, int64_t i, float v, int dtype)
 }
 
 template <class C, int ELT, bool TP, bool SPLIT, int OUT>
-__global__ __launch_bounds__(256, 2) void grad_kernel(GradArgs a) {
+__global__ __launch_bounds__(C::THREADS, 2) void grad_kernel(GradArgs a) {
     extern __shared__ __attribute__((aligned(16))) short lds[];
     int ti_, tj_, z;
     if (!tile_of(a.map, blockIdx.x, ti_, tj_, z)) return;
@@ -581,7 +603,7 @@ __global__ __launch_bounds__(256, 2) void grad_kernel(GradArgs a) {
     const int per = (kt + a.nsplit - 1) / a.nsplit;
     f32x16 acc[C::TI][C::TJ];
     contract<C, ELT, TP, true, SPLIT>(a.P, a.Q, i0, j0, z * per, min(kt, (z + 1) * per), lds, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave >> 1, wj = wave & 1, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave / C::WJ, wj = wave % C::WJ, h = lane >> 5;
     float f = 1.f;
     if (OUT == 1) {
         f = a.bh->factor;
@@ -632,14 +654,14 @@ __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part,
 __global__ __launch_bounds__(256) void dw_kernel(const float* __restrict__ part, int64_t plane, int nsplit, int Kp, int rows,
                                                  int K, const Head* __restrict__ head, const BwdHead* __restrict__ bh,
                                                  int split, void* dW, int64_t ldw, int dtype, const float* __restrict__ dbp,
-                                                 int piece, void* db, int v0) {
+                                                 int piece, int row_tile, void* db, int v0) {
     const float fb = bh->factor;
     const float f = fb * (split ? pow2(-scale_exp(head->amax_x)) : 1.f);
     const int cpr = (K + 3) / 4;
     const int64_t nw = nsplit > 1 ? (int64_t)rows * cpr : 0;
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < nw + (dbp ? rows : 0); t += (int64_t)gridDim.x * 256) {
         if (t >= nw) {
-            const int v = (int)(t - nw), tiles = (head->count + 127) / 128;
+            const int v = (int)(t - nw), tiles = (head->count + row_tile - 1) / row_tile;
             float s = 0.f;
             for (int k = 0; k < tiles; ++k) s += dbp[(int64_t)k * piece + v];
             store_as(db, v0 + v, s * fb, dtype);
@@ -666,25 +688,28 @@ int allow_lds(K kernel, int bytes) {
 }
 
 template <class C, int ELT, bool SPLIT>
-int launch_lse(const LogitArgs& a, unsigned grid, hipStream_t s) {
+int launch_lse(LogitArgs a, int words, int rows, hipStream_t s) {
+    const unsigned grid = make_map(a.map, words / C::BI, rows / C::BJ, 1);
     CAPDEC_TRY(allow_lds(lse_kernel<C, ELT, SPLIT>, C::LDS_BYTES));
-    lse_kernel<C, ELT, SPLIT><<<grid, 256, C::LDS_BYTES, s>>>(a);
+    lse_kernel<C, ELT, SPLIT><<<grid, C::THREADS, C::LDS_BYTES, s>>>(a);
     CAPDEC_LAUNCH_CHECK();
     return 0;
 }
 template <class C, int ELT, bool SPLIT>
-int launch_dlogits(const LogitArgs& a, unsigned grid, hipStream_t s) {
-    constexpr int turned = (4 * 32 * (32 * C::TI * (SPLIT ? 2 : 1) + 8)) * 2 + 2 * C::BI * 4;
+int launch_dlogits(LogitArgs a, int words, int rows, hipStream_t s) {
+    constexpr int turned = C::WAVES * 32 * (32 * C::TI * (SPLIT ? 2 : 1) + 8) * 2 + C::WJ * C::BI * 4;
     constexpr int bytes = turned > C::LDS_BYTES ? turned : C::LDS_BYTES;
+    const unsigned grid = make_map(a.map, words / C::BI, rows / C::BJ, 1);
     CAPDEC_TRY(allow_lds(dlogits_kernel<C, ELT, SPLIT>, bytes));
-    dlogits_kernel<C, ELT, SPLIT><<<grid, 256, bytes, s>>>(a);
+    dlogits_kernel<C, ELT, SPLIT><<<grid, C::THREADS, bytes, s>>>(a);
     CAPDEC_LAUNCH_CHECK();
     return 0;
 }
 template <class C, int ELT, bool TP, bool SPLIT, int OUT>
-int launch_grad(const GradArgs& a, unsigned grid, hipStream_t s) {
+int launch_grad(GradArgs a, int I, int J, hipStream_t s) {
+    const unsigned grid = make_map(a.map, (I + C::BI - 1) / C::BI, (J + C::BJ - 1) / C::BJ, a.nsplit);
     CAPDEC_TRY(allow_lds(grad_kernel<C, ELT, TP, SPLIT, OUT>, C::LDS_BYTES));
-    grad_kernel<C, ELT, TP, SPLIT, OUT><<<grid, 256, C::LDS_BYTES, s>>>(a);
+    grad_kernel<C, ELT, TP, SPLIT, OUT><<<grid, C::THREADS, C::LDS_BYTES, s>>>(a);
     CAPDEC_LAUNCH_CHECK();
     return 0;
 }
@@ -751,8 +776,7 @@ int capdec_vocab_ce_forward(const capdec_vocab_ce* a, void* saved, size_t saved_
     g.X = View{k.px, (int64_t)p.xs, p.Mp, 0};
     g.b2 = k.b2; g.head = head; g.kt = p.xs / 32; g.Mp = p.Mp;
     g.part = (float2*)((char*)workspace + p.o_part);
-    const unsigned grid = make_map(g.map, p.Vp / Big::BI, p.Mp / Big::BJ, 1);
-#define LSE(E, S) launch_lse<Big, E, S>(g, grid, s)
+#define LSE(E, S) (p.wide_z ? launch_lse<Wide, E, S>(g, p.Vp, p.Mp, s) : launch_lse<Big, E, S>(g, p.Vp, p.Mp, s))
     CAPDEC_TRY(BY_TYPE(p, LSE));
 #undef LSE
     nll_kernel<<<(p.M + 3) / 4, 256, 0, s>>>(g.part, p.Vp / 256, p.Mp, a->x, a->ldx, a->W, a->ldw, a->bias, a->dtype, p.M, p.K,
@@ -798,8 +822,7 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
         g.b2 = (const float*)(sv + p.o_b2); g.head = head; g.kt = p.xs / 32; g.Mp = p.Mp;
         g.lse = (const float*)(sv + p.o_lse); g.dlt = (const float*)(sv + p.o_dlt); g.rw = rw; g.tgt = (const int*)(sv + p.o_tgt);
         g.g = G; g.ldg = (int64_t)p.piece * pl; g.dbp = dbias ? (float*)(ws + p.o_db) : nullptr; g.v0 = v0; g.piece = p.piece;
-        unsigned grid = make_map(g.map, words / Big::BI, p.Mp / Big::BJ, 1);
-#define DL(E, S) launch_dlogits<Big, E, S>(g, grid, s)
+#define DL(E, S) (p.wide_z ? launch_dlogits<Wide, E, S>(g, words, p.Mp, s) : launch_dlogits<Big, E, S>(g, words, p.Mp, s))
         CAPDEC_TRY(BY_TYPE(p, DL));
 #undef DL
         if (dx) {
@@ -808,8 +831,7 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
             d.Q = View{W + (int64_t)v0 * ldw, ldw, p.Kp, real};
             d.head = head; d.bh = bh; d.I = p.Mp; d.J = p.Kp; d.rows_live = 1; d.kt = words / kt; d.nsplit = p.sx;
             d.part = dxp; d.ldp = p.Kp; d.plane = (int64_t)p.Mp * p.Kp; d.add = v0 > 0;
-            grid = make_map(d.map, (p.Mp + Big::BI - 1) / Big::BI, (p.Kp + Big::BJ - 1) / Big::BJ, p.sx);
-#define DX(E, S) launch_grad<Big, E, false, S, 0>(d, grid, s)
+#define DX(E, S) (p.wide_dx ? launch_grad<Wide, E, false, S, 0>(d, p.Mp, p.Kp, s) : launch_grad<Big, E, false, S, 0>(d, p.Mp, p.Kp, s))
             CAPDEC_TRY(BY_TYPE(p, DX));
 #undef DX
         }
@@ -818,17 +840,16 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
             d.P = View{G, g.ldg, words, p.Mp};
             d.Q = View{px, (int64_t)p.xs, p.Kp, p.Mp};
             d.head = head; d.bh = bh; d.k_live = 1; d.nsplit = p.sw;
-            grid = make_map(d.map, words / Big::BI, (p.Kp + Big::BJ - 1) / Big::BJ, p.sw);
             if (p.sw == 1) {
                 d.I = real; d.J = p.K;
                 d.out = (char*)dW + (int64_t)v0 * lddw * (p.split ? 4 : 2); d.ldo = lddw; d.dtype = a->dtype;
-#define DW(E, S) launch_grad<Big, E, true, S, 1>(d, grid, s)
+#define DW(E, S) (p.wide_dw ? launch_grad<Wide, E, true, S, 1>(d, words, p.Kp, s) : launch_grad<Big, E, true, S, 1>(d, words, p.Kp, s))
                 CAPDEC_TRY(BY_TYPE(p, DW));
 #undef DW
             } else {
                 d.I = real; d.J = p.Kp;
                 d.part = (float*)(ws + p.o_dw); d.ldp = p.Kp; d.plane = (int64_t)p.piece * p.Kp;
-#define DW(E, S) launch_grad<Big, E, true, S, 0>(d, grid, s)
+#define DW(E, S) (p.wide_dw ? launch_grad<Wide, E, true, S, 0>(d, words, p.Kp, s) : launch_grad<Big, E, true, S, 0>(d, words, p.Kp, s))
                 CAPDEC_TRY(BY_TYPE(p, DW));
 #undef DW
             }
@@ -838,7 +859,7 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
             const int64_t items = (slabs > 1 ? (int64_t)real * ((p.K + 3) / 4) : 0) + (dbias ? real : 0);
             dw_kernel<<<blocks_for(items, 256, 8192), 256, 0, s>>>((const float*)(ws + p.o_dw), (int64_t)p.piece * p.Kp, slabs,
                                                                    p.Kp, real, p.K, head, bh, p.split, dW, lddw, a->dtype,
-                                                                   g.dbp, p.piece, dbias, v0);
+                                                                   g.dbp, p.piece, p.wide_z ? Wide::BJ : Big::BJ, dbias, v0);
             CAPDEC_LAUNCH_CHECK();
         }
     }
