@@ -45,8 +45,11 @@ __device__ __forceinline__ float from_bits(short b) {
     if (ELT == BF16) return (float)__builtin_bit_cast(__bf16, b);
     return (float)__builtin_bit_cast(_Float16, b);
 }
-// v = hi + lo in fp16; an infinite or not-a-number v stays that in hi
+// v = hi + lo in fp16; an infinite or not-a-number v stays that in hi.  v is made a rounded fp32 number first: where it is
+// a product, the compiler may round that straight to fp16 for hi and by way of fp32 for lo's difference, which are not
+// always the same number (an error of a whole fp16 step in one of some thousand values).
 __device__ __forceinline__ void split16(float v, short& hi, short& lo) {
+    asm("" : "+v"(v));
     const _Float16 h = (_Float16)v;
     const _Float16 l = (_Float16)(v - (float)h);
     hi = __builtin_bit_cast(short, h);

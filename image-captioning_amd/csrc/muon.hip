@@ -18,7 +18,8 @@ namespace {
 
 constexpr int MAX_BATCH = 32;             // matrices per launch (their descriptors are kernel arguments)
 constexpr size_t BATCH_BYTES = (size_t)1 << 30;
-constexpr int NORM_BLOCKS = 64;           // partial sums of squares per matrix
+constexpr int NORM_BLOCKS = 512;          // most partial sums of squares per matrix
+constexpr int CHUNK = 1024;               // columns a wavefront reads of a row at a time
 
 struct Item {
     const void* src;                      // orthogonalize: the matrix;  update: the gradient
@@ -66,29 +67,68 @@ __device__ __forceinline__ void store_as(void* p, int64_t i, float v, int dtype)
     else ((short*)p)[i] = dtype == CAPDEC_BF16 ? to_bits<BF16>(v) : to_bits<F16>(v);
 }
 
+// four consecutive elements, aligned to their own size
+__device__ __forceinline__ void load4(const void* p, int64_t i, int dtype, float* v) {
+    if (dtype == CAPDEC_F32) {
+        const f32x4 q = *reinterpret_cast<const f32x4*>((const float*)p + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = q[e];
+    } else {
+        const s16x4 q = *reinterpret_cast<const s16x4*>((const short*)p + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = dtype == CAPDEC_BF16 ? from_bits<BF16>(q[e]) : from_bits<F16>(q[e]);
+    }
+}
+
 struct Momentum {                         // update only (on != 0)
     int on, nesterov;
     float mu, grad_scale;
 };
 
+// the next momentum; u: the gradient in, U out
+__device__ __forceinline__ float advance(const Momentum& mo, float m, float& u) {
+    u *= mo.grad_scale;
+    m = fmaf(mo.mu, m, u);
+    u = mo.nesterov ? fmaf(mo.mu, m, u) : m;
+    return m;
+}
+
 // Sums of squares of U in double (no square over- or underflows), one partial per block in a fixed order; an update
-// advances its momentum here.  A wavefront per row.
-__global__ __launch_bounds__(256) void norm_kernel(Batch b, int rows, int cols, int dtype, Momentum mo, double* __restrict__ part) {
+// advances its momentum here.  A wavefront per row and 1024 columns, four elements of each lane in flight when the
+// rows are aligned.
+__global__ __launch_bounds__(256) void norm_kernel(Batch b, int rows, int cols, int dtype, Momentum mo, int vec,
+                                                   double* __restrict__ part) {
     const Item& it = b.it[blockIdx.y];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int cpr = (cols + CHUNK - 1) / CHUNK;
     double s = 0.0;
-    for (int r = blockIdx.x * 4 + wave; r < rows; r += NORM_BLOCKS * 4)
-        for (int c = lane; c < cols; c += 64) {
-            float u = load_as_f32(it.src, (int64_t)r * it.lds + c, dtype);
-            if (mo.on) {
-                u *= mo.grad_scale;
-                float* q = it.mom + (int64_t)r * it.ldm + c;
-                const float m = fmaf(mo.mu, *q, u);
-                *q = m;
-                u = mo.nesterov ? fmaf(mo.mu, m, u) : m;
+    for (int64_t t = (int64_t)blockIdx.x * 4 + wave; t < (int64_t)rows * cpr; t += (int64_t)gridDim.x * 4) {
+        const int r = (int)(t / cpr), c0 = (int)(t - (int64_t)r * cpr) * CHUNK, c1 = min(cols, c0 + CHUNK);
+        const int64_t src = (int64_t)r * it.lds, mom = (int64_t)r * it.ldm;
+        if (vec) {
+#pragma unroll
+            for (int k = 0; k < CHUNK / 256; ++k) {
+                const int c = c0 + k * 256 + lane * 4;
+                if (c >= c1) break;
+                float u[4];
+                load4(it.src, src + c, dtype, u);
+                if (mo.on) {
+                    f32x4 m = *reinterpret_cast<const f32x4*>(it.mom + mom + c);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) m[e] = advance(mo, m[e], u[e]);
+                    *reinterpret_cast<f32x4*>(it.mom + mom + c) = m;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s += (double)u[e] * (double)u[e];
             }
-            s += (double)u * (double)u;
+        } else {
+            for (int c = c0 + lane; c < c1; c += 64) {
+                float u = load_as_f32(it.src, src + c, dtype);
+                if (mo.on) it.mom[mom + c] = advance(mo, it.mom[mom + c], u);
+                s += (double)u * (double)u;
+            }
         }
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     __shared__ double ws[4];
@@ -97,12 +137,13 @@ __global__ __launch_bounds__(256) void norm_kernel(Batch b, int rows, int cols, 
     if (threadIdx.x == 0) part[blockIdx.y * NORM_BLOCKS + blockIdx.x] = (ws[0] + ws[1]) + (ws[2] + ws[3]);
 }
 
-// X_0 2^sx = U 2^sx / (|U| + eps) into the padded two-number layout
+// X_0 2^sx = U 2^sx / (|U| + eps) into the padded layout
 __global__ __launch_bounds__(256) void normalise_kernel(Batch b, int rows, int cols, int rp, int cp, int dtype, Momentum mo,
-                                                        const double* __restrict__ part, float eps, float scale, int split,
-                                                        short* __restrict__ X, int64_t x_elems) {
+                                                        int vec, const double* __restrict__ part, int nparts, float eps,
+                                                        float scale, int split, short* __restrict__ X, int64_t x_elems) {
     const Item& it = b.it[blockIdx.y];
-    double s = part[blockIdx.y * NORM_BLOCKS + (threadIdx.x & 63)];
+    double s = 0.0;
+    for (int k = threadIdx.x & 63; k < nparts; k += 64) s += part[blockIdx.y * NORM_BLOCKS + k];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     const float inv = (float)((double)scale / (sqrt(s) + (double)eps));
@@ -110,20 +151,33 @@ __global__ __launch_bounds__(256) void normalise_kernel(Batch b, int rows, int c
     const int cpr = cp / 8;
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < (int64_t)rp * cpr; t += (int64_t)gridDim.x * 256) {
         const int r = (int)(t / cpr), c = (int)(t - (int64_t)r * cpr) * 8;
+        const int64_t src = (int64_t)r * it.lds + c, mom = (int64_t)r * it.ldm + c;
+        float u[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, m[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (r < rows) {
+            if (vec && c + 8 <= cols) {
+                if (!mo.on || mo.nesterov) {
+                    load4(it.src, src, dtype, u);
+                    load4(it.src, src + 4, dtype, u + 4);
+                }
+                if (mo.on) {
+                    load4(it.mom, mom, CAPDEC_F32, m);
+                    load4(it.mom, mom + 4, CAPDEC_F32, m + 4);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (c + e < cols) {
+                        u[e] = load_as_f32(it.src, src + e, dtype);
+                        if (mo.on) m[e] = it.mom[mom + e];
+                    }
+            }
+        }
         s16x8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            float u = 0.f;
-            if (r < rows && c + e < cols) {
-                u = load_as_f32(it.src, (int64_t)r * it.lds + c + e, dtype);
-                if (mo.on) {
-                    const float m = it.mom[(int64_t)r * it.ldm + c + e];
-                    u = mo.nesterov ? fmaf(mo.mu, m, u * mo.grad_scale) : m;
-                }
-                u *= inv;
-            }
+            if (mo.on) u[e] = mo.nesterov ? fmaf(mo.mu, m[e], u[e] * mo.grad_scale) : m[e];
             short h, l;
-            split16(u, h, l);
+            split16(u[e] * inv, h, l);
             hi[e] = h;
             lo[e] = l;
         }
@@ -288,11 +342,19 @@ int run_batch(const Batch& b, int nz, const Dims& d, const Iteration& n, int dty
     double sigma = 1.0;                           // bound of the iterate's singular values
     int sx = exponent_for(sigma);
     bool split = n.exact_steps > 0;
-    norm_kernel<<<dim3(NORM_BLOCKS, nz), 256, 0, s>>>(b, d.rows, d.cols, dtype, mo, part);
+    int vec = d.cols % 4 == 0;                    // every row of every matrix starts on four elements
+    for (int z = 0; z < nz && vec; ++z) {
+        const Item& it = b.it[z];
+        vec = it.lds % 4 == 0 && reinterpret_cast<uintptr_t>(it.src) % (dtype == CAPDEC_F32 ? 16 : 8) == 0 &&
+              (!mo.on || (it.ldm % 4 == 0 && capdec_aligned16(it.mom)));
+    }
+    const int64_t chunks = (int64_t)d.rows * ((d.cols + CHUNK - 1) / CHUNK);
+    const int nparts = (int)(chunks < 4 * NORM_BLOCKS ? (chunks + 3) / 4 : NORM_BLOCKS);
+    norm_kernel<<<dim3(nparts, nz), 256, 0, s>>>(b, d.rows, d.cols, dtype, mo, vec, part);
     const int64_t items = (int64_t)d.rp * (d.cp / 8);
     const unsigned blocks = (unsigned)(items / 256 + 1 < 1024 ? items / 256 + 1 : 1024);
-    normalise_kernel<<<dim3(blocks, nz), 256, 0, s>>>(b, d.rows, d.cols, d.rp, d.cp, dtype, mo, part, n.eps, ldexpf(1.f, sx),
-                                                      split, X[0], (int64_t)d.x_elems);
+    normalise_kernel<<<dim3(blocks, nz), 256, 0, s>>>(b, d.rows, d.cols, d.rp, d.cp, dtype, mo, vec, part, nparts, n.eps,
+                                                      ldexpf(1.f, sx), split, X[0], (int64_t)d.x_elems);
     CAPDEC_LAUNCH_CHECK();
     for (int k = 0; k < n.steps; ++k) {
         const int pl = split ? 2 : 1, kdiv = split ? 16 : 32;
@@ -351,6 +413,11 @@ int run_batch(const Batch& b, int nz, const Dims& d, const Iteration& n, int dty
     return 0;
 }
 
+// A bfloat16 result is rounded by 2^-9: its last two steps take one fp16 number per value, a third of the products.  Their
+// error, about 2^-12 a value and grown once by a, stays below that rounding (6.5e-4 against 1.7e-3 in norm for gradients
+// of a few strong directions over noise; 2.5e-3 where all but 16 of 512 directions are a thousandth of those).
+int exact_steps(int steps, int dtype) { return dtype == CAPDEC_BF16 ? (steps > 2 ? steps - 2 : 0) : steps; }
+
 // the iterate's bound must leave the powers of two in fp32's and fp16's range
 bool iteration_fits(const float* coeffs, int steps) {
     if (!coeffs || steps < 1 || steps > 32) return false;
@@ -383,7 +450,7 @@ int capdec_orthogonalize(const capdec_matrix* mats, int count, int rows, int col
         CAPDEC_REQUIRE(mats[k].src && mats[k].dst && (rows == 1 || (mats[k].ld_src >= cols && mats[k].ld_dst >= cols)));
     if (!capdec_aligned16(workspace)) return CAPDEC_EALIGN;
     if (workspace_bytes < capdec_orthogonalize_workspace_bytes(count, rows, cols)) return CAPDEC_ENOMEM;
-    const Iteration n{steps, steps, coeffs[0], coeffs[1], coeffs[2], eps};
+    const Iteration n{steps, exact_steps(steps, dtype), coeffs[0], coeffs[1], coeffs[2], eps};
     for (int k = 0; k < count; k += d.batch) {
         const int nz = count - k < d.batch ? count - k : d.batch;
         Batch b{};

@@ -32,7 +32,7 @@ struct Plan {
     int sx, sw;                                  // contraction splits of dx and dW
     bool wide_z, wide_dx, wide_dw;               // tiles of 256 x 256 for the logits, dx and dW
     size_t o_order, o_slot, o_tgt, o_lse, o_dlt, o_b2, o_x, o_w, saved;
-    size_t o_part, fwd;
+    size_t o_part, o_amax, fwd;
     size_t o_rw, o_g, o_dx, o_dw, o_db, bwd;
 };
 
@@ -84,6 +84,7 @@ bool make_plan(const capdec_vocab_ce* a, Plan& p) {
 
     at = 256;
     p.o_part = take(at, (size_t)(p.Vp / 256) * p.Mp * 8);
+    p.o_amax = take(at, 2 * 512 * 4);
     p.fwd = at;
 
     const int es = p.split ? 4 : 2;
@@ -188,11 +189,12 @@ __device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int dtype
     return dtype == CAPDEC_BF16 ? from_bits<BF16>(b) : from_bits<F16>(b);
 }
 
-// largest finite magnitude of x (counted rows) and W; blockIdx.y picks the operand.  atomicMax of non-negative floats'
-// bits: the order does not matter.
+// Largest finite magnitude of x (counted rows) and W, one partial per block; blockIdx.y picks the operand.  A wavefront
+// reads four rows at a time.
+constexpr int AMAX_BLOCKS = 512;
 __global__ __launch_bounds__(256) void amax_kernel(const float* __restrict__ x, int64_t ldx, const float* __restrict__ W,
-                                                   int64_t ldw, int V, int K, Head* __restrict__ head,
-                                                   const int* __restrict__ order, int vec) {
+                                                   int64_t ldw, int V, int K, const Head* __restrict__ head,
+                                                   const int* __restrict__ order, int vec, float* __restrict__ part) {
     const bool isw = blockIdx.y != 0;
     const int rows = isw ? V : head->count;
     float m = 0.f;
@@ -201,26 +203,35 @@ __global__ __launch_bounds__(256) void amax_kernel(const float* __restrict__ x, 
         v = fabsf(v);
         if (v < INFINITY) m = fmaxf(m, v);
     };
-    for (int r = wave; r < rows; r += nw) {
-        const float* row = isw ? W + (int64_t)r * ldw : x + (int64_t)order[r] * ldx;
+    for (int r = wave; r < rows; r += 4 * nw) {
+        const float* row[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int q = min(r + k * nw, rows - 1);             // the last row again past the end
+            row[k] = isw ? W + (int64_t)q * ldw : x + (int64_t)order[q] * ldx;
+        }
         if (vec) {
             for (int c = lane * 4; c < K; c += 256) {
-                const f32x4 v = *reinterpret_cast<const f32x4*>(row + c);
+                f32x4 v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) see(v[e]);
+                for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const f32x4*>(row[k] + c);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) see(v[k][e]);
             }
         } else {
-            for (int c = lane; c < K; c += 64) see(row[c]);
+            for (int c = lane; c < K; c += 64) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) see(row[k][c]);
+            }
         }
     }
     m = wave_max(m);
     __shared__ float wm[4];
     if (lane == 0) wm[threadIdx.x >> 6] = m;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        m = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
-        if (m > 0.f) atomicMax(isw ? &head->amax_w : &head->amax_x, __float_as_uint(m));
-    }
+    if (threadIdx.x == 0) part[blockIdx.y * AMAX_BLOCKS + blockIdx.x] = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
 }
 
 // Packed operands: rows of whole k-tiles, zero beyond the width; x by slot (zero rows up to the next multiple of 32
@@ -234,11 +245,37 @@ struct PackArgs {
     const int* order;
     short* px; short* pw; float* b2;
     int64_t nx, nw;           // 8-column chunks of x and W
+    const float* part;        // split operands: the partial maxima
+    int nparts;
 };
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     const int64_t total = a.nx + a.nw + a.Vp;
     const int cpr = a.Kp / 8;
     const int count = a.head->count;
+    float scale[2] = {1.f, 1.f};
+    if (a.split) {                                  // every block joins the partial maxima for itself; the first notes them
+        __shared__ float wm[2][4];
+        float m[2] = {0.f, 0.f};
+        for (int k = threadIdx.x; k < a.nparts; k += 256) {
+            m[0] = fmaxf(m[0], a.part[k]);
+            m[1] = fmaxf(m[1], a.part[AMAX_BLOCKS + k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            m[k] = wave_max(m[k]);
+            if ((threadIdx.x & 63) == 0) wm[k][threadIdx.x >> 6] = m[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            m[k] = fmaxf(fmaxf(wm[k][0], wm[k][1]), fmaxf(wm[k][2], wm[k][3]));
+            scale[k] = pow2(scale_exp(__float_as_uint(m[k])));
+        }
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            a.head->amax_x = __float_as_uint(m[0]);
+            a.head->amax_w = __float_as_uint(m[1]);
+        }
+    }
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
         if (t >= a.nx + a.nw) {
             const int v = (int)(t - a.nx - a.nw);
@@ -263,7 +300,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
             }
             *reinterpret_cast<s16x8*>(dst + c) = o;
         } else {
-            const float s = pow2(scale_exp(isw ? a.head->amax_w : a.head->amax_x));
+            const float s = scale[isw];
             float v[8];
             if (!zero && a.vec && c + 8 <= a.K) {
                 const f32x4* q = reinterpret_cast<const f32x4*>((const float*)src + base + c);
@@ -755,12 +792,13 @@ int capdec_vocab_ce_forward(const capdec_vocab_ce* a, void* saved, size_t saved_
     compact_kernel<<<1, 1024, 0, s>>>(a->targets, a->M, a->V, a->ignore_index, head, order, slot, tgt);
     const int esz = p.split ? 4 : 2;
     const int vec = capdec_aligned16(a->x) && capdec_aligned16(a->W) && a->ldx * esz % 16 == 0 && a->ldw * esz % 16 == 0;
-    if (p.split) {
-        const unsigned bx = blocks_for((int64_t)(p.V > p.M ? p.V : p.M), 4, 2048);
-        amax_kernel<<<dim3(bx, 2), 256, 0, s>>>((const float*)a->x, a->ldx, (const float*)a->W, a->ldw, p.V, p.K, head, order,
-                                                vec && p.K % 4 == 0);
-    }
     PackArgs k{};
+    if (p.split) {
+        k.nparts = (int)blocks_for((int64_t)(p.V > p.M ? p.V : p.M), 4, AMAX_BLOCKS);
+        k.part = (const float*)((char*)workspace + p.o_amax);
+        amax_kernel<<<dim3(k.nparts, 2), 256, 0, s>>>((const float*)a->x, a->ldx, (const float*)a->W, a->ldw, p.V, p.K, head,
+                                                      order, vec && p.K % 4 == 0, (float*)((char*)workspace + p.o_amax));
+    }
     k.x = a->x; k.ldx = a->ldx; k.W = a->W; k.ldw = a->ldw; k.bias = a->bias;
     k.M = p.M; k.V = p.V; k.K = p.K; k.Kp = p.Kp; k.xs = p.xs; k.dtype = a->dtype; k.split = p.split; k.Vp = p.Vp;
     k.pack_w = p.pack_w; k.vec = vec;
