@@ -542,7 +542,18 @@ def vocab_logits_bwd(dec, x, dlogits, grads):
     return _lin_bwd(grads, "fc2", dec.fc2, dlogits, x)
 
 
-def vocab_loss(dec, x, targets, ignore_index=0, materialize=True, skip_ignored=True, rows=None):
+_ONES = {}
+
+
+def _one(device):
+    """The constant 1.0 of a device: the upstream gradient of a loss that is differentiated itself."""
+    t = _ONES.get(device)
+    if t is None:
+        t = _ONES[device] = torch.ones(1, device=device)
+    return t
+
+
+def vocab_loss(dec, x, targets, ignore_index=0, materialize=True, skip_ignored=True, rows=None, pieces=False):
     """Projection + CrossEntropyLoss(ignore_index) (reference train.py:216,254-256).
     Returns (loss [1] device tensor, saved state for ``vocab_loss_bwd``).
 
@@ -554,8 +565,14 @@ def vocab_loss(dec, x, targets, ignore_index=0, materialize=True, skip_ignored=T
     every gradient through them are exactly zero in the reference too.  Nothing is synchronised: the number of
     counted rows stays on the device and bounds the kernels' row and contraction ranges.
     materialize=False: fused log-sum-exp + NLL, no logits (evaluation loss; its backward recomputes the projection
-    tile-wise)."""
+    tile-wise).
+    pieces=True: no logits in either direction (``ops.vocab_ce_forward`` / ``vocab_ce_backward``): the gradient is formed for a
+    piece of the vocabulary at a time, on the 16-bit matrix cores from pairs of fp16 numbers per fp32 value.  Ignored rows
+    are left out on the device as above; ``rows`` is not needed, since the rows past it have an ignored target."""
     tg = targets.reshape(-1).contiguous()
+    if pieces:
+        _, loss, state = ops.vocab_ce_forward(x, dec.fc2.weight, dec.fc2.bias, tg, ignore_index)
+        return loss[:1], ("pieces", tg, ignore_index, state)
     if rows is not None:
         # x comes from a ragged stack: only its first rows[0] rows exist, the dead rows are gone already
         M, V = tg.numel(), dec.fc2.weight.shape[0]
@@ -586,7 +603,14 @@ def vocab_loss(dec, x, targets, ignore_index=0, materialize=True, skip_ignored=T
 
 
 def vocab_loss_bwd(dec, x, saved, grads):
-    """d(loss)/dx and the fc2 gradients from what ``vocab_loss`` saved."""
+    """d(loss)/dx and the fc2 gradients from what ``vocab_loss`` saved (the form without logits writes the fc2 gradients,
+    the others add to them)."""
+    if saved[0] == "pieces":
+        _, tg, ignore_index, state = saved
+        W, b = dec.fc2.weight, dec.fc2.bias
+        dx, _, _ = ops.vocab_ce_backward(x, W, b, tg, state, grad=_one(x.device), ignore_index=ignore_index,
+                                         dW=_new(grads, "fc2.weight", W), db=None if b is None else _new(grads, "fc2.bias", b))
+        return dx
     if saved[0] == "rows":
         _, dlogits, rows = saved
         return _lin_bwd(grads, "fc2", dec.fc2, dlogits, x, rows=rows)

@@ -20,7 +20,8 @@ def load_reference_checkpoint(path_or_dict, model, trainer=None):
     """Load a reference checkpoint into ``model`` (in place; with a ``CaptionTrainer`` the parameters are views of
     its flat buffer, which therefore receives the weights).  Returns the stored global step.
 
-    With ``trainer`` the Adam moments are restored too.  The reference's optimizer state is keyed by parameter
+    With ``trainer`` the Adam moments are restored too, and the momenta of the matrices that a trainer with
+    ``optimizer="muon"`` steps (entry ``"muon"`` of a checkpoint that such a trainer wrote, by parameter name).  The reference's optimizer state is keyed by parameter
     index in ``model.parameters()`` order of ITS model (backbone first); the index of a name is recovered as its rank
     among the state_dict keys that are not buffers (``running_*``, ``num_batches_tracked``, ``positional_encoding.pe``).
     Parameters without a stored state (the frozen backbone never gets one) are skipped."""
@@ -39,7 +40,16 @@ def load_reference_checkpoint(path_or_dict, model, trainer=None):
         state = ckpt["optimizer"].get("state", {})
         prefix = "decoderRNN." if core is not None else ""
         steps = set()
+        momenta = ckpt.get("muon", {})
         for name, grad_view in trainer.grads.items():
+            if name in trainer.muon_names:                 # a checkpoint written with Adam has no momentum for it: zero
+                a = (grad_view.data_ptr() - trainer.flat_g.data_ptr()) // 4
+                mom = trainer.m[a:a + grad_view.numel()]
+                if prefix + name in momenta:
+                    mom.copy_(momenta[prefix + name].reshape(-1))
+                else:
+                    mom.zero_()
+                continue
             st = state.get(index_of.get(prefix + name, -1))
             if st is None:
                 continue
@@ -74,6 +84,9 @@ def save_reference_checkpoint(path, model, trainer=None, step=0, backbone_state=
         for name, grad_view in trainer.grads.items():
             a = (grad_view.data_ptr() - trainer.flat_g.data_ptr()) // 4
             n = grad_view.numel()
+            if name in trainer.muon_names:
+                out.setdefault("muon", {})[prefix + name] = trainer.m[a:a + n].detach().cpu().reshape(grad_view.shape).clone()
+                continue
             state[order.index(prefix + name)] = {
                 "step": torch.tensor(float(trainer.t)),
                 "exp_avg": trainer.m[a:a + n].detach().cpu().reshape(grad_view.shape).clone(),

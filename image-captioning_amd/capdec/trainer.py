@@ -90,7 +90,9 @@ class CaptionTrainer:
     _SEED_HEAD, _SEED_DECODER = 0x2545F4914F6CDD1D, 0
 
     def __init__(self, model, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, process_group=None, pad_idx=0, overlap=True,
-                 skip_dead_rows=True, wgrad_stream=None, graph=False, exercise_collectives=False, graph_cache=8):
+                 skip_dead_rows=True, wgrad_stream=None, graph=False, exercise_collectives=False, graph_cache=8,
+                 vocab_loss="logits", optimizer="adam", muon_momentum=0.95, muon_nesterov=True, muon_weight_decay=0.0,
+                 muon_rms=0.2):
         """overlap=True: one all-reduce per gradient segment on a communication stream of its own, issued as soon as the
         backward pass has enqueued that segment; overlap=False: a single all-reduce of the whole flat gradient buffer after the backward pass.
         skip_dead_rows: run the Transformer stack on the live prefix of every caption only (the positions from a
@@ -109,6 +111,14 @@ class CaptionTrainer:
         ``graph_cache`` captured shapes are kept (the reference pads every batch to its own longest caption,
         get_loader.py:184, so the shape changes from batch to batch: pad or bucket the captions to few lengths, or the
         step mostly runs launch by launch); the least recently used one is dropped.
+        vocab_loss: "logits" materialises the [rows, vocabulary] logits and turns them into their gradient in place; "pieces"
+        keeps no logits and forms the gradient for a piece of the vocabulary at a time (same loss and gradients to fp32's
+        rounding; less memory, and faster from a few thousand rows on).
+        optimizer: "adam" for every parameter; "muon" steps the matrices of the decoder layers and of the LSTM along their
+        orthogonalised momentum (``ops.muon_step`` with ``muon_momentum``, ``muon_nesterov``, ``muon_weight_decay``) and
+        everything else -- embedding, vocabulary projection, feature head, biases, norms -- with Adam.  Both share the
+        learning rate: an orthogonalised update is scaled to the root mean square ``muon_rms`` of its entries, 0.2 being
+        what Adam's updates usually have.
         exercise_collectives: issue every broadcast / all-reduce even in a one-rank process group (where each is the
         identity), so that the device-collective code path -- the communication stream, segment boundaries, stream
         ordering -- can run on a single GPU under RCCL."""
@@ -118,6 +128,12 @@ class CaptionTrainer:
         self._want_side = (os.environ.get("CAPDEC_WGRAD_STREAM", "1") == "1") if wgrad_stream is None else bool(wgrad_stream)
         self.side_stream = None
         self.betas, self.eps, self.pad_idx = betas, eps, pad_idx
+        if vocab_loss not in ("logits", "pieces") or optimizer not in ("adam", "muon"):
+            raise ValueError(f"capdec: vocab_loss must be 'logits' or 'pieces' and optimizer 'adam' or 'muon', got "
+                             f"{vocab_loss!r}, {optimizer!r}")
+        self.vocab_pieces, self.optimizer = vocab_loss == "pieces", optimizer
+        self.muon = dict(momentum=muon_momentum, nesterov=muon_nesterov, weight_decay=muon_weight_decay)
+        self.muon_rms = muon_rms
         self.graph = bool(graph)
         self._graphs = collections.OrderedDict()   # input shapes -> None (seen once, run eagerly) | captured step
         self._graph_cache = max(1, int(graph_cache))
@@ -160,6 +176,11 @@ class CaptionTrainer:
                 seg_names.append(first + [n for n in names if n not in first])
             seg_names.append(["decoder_embedding.weight"])
         seg_names.append([n for n in named if n.split(".")[0] in ("fc1", "fc_vit", "fc_cnn", "fc_yolo", "batchnorm")])
+        # Muon: a segment's matrices ahead of the rest of it (the order within each part stays, so stacked projections do
+        # too), which leaves Adam one run of the flat buffers per segment
+        self.muon_names = [n for seg in seg_names for n in seg if optimizer == "muon" and named[n].dim() == 2 and
+                           n.startswith(("decoder_layers.", "lstm."))]
+        seg_names = [[n for n in seg if n in self.muon_names] + [n for n in seg if n not in self.muon_names] for seg in seg_names]
         flat_names = [n for seg in seg_names for n in seg]
         missing = set(named) - set(flat_names)
         if missing:
@@ -170,6 +191,7 @@ class CaptionTrainer:
         self.m = torch.zeros(total, device=dev, dtype=torch.float32)
         self.v = torch.zeros(total, device=dev, dtype=torch.float32)
         self.grads, self.segments = {}, []
+        self.muon_groups, self.adam_runs = {}, []      # rows x cols -> (params, grads, momenta); (begin, end) of the buffers
         off = 0
         with torch.no_grad():
             for seg in seg_names:
@@ -182,7 +204,16 @@ class CaptionTrainer:
                     prm.data = view                       # the module now reads and updates the flat buffer
                     self.grads[n] = self.flat_g[off:off + k].view_as(prm)
                     prm.grad = self.grads[n]
-                    off += (k + 3) // 4 * 4               # keep every tensor 16-byte aligned
+                    end = off + (k + 3) // 4 * 4          # keep every tensor 16-byte aligned
+                    if n in self.muon_names:
+                        group = self.muon_groups.setdefault(tuple(prm.shape), ([], [], []))
+                        for lst, t in zip(group, (view, self.grads[n], self.m[off:off + k].view_as(prm))):
+                            lst.append(t)
+                    elif self.adam_runs and self.adam_runs[-1][1] == off:
+                        self.adam_runs[-1] = (self.adam_runs[-1][0], end)
+                    else:
+                        self.adam_runs.append((off, end))
+                    off = end
                 self.segments.append((start, off))
             self.flat_p[off:].zero_()
         # BatchNorm running statistics as views of one small buffer: DDP (broadcast_buffers=True, the default the
@@ -306,9 +337,15 @@ class CaptionTrainer:
                                f"(whole buffer, {self.flat_g.numel() * 4} bytes): {e}") from e
 
     def _adam(self):
+        """The optimizer step: Adam over its runs of the flat buffers (all of them without Muon), Muon over its matrices."""
         # DDP semantics: mean of the per-rank gradients
-        ops.adam_step_dev(self.flat_p, self.flat_g, self.m, self.v, self.state, self.betas[0], self.betas[1], self.eps,
-                          grad_scale=1.0 / self.world)
+        for a, b in self.adam_runs:
+            ops.adam_step_dev(self.flat_p[a:b], self.flat_g[a:b], self.m[a:b], self.v[a:b], self.state, self.betas[0],
+                              self.betas[1], self.eps, grad_scale=1.0 / self.world)
+        for (rows, cols), (p, g, m) in self.muon_groups.items():
+            # an orthogonalised matrix has entries of root mean square 1 / sqrt(max(rows, cols))
+            ops.muon_step(p, g, m, state=self.state, update_scale=self.muon_rms * max(rows, cols) ** 0.5,
+                          grad_scale=1.0 / self.world, **self.muon)
 
     def step(self, feats, captions):
         """feats: precomputed backbone features [B,D]; captions [B,T+1] int64 (inputs [:, :-1], targets [:, 1:]).
@@ -380,7 +417,7 @@ class CaptionTrainer:
         sdev = self.state.seed_dev
         x0, htape = AG.head_forward(rnn, [(rnn.fc1, 0, feats.shape[1])], feats, True, self._SEED_HEAD, seed_dev=sdev)
         h, tape = AG.rnn_forward(rnn, x0, ids, p, self._SEED_DECODER, seed_dev=sdev)
-        loss, saved = AG.vocab_loss(rnn, h, tgt.t().contiguous(), self.pad_idx)      # rows of h are time-major
+        loss, saved = AG.vocab_loss(rnn, h, tgt.t().contiguous(), self.pad_idx, pieces=self.vocab_pieces)      # rows of h are time-major
         works = []
         dh = AG.vocab_loss_bwd(rnn, h, saved, self.grads)
         self._reduce_segment(0, works)
@@ -411,9 +448,9 @@ class CaptionTrainer:
             ids, tgt = ids.contiguous(), tgt.contiguous()
         x, tape = AG.tf_forward(model, enc, ids, p, self._SEED_DECODER, ragged=rg, seed_dev=sdev)
         if rg is not None:
-            loss, saved = AG.vocab_loss(model, x, rg.targets_c, self.pad_idx, rows=rg.rows)
+            loss, saved = AG.vocab_loss(model, x, rg.targets_c, self.pad_idx, rows=rg.rows, pieces=self.vocab_pieces)
         else:
-            loss, saved = AG.vocab_loss(model, x, tgt, self.pad_idx)
+            loss, saved = AG.vocab_loss(model, x, tgt, self.pad_idx, pieces=self.vocab_pieces)
         # ---- backward, gradient exchange overlapped segment by segment ----
         works = []
         dx = AG.vocab_loss_bwd(model, x, saved, self.grads)
