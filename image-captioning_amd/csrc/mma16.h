@@ -138,31 +138,48 @@ struct Operand {
 // SPREAD: the loads of a later k-tile are issued between the matrix instructions, at raised priority, which suits
 // workgroups that share a CU (256 x 128: 223 against 243 us for 7424 x 10000 x 512 in fp32); else ahead of them, with the
 // LDS reads spread instead (256 x 256: 1076 against 1090 us for 8192 x 32768 x 2048 in bf16, gradients 941 against 1041).
-template <int WI_, int WJ_, int TI_, int TJ_, int STAGES_, bool SPREAD_>
+// KG: groups of WI x WJ wavefronts that share a tile's k-tiles in turn and add their sums through LDS at the end, for launches
+// that leave CUs idle: a k-tile's way through LDS takes some 750 cycles however deep the ring, so 512 x 512 x 512 in 64
+// workgroups went from 12 us with one group (and eight buffers) to KGTIME us with four.
+template <int WI_, int WJ_, int TI_, int TJ_, int STAGES_, bool SPREAD_, int KG_ = 1>
 struct Tile {
     static constexpr int WI = WI_, WJ = WJ_, TI = TI_, TJ = TJ_, STAGES = STAGES_;
     static constexpr bool SPREAD = SPREAD_;
+    static constexpr int KG = KG_;
     static constexpr int BI = 32 * WI * TI, BJ = 32 * WJ * TJ;
-    static constexpr int WAVES = WI * WJ, THREADS = 64 * WAVES;
+    static constexpr int WAVES = WI * WJ, GROUP = 64 * WAVES, THREADS = GROUP * KG;
     static constexpr int STAGE = (BI + BJ) * 32;              // 16-bit elements of one ring buffer
-    static constexpr int LDS_BYTES = STAGES * STAGE * 2;
+    static constexpr int LDS_BYTES = KG * STAGES * STAGE * 2;
+    static_assert((KG - 1) * GROUP * TI * TJ * 64 <= LDS_BYTES, "the groups' sums do not fit");
 };
 typedef Tile<2, 4, 4, 2, 4, false> Wide;    // 256 x 256: 128 KiB of LDS, one workgroup per CU
 typedef Tile<2, 2, 4, 2, 3, true> Big;     // 256 x 128: 72 KiB, two workgroups per CU
 typedef Tile<2, 2, 2, 2, 3, true> Mid;     // 128 x 128: 48 KiB, three
-typedef Tile<2, 2, 1, 1, 3, false> Small;   //  64 x  64: 24 KiB
+typedef Tile<2, 2, 1, 1, 3, false> Small;      //  64 x  64: 24 KiB
+typedef Tile<2, 2, 1, 1, 3, false, 4> Deep;    //  64 x  64 by four groups: 96 KiB
 
-// Adds k-tiles [kt0, kt1) of the tile at (i0, j0) onto zero.  Ends behind a barrier: the caller may reuse `lds`.
+// Waits until at most min(ahead, MOST) k-tiles of PER loads each are in flight and this wavefront's LDS reads are done,
+// then for the workgroup.
+template <int MOST, int PER>
+__device__ __forceinline__ void wait_tiles(int ahead) {
+    static_assert(MOST * PER < 64, "vmcnt counts to 63");
+    if (MOST == 0 || ahead >= MOST) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(MOST * PER) : "memory");
+    else wait_tiles<(MOST > 0 ? MOST - 1 : 0), PER>(ahead);
+}
+
+// Sums k-tiles [kt0, kt1) of the tile at (i0, j0); the sums are the first group's.  Ends behind a barrier: the caller may
+// reuse `lds`.
 template <class C, int ELT, bool TP, bool TQ, bool SPLIT>
 __device__ __forceinline__ void contract(const View& P, const View& Q, int i0, int j0, int kt0, int kt1, short* lds,
                                          f32x16 (&acc)[C::TI][C::TJ]) {
     using OpP = Operand<C::BI, TP, SPLIT>;
     using OpQ = Operand<C::BJ, TQ, SPLIT>;
     constexpr int W = C::WAVES, S = C::STAGES, NPW = (OpP::PIECES + OpQ::PIECES) / W;
-    static_assert(S == 3 || S == 4, "the waits below count for these ring depths");
     static_assert(OpP::PIECES % W == 0 && OpQ::PIECES % W == 0, "pieces do not divide over the wavefronts");
+    constexpr int KG = C::KG;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / C::GROUP) : 0;
+    const int wave = __builtin_amdgcn_readfirstlane((threadIdx.x % C::GROUP) >> 6);
     const int wi = wave / C::WJ, wj = wave % C::WJ;
 #pragma unroll
     for (int ti = 0; ti < C::TI; ++ti)
@@ -180,7 +197,7 @@ __device__ __forceinline__ void contract(const View& P, const View& Q, int i0, i
                                          : OpQ::source(Q, j0, kt, piece - OpP::PIECES, lane);
         }
     };
-    const int64_t stepP = OpP::step(P), stepQ = OpQ::step(Q);
+    const int64_t stepP = OpP::step(P) * KG, stepQ = OpQ::step(Q) * KG;
     // the first k-tile that reaches past a T operand's rows: its addresses are clamped one by one
     const int ragged = min(TP ? P.klim / OpP::KT : kt1, TQ ? Q.klim / OpQ::KT : kt1);
     // one of this wavefront's pieces of k-tile kt
@@ -211,13 +228,15 @@ __device__ __forceinline__ void contract(const View& P, const View& Q, int i0, i
             for (int ti = 0; ti < C::TI; ++ti) a[hf][ti] = OpP::frag(ip, (wi * C::TI + ti) * 32, hf, lane);
         }
         if (C::SPREAD) __builtin_amdgcn_sched_barrier(0);
-        constexpr int TERMS = SPLIT ? 3 : 2, N = TERMS * C::TI * C::TJ, EVERY = N / NPW > 0 ? N / NPW : 1;
+        // one 32x32 block per wavefront: the fourth product, lo*lo, costs nothing there, and small matrices have no long sums
+        // in which the other roundings drown its loss
+        constexpr int TERMS = SPLIT ? (C::TI * C::TJ == 1 ? 4 : 3) : 2, N = TERMS * C::TI * C::TJ, EVERY = N / NPW > 0 ? N / NPW : 1;
         static_assert(!C::SPREAD || N >= NPW, "not every piece would be issued");
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int t = n / (C::TI * C::TJ), ti = n / C::TJ % C::TI, tj = n % C::TJ;
-            // SPLIT: hi*hi, hi*lo, lo*hi
-            acc[ti][tj] = mfma<ELT>(a[SPLIT ? t == 2 : t][ti], b[SPLIT ? t == 1 : t][tj], acc[ti][tj]);
+            // SPLIT: hi*hi, hi*lo, lo*hi, lo*lo
+            acc[ti][tj] = mfma<ELT>(a[SPLIT ? t >> 1 : t][ti], b[SPLIT ? t & 1 : t][tj], acc[ti][tj]);
             if (C::SPREAD && n % EVERY == 0 && n / EVERY < NPW) {
                 __builtin_amdgcn_sched_barrier(0);
                 if (more) issue_piece(buf, n / EVERY);
@@ -225,31 +244,34 @@ __device__ __forceinline__ void contract(const View& P, const View& Q, int i0, i
             }
         }
     };
-    short* rd = lds;                          // the buffer of tile kt
-    short* wr = lds + (S - 1) * C::STAGE;     // the buffer of tile kt + S - 1
+    // group g takes the tiles kt0 + g, kt0 + g + KG, ...: `mine` of them, in as many rounds as group 0 needs
+    const int first = kt0 + group, rounds = (kt1 - kt0 + KG - 1) / KG;
+    const int mine = KG == 1 ? rounds : max(0, (kt1 - first + KG - 1) / KG);
+    short* const ring = lds + group * S * C::STAGE;
+    short* rd = ring;                          // the buffer of this round's tile
+    short* wr = ring + (S - 1) * C::STAGE;     // the buffer of the tile S - 1 rounds later
 #pragma unroll
     for (int t = 0; t < S - 1; ++t)
-        if (kt0 + t < kt1) {
-            if (t == 0) seek(kt0);
-            issue(lds + t * C::STAGE, kt0 + t);
+        if (t < mine) {
+            if (t == 0) seek(first);
+            issue(ring + t * C::STAGE, first + t * KG);
         }
-    for (int kt = kt0; kt < kt1; ++kt) {
-        // this wavefront's pieces of tile kt have landed (those of later tiles may stay in flight, loads retire in order)
-        // and it is done reading the buffer that tile kt + S - 1 goes to; the barrier says so for all wavefronts
-        if (kt + S - 2 < kt1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * NPW) : "memory");
-        else if (S > 3 && kt + S - 3 < kt1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 3) * NPW) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    for (int it = 0; it < rounds; ++it) {
+        // this wavefront's pieces of its tile have landed (those of later tiles may stay in flight, loads retire in order)
+        // and it is done reading the buffer that the next loads go to; the barrier says so for all wavefronts
+        wait_tiles<S - 2, NPW>(mine - 1 - it);
         __builtin_amdgcn_sched_barrier(0);
-        const bool more = kt + S - 1 < kt1;
+        const bool more = it + S - 1 < mine;
+        const int later = first + (it + S - 1) * KG;
         if (C::SPREAD) {
-            if ((TP || TQ) && more && kt + S - 1 >= ragged) seek(kt + S - 1);
+            if ((TP || TQ) && more && later >= ragged) seek(later);
             __builtin_amdgcn_s_setprio(1);
             compute(rd, wr, more);
             __builtin_amdgcn_s_setprio(0);
         } else {
-            if (more) issue(wr, kt + S - 1);
+            if (more) issue(wr, later);
             __builtin_amdgcn_sched_barrier(0);
-            compute(rd, wr, more);
+            if (KG == 1 || it < mine) compute(rd, wr, more);
             // the first half's LDS reads, then one read between matrix instructions
             constexpr int READS = C::TI * (TP ? 2 : 1) + C::TJ * (TQ ? 2 : 1);
             __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
@@ -258,13 +280,31 @@ __device__ __forceinline__ void contract(const View& P, const View& Q, int i0, i
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
-            __builtin_amdgcn_sched_group_barrier(0x008, (SPLIT ? 3 : 2) * C::TI * C::TJ - READS, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 4 * C::TI * C::TJ, 0);      // the rest
         }
         __builtin_amdgcn_sched_barrier(0);
         wr = rd;
-        rd = rd == lds + (S - 1) * C::STAGE ? lds : rd + C::STAGE;
+        rd = rd == ring + (S - 1) * C::STAGE ? ring : rd + C::STAGE;
     }
     __syncthreads();
+    if (KG > 1) {
+        constexpr int PER = C::TI * C::TJ * 16 * C::GROUP;       // floats of one group
+        float* const red = reinterpret_cast<float*>(lds) + threadIdx.x % C::GROUP;
+        if (group > 0) {
+#pragma unroll
+            for (int e = 0; e < C::TI * C::TJ * 16; ++e)
+                red[(group - 1) * PER + e * C::GROUP] = acc[e / 16 / C::TJ][e / 16 % C::TJ][e % 16];
+        }
+        __syncthreads();
+        if (group == 0) {
+#pragma unroll
+            for (int g = 0; g < KG - 1; ++g)
+#pragma unroll
+                for (int e = 0; e < C::TI * C::TJ * 16; ++e)
+                    acc[e / 16 / C::TJ][e / 16 % C::TJ][e % 16] += red[g * PER + e * C::GROUP];
+        }
+        __syncthreads();
+    }
 }
 
 // Workgroup -> tile.  Workgroup ids go round-robin to the 8 XCDs, each with an L2 of its own: XCD x takes the x-th

@@ -205,7 +205,7 @@ struct StepArgs {
 enum { INNER = 0, RESULT = 1, UPDATE = 2 };
 
 template <class C, bool TP, bool TQ, bool SPLIT, int OUT>
-__global__ __launch_bounds__(C::THREADS, 2) void step_kernel(StepArgs a) {
+__global__ __launch_bounds__(C::THREADS, C::KG > 1 ? 4 : 2) void step_kernel(StepArgs a) {
     extern __shared__ __attribute__((aligned(16))) short lds[];
     int ti_, tj_, z;
     if (!tile_of(a.map, blockIdx.x, ti_, tj_, z)) return;
@@ -215,6 +215,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void step_kernel(StepArgs a) {
     Q.p += z * a.strideQ;
     f32x16 acc[C::TI][C::TJ];
     contract<C, F16, TP, TQ, SPLIT>(P, Q, i0, j0, 0, a.kt, lds, acc);
+    if (threadIdx.x >= C::GROUP) return;
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));
     const int lane = tid & 63, wave = tid >> 6, wi = wave / C::WJ, wj = wave % C::WJ, h = lane >> 5;
@@ -231,15 +232,25 @@ __global__ __launch_bounds__(C::THREADS, 2) void step_kernel(StepArgs a) {
         for (int ti = 0; ti < C::TI; ++ti) {
             float v[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int i = i0 + (wi * C::TI + ti) * 32 + acc_row(e, h);
-                v[e] = a.alpha * acc[ti][tj][e];
-                if (R && i < a.I) {
-                    const short* q = R + (int64_t)i * a.ldr + js;
-                    float x = from_bits<F16>(q[0]);
-                    if (SPLIT) x += from_bits<F16>(q[16]);
-                    v[e] = fmaf(a.beta, x, v[e]);
+            for (int e = 0; e < 16; ++e) v[e] = a.alpha * acc[ti][tj][e];
+            if (R) {                       // every load first, without branches: one round trip
+                short hi[16], lo[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const short* q = R + (int64_t)min(i0 + (wi * C::TI + ti) * 32 + acc_row(e, h), a.I - 1) * a.ldr + js;
+                    hi[e] = q[0];
+                    lo[e] = SPLIT ? q[16] : (short)0;
                 }
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    v[e] = fmaf(a.beta, from_bits<F16>(hi[e]) + (SPLIT ? from_bits<F16>(lo[e]) : 0.f), v[e]);
+            }
+            float old[16];
+            if (OUT == UPDATE) {
+                const Item& it = a.b.it[z];
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    old[e] = ((const float*)it.dst)[(int64_t)min(i0 + (wi * C::TI + ti) * 32 + acc_row(e, h), a.I - 1) * it.ldd + j];
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -257,8 +268,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void step_kernel(StepArgs a) {
                     if (OUT == RESULT) {
                         store_as(it.dst, at, v[e], a.dtype);
                     } else {
-                        float* p = (float*)it.dst + at;
-                        *p = fmaf(-lr * a.scale, v[e], *p * (1.f - lr * a.decay));
+                        ((float*)it.dst)[at] = fmaf(-lr * a.scale, v[e], old[e] * (1.f - lr * a.decay));
                     }
                 }
             }
@@ -278,14 +288,15 @@ int launch(const StepArgs& a0, int nz, hipStream_t s) {
     return 0;
 }
 
-// the largest tiles that give every CU one, from 256x256 to 64x64
+// the largest tiles that give every CU one, from 256x256 to 64x64; fewer than two of those for each: four groups to a tile
 template <bool TP, bool TQ, bool SPLIT, int OUT>
 int launch_sized(const StepArgs& a, int nz, hipStream_t s) {
     auto tiles = [&](int bi, int bj) { return (int64_t)((a.I + bi - 1) / bi) * ((a.J + bj - 1) / bj) * nz; };
     if (tiles(256, 256) >= 256) return launch<Wide, TP, TQ, SPLIT, OUT>(a, nz, s);
     if (tiles(256, 128) >= 256) return launch<Big, TP, TQ, SPLIT, OUT>(a, nz, s);
     if (tiles(128, 128) >= 256) return launch<Mid, TP, TQ, SPLIT, OUT>(a, nz, s);
-    return launch<Small, TP, TQ, SPLIT, OUT>(a, nz, s);
+    if (tiles(64, 64) >= 512) return launch<Small, TP, TQ, SPLIT, OUT>(a, nz, s);
+    return launch<Deep, TP, TQ, SPLIT, OUT>(a, nz, s);
 }
 template <bool TP, bool TQ, int OUT>
 int launch_split(const StepArgs& a, bool split, int nz, hipStream_t s) {
