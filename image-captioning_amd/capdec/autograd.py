@@ -572,7 +572,7 @@ def vocab_loss(dec, x, targets, ignore_index=0, materialize=True, skip_ignored=T
     tg = targets.reshape(-1).contiguous()
     if pieces:
         _, loss, state = ops.vocab_ce_forward(x, dec.fc2.weight, dec.fc2.bias, tg, ignore_index)
-        return loss[:1], ("pieces", tg, ignore_index, state)
+        return loss[:1], ("pieces", state)
     if rows is not None:
         # x comes from a ragged stack: only its first rows[0] rows exist, the dead rows are gone already
         M, V = tg.numel(), dec.fc2.weight.shape[0]
@@ -606,11 +606,9 @@ def vocab_loss_bwd(dec, x, saved, grads):
     """d(loss)/dx and the fc2 gradients from what ``vocab_loss`` saved (the form without logits writes the fc2 gradients,
     the others add to them)."""
     if saved[0] == "pieces":
-        _, tg, ignore_index, state = saved
         W, b = dec.fc2.weight, dec.fc2.bias
-        dx, _, _ = ops.vocab_ce_backward(x, W, b, tg, state, grad=_one(x.device), ignore_index=ignore_index,
-                                         dW=_new(grads, "fc2.weight", W), db=None if b is None else _new(grads, "fc2.bias", b))
-        return dx
+        return ops.vocab_ce_backward(saved[1], grad=_one(x.device), dW=_new(grads, "fc2.weight", W),
+                                     db=None if b is None else _new(grads, "fc2.bias", b))[0]
     if saved[0] == "rows":
         _, dlogits, rows = saved
         return _lin_bwd(grads, "fc2", dec.fc2, dlogits, x, rows=rows)
@@ -689,26 +687,24 @@ class _VocabCrossEntropyFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, W, b, targets, ignore_index, reduction):
-        ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        ctx.reduction, ctx.state = reduction, None
+        ctx.save_for_backward(x, W, b)
         if x.shape[0] == 0:                       # no rows: the mean over none is NaN, every gradient zero
-            ctx.save_for_backward(x, W, b, targets, None)
             return {"none": x.new_zeros(0, dtype=torch.float32), "sum": x.new_zeros((), dtype=torch.float32),
                     "mean": x.new_full((), float("nan"), dtype=torch.float32)}[reduction]
-        nll, loss, saved = ops.vocab_ce_forward(x, W, b, targets, ignore_index, want_loss=reduction != "none")
-        ctx.save_for_backward(x, W, b, targets, saved)
+        nll, loss, ctx.state = ops.vocab_ce_forward(x, W, b, targets, ignore_index, want_loss=reduction != "none")
         return nll if reduction == "none" else loss[0 if reduction == "mean" else 1]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        x, W, b, targets, saved = ctx.saved_tensors
-        if saved is None:
+        x, W, b = ctx.saved_tensors               # raises where one was changed in place since
+        if ctx.state is None:
             return tuple(torch.zeros_like(t) if t is not None and n else None
                          for t, n in zip((x, W, b), ctx.needs_input_grad)) + (None, None, None)
         g = g.float().contiguous()
         up = dict(row_grad=g) if ctx.reduction == "none" else dict(grad=g, mean=ctx.reduction == "mean")
-        dx, dW, db = ops.vocab_ce_backward(x, W, b, targets, saved, ignore_index=ctx.ignore_index,
-                                           need=ctx.needs_input_grad[:3], **up)
+        dx, dW, db = ops.vocab_ce_backward(ctx.state, need=ctx.needs_input_grad[:3], **up)
         return dx, dW, db, None, None, None
 
 

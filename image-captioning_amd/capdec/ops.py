@@ -977,86 +977,92 @@ def adam_step_dev(p, g, m, v, state, beta1=0.9, beta2=0.999, eps=1e-8, grad_scal
 _DTYPE_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
-def _same_device(what, *tensors):
+def _same_device(what, tensors):
     """Every tensor on the current GPU (the wrappers launch on its current stream)."""
+    here = torch.cuda.current_device() if torch.cuda.is_available() else None
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != torch.cuda.current_device()):
-            raise RuntimeError(f"capdec {what}: every tensor must be on the current GPU (HIP device "
-                               f"{torch.cuda.current_device() if torch.cuda.is_available() else 'none'}), got {t.device}")
+        if t.get_device() != here:
+            raise RuntimeError(f"capdec {what}: every tensor must be on the current GPU (HIP device {here}), got {t.device}; "
+                               "there is no CPU path")
 
 
 def _bytes(n, device):
-    return torch.empty(int(n), device=device, dtype=torch.uint8)
+    return torch.empty(n, device=device, dtype=torch.uint8)
 
 
-def _vocab_ce_args(x, W, b, targets, ignore_index):
-    for t, name in ((x, "x"), (W, "W"), (targets, "targets")) + (((b, "bias"),) if b is not None else ()):
-        if not isinstance(t, torch.Tensor):
-            raise RuntimeError(f"capdec vocab_ce: {name} must be a tensor")
-    _same_device("vocab_ce", x, W, b, targets)
-    if x.dtype not in _DTYPE_CODE or W.dtype != x.dtype or (b is not None and b.dtype != x.dtype):
-        raise RuntimeError("capdec vocab_ce: x, W and bias must share one type, float32, bfloat16 or float16; got "
-                           f"{x.dtype}, {W.dtype}" + (f", {b.dtype}" if b is not None else ""))
-    if x.dim() != 2 or W.dim() != 2 or x.shape[1] != W.shape[1] or min(x.shape + W.shape) < 1:
-        raise RuntimeError(f"capdec vocab_ce: x [M,K] and W [V,K] expected, got {tuple(x.shape)} and {tuple(W.shape)}")
-    if targets.dtype != torch.int64 or targets.dim() != 1 or targets.shape[0] != x.shape[0] or not targets.is_contiguous():
-        raise RuntimeError(f"capdec vocab_ce: targets must be {x.shape[0]} contiguous int64 values, got {targets.dtype} "
-                           f"{tuple(targets.shape)}")
-    if b is not None and (b.dim() != 1 or b.shape[0] != W.shape[0] or not b.is_contiguous()):
-        raise RuntimeError(f"capdec vocab_ce: bias must hold {W.shape[0]} contiguous values, got {tuple(b.shape)}")
-    a = _lib.VocabCE(x=x.data_ptr(), W=W.data_ptr(), bias=_ptr(b), targets=targets.data_ptr(), ldx=_row_stride(x, "x"),
-                     ldw=_row_stride(W, "W"), ignore_index=ignore_index, M=x.shape[0], V=W.shape[0], K=x.shape[1],
-                     dtype=_DTYPE_CODE[x.dtype])
-    return a
+class VocabCEState:
+    """What ``vocab_ce_forward`` leaves for ``vocab_ce_backward``: the operands (neither of them may change in between), the
+    call's arguments, and the packed operands and row statistics in device memory."""
+    __slots__ = ("x", "W", "b", "targets", "args", "saved")
 
 
 def vocab_ce_forward(x, W, b, targets, ignore_index=0, want_loss=True):
     """Cross entropy of the projection x W^T + b, no logits kept: x [M,K], W [V,K], b [V] or None, all float32, bfloat16
     or float16 with unit column stride; targets [M] int64.  Returns (nll [M] fp32 with zeros for ignored rows,
-    loss [3] fp32 = (mean over the counted rows, sum, their number) or None, saved): ``saved`` goes to
-    ``vocab_ce_backward``."""
+    loss [3] fp32 = (mean over the counted rows, sum, their number) or None, the state for ``vocab_ce_backward``)."""
     lib = _lib.load()
-    a = _vocab_ce_args(x, W, b, targets, ignore_index)
-    saved_bytes = lib.capdec_vocab_ce_saved_bytes(byref(a))
-    ws_bytes = lib.capdec_vocab_ce_forward_workspace_bytes(byref(a))
+    ts = (x, W, targets) if b is None else (x, W, targets, b)
+    for t in ts:
+        if not isinstance(t, torch.Tensor):
+            raise RuntimeError(f"capdec vocab_ce: tensors expected, got {type(t).__name__}")
+    _same_device("vocab_ce", ts)
+    code = _DTYPE_CODE.get(x.dtype)
+    if code is None or W.dtype != x.dtype or (b is not None and b.dtype != x.dtype):
+        raise RuntimeError("capdec vocab_ce: x, W and bias must share one type, float32, bfloat16 or float16; got "
+                           f"{x.dtype}, {W.dtype}" + (f", {b.dtype}" if b is not None else ""))
+    if x.dim() != 2 or W.dim() != 2:
+        raise RuntimeError(f"capdec vocab_ce: x [M,K] and W [V,K] expected, got {tuple(x.shape)} and {tuple(W.shape)}")
+    (M, K), (V, k) = x.shape, W.shape
+    if k != K or min(M, K, V) < 1:
+        raise RuntimeError(f"capdec vocab_ce: x [M,K] and W [V,K] expected, got {tuple(x.shape)} and {tuple(W.shape)}")
+    if targets.dtype != torch.int64 or targets.dim() != 1 or targets.shape[0] != M or not targets.is_contiguous():
+        raise RuntimeError(f"capdec vocab_ce: targets must be {M} contiguous int64 values, got {targets.dtype} "
+                           f"{tuple(targets.shape)}")
+    if b is not None and (b.dim() != 1 or b.shape[0] != V or not b.is_contiguous()):
+        raise RuntimeError(f"capdec vocab_ce: bias must hold {V} contiguous values, got {tuple(b.shape)}")
+    a = _lib.VocabCE(x.data_ptr(), W.data_ptr(), _ptr(b), targets.data_ptr(), _row_stride(x, "x"), _row_stride(W, "W"),
+                     ignore_index, M, V, K, code)
+    r = byref(a)
+    saved_bytes, ws_bytes = lib.capdec_vocab_ce_saved_bytes(r), lib.capdec_vocab_ce_forward_workspace_bytes(r)
     if not saved_bytes:
-        raise RuntimeError(f"capdec vocab_ce: unsupported sizes M={a.M} V={a.V} K={a.K}")
+        raise RuntimeError(f"capdec vocab_ce: unsupported sizes M={M} V={V} K={K}")
     saved, ws = _bytes(saved_bytes, x.device), _bytes(ws_bytes, x.device)
-    out = torch.empty(a.M + 3, device=x.device, dtype=torch.float32)
-    nll, loss = out[:a.M], (out[a.M:] if want_loss else None)
-    _lib.check(lib.capdec_vocab_ce_forward(byref(a), saved.data_ptr(), saved_bytes, ws.data_ptr(), ws_bytes, nll.data_ptr(),
-                                           _ptr(loss), _stream()), "capdec_vocab_ce_forward")
-    return nll, loss, saved
+    out = torch.empty(M + 3, device=x.device, dtype=torch.float32)
+    p = out.data_ptr()
+    _lib.check(lib.capdec_vocab_ce_forward(r, saved.data_ptr(), saved_bytes, ws.data_ptr(), ws_bytes, p,
+                                           p + 4 * M if want_loss else None, _stream()), "capdec_vocab_ce_forward")
+    state = VocabCEState()
+    state.x, state.W, state.b, state.targets, state.args, state.saved = x, W, b, targets, a, saved
+    return out[:M], out[M:] if want_loss else None, state
 
 
-def vocab_ce_backward(x, W, b, targets, saved, grad=None, row_grad=None, mean=True, ignore_index=0, dx=None, dW=None, db=None,
-                      need=(True, True, True)):
+def vocab_ce_backward(state, grad=None, row_grad=None, mean=True, dx=None, dW=None, db=None, need=(True, True, True)):
     """Gradients of ``vocab_ce_forward``.  The upstream gradient is ``row_grad`` [M] fp32 (of nll) or ``grad``, a one-element
     fp32 tensor (of the mean, or with ``mean=False`` of the sum).  Returns (dx, dW, db) in the operands' type, written into
     the tensors given for them, or None where ``need`` says so."""
     lib = _lib.load()
-    a = _vocab_ce_args(x, W, b, targets, ignore_index)
     if (grad is None) == (row_grad is None):
         raise RuntimeError("capdec vocab_ce_backward: exactly one of grad and row_grad")
-    g = grad if grad is not None else row_grad
-    _same_device("vocab_ce_backward", _chk(g, name="upstream gradient"), saved)
-    if g.numel() != (1 if grad is not None else a.M) or not g.is_contiguous():
-        raise RuntimeError(f"capdec vocab_ce_backward: upstream gradient {tuple(g.shape)} does not fit {a.M} rows")
+    g = _chk(grad if grad is not None else row_grad, name="upstream gradient")
+    if g.numel() != (1 if grad is not None else state.args.M) or not g.is_contiguous():
+        raise RuntimeError(f"capdec vocab_ce_backward: upstream gradient {tuple(g.shape)} does not fit {state.args.M} rows")
     outs = []
-    for given, like, want, name in ((dx, x, need[0], "dx"), (dW, W, need[1], "dW"), (db, b, need[2], "db")):
+    for given, like, want, name in ((dx, state.x, need[0], "dx"), (dW, state.W, need[1], "dW"), (db, state.b, need[2], "db")):
         if like is None or not want:
             outs.append(None)
             continue
         if given is None:
             given = torch.empty(like.shape, device=like.device, dtype=like.dtype)
-        elif given.dtype != like.dtype or given.shape != like.shape or given.device != like.device or given.stride(-1) != 1:
-            raise RuntimeError(f"capdec vocab_ce_backward: {name} must be {like.dtype} {tuple(like.shape)} on {like.device}")
+        elif given.dtype != like.dtype or given.shape != like.shape or given.stride(-1) != 1:
+            raise RuntimeError(f"capdec vocab_ce_backward: {name} must be {like.dtype} {tuple(like.shape)}")
         outs.append(given)
+    _same_device("vocab_ce_backward", [t for t in (g, state.saved, *outs) if t is not None])
     dx, dW, db = outs
-    ws_bytes = lib.capdec_vocab_ce_backward_workspace_bytes(byref(a))
-    ws = _bytes(ws_bytes, x.device)
-    _lib.check(lib.capdec_vocab_ce_backward(byref(a), _chk(saved, torch.uint8, "saved").data_ptr(), saved.numel(),
-                                            ws.data_ptr(), ws_bytes, _ptr(row_grad), _ptr(grad), 1 if mean else 0, _ptr(dx),
+    r = byref(state.args)
+    ws_bytes = lib.capdec_vocab_ce_backward_workspace_bytes(r)
+    ws = _bytes(ws_bytes, g.device)
+    _lib.check(lib.capdec_vocab_ce_backward(r, state.saved.data_ptr(), state.saved.numel(), ws.data_ptr(), ws_bytes,
+                                            _ptr(row_grad), _ptr(grad), 1 if mean else 0, _ptr(dx),
                                             0 if dx is None else _row_stride(dx, "dx"), _ptr(dW),
                                             0 if dW is None else _row_stride(dW, "dW"), _ptr(db), _stream()),
                "capdec_vocab_ce_backward")
@@ -1115,7 +1121,7 @@ def orthogonalize(mats, steps=5, coeffs=NS_COEFFS, eps=1e-7, out=None):
     dst = _matrices("orthogonalize", out, tuple(_DTYPE_CODE))
     if [(t.shape, t.dtype) for t in src] != [(t.shape, t.dtype) for t in dst]:
         raise RuntimeError("capdec orthogonalize: out must match the matrices in shape and type")
-    _same_device("orthogonalize", *src, *dst)
+    _same_device("orthogonalize", src + dst)
     if len(dst) > 1:
         _distinct("orthogonalize", dst)
     co = _ns_coeffs(coeffs)
@@ -1152,7 +1158,7 @@ def muon_step(params, grads, momenta, lr=None, state=None, momentum=0.95, nester
     p, g, m = (_matrices("muon_step", t, f32) for t in (params, grads, momenta))
     if not ([t.shape for t in p] == [t.shape for t in g] == [t.shape for t in m]):
         raise RuntimeError("capdec muon_step: params, grads and momenta must match in number and shape")
-    _same_device("muon_step", *p, *g, *m)
+    _same_device("muon_step", p + g + m)
     _distinct("muon_step", p + m)
     co = _ns_coeffs(coeffs)
     for (rows, cols), idx in _by_shape(p).items():

@@ -205,7 +205,7 @@ struct StepArgs {
 enum { INNER = 0, RESULT = 1, UPDATE = 2 };
 
 template <class C, bool TP, bool TQ, bool SPLIT, int OUT>
-__global__ __launch_bounds__(C::THREADS, C::KG > 1 ? 4 : 2) void step_kernel(StepArgs a) {
+__global__ __launch_bounds__(C::THREADS, C::EU) void step_kernel(StepArgs a) {
     extern __shared__ __attribute__((aligned(16))) short lds[];
     int ti_, tj_, z;
     if (!tile_of(a.map, blockIdx.x, ti_, tj_, z)) return;

@@ -348,7 +348,7 @@ __device__ __forceinline__ float logit_scale(const Head* head) {
 }
 
 template <class C, int ELT, bool SPLIT>
-__global__ __launch_bounds__(C::THREADS, 2) void lse_kernel(LogitArgs a) {
+__global__ __launch_bounds__(C::THREADS, C::EU) void lse_kernel(LogitArgs a) {
     extern __shared__ __attribute__((aligned(16))) short lds[];
     int ti_, tj_, z;
     if (!tile_of(a.map, blockIdx.x, ti_, tj_, z)) return;
@@ -496,7 +496,7 @@ __global__ __launch_bounds__(1024) void weights_kernel(const float* __restrict__
 // that rows are stored 256 contiguous bytes at a time; on the way the targets' entries are put in, (p_t - 1) g as
 // expm1(log p_t) g, and each word's column is summed for the bias gradient.
 template <class C, int ELT, bool SPLIT>
-__global__ __launch_bounds__(C::THREADS, 2) void dlogits_kernel(LogitArgs a) {
+__global__ __launch_bounds__(C::THREADS, C::EU) void dlogits_kernel(LogitArgs a) {
     extern __shared__ __attribute__((aligned(16))) short lds[];
     int ti_, tj_, z;
     if (!tile_of(a.map, blockIdx.x, ti_, tj_, z)) return;
@@ -627,7 +627,7 @@ __device__ __forceinline__ void store_as(void* p, int64_t i, float v, int dtype)
 }
 
 template <class C, int ELT, bool TP, bool SPLIT, int OUT>
-__global__ __launch_bounds__(C::THREADS, 2) void grad_kernel(GradArgs a) {
+__global__ __launch_bounds__(C::THREADS, C::EU) void grad_kernel(GradArgs a) {
     extern __shared__ __attribute__((aligned(16))) short lds[];
     int ti_, tj_, z;
     if (!tile_of(a.map, blockIdx.x, ti_, tj_, z)) return;

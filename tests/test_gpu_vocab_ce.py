@@ -222,14 +222,14 @@ def test_gradients_written_into_given_buffers_with_strides():
     x, W, b, t = make(130, 520, 96, torch.float32, seed=8)
     nll, loss, saved = ops.vocab_ce_forward(x, W, b, t)
     one = torch.ones(1, device="cuda")
-    want = ops.vocab_ce_backward(x, W, b, t, saved, grad=one)
+    want = ops.vocab_ce_backward(saved, grad=one)
     bx, bw = torch.full((130, 100), 7.0, device="cuda"), torch.full((520, 101), 7.0, device="cuda")
-    got = ops.vocab_ce_backward(x, W, b, t, saved, grad=one, dx=bx[:, :96], dW=bw[:, :96])
+    got = ops.vocab_ce_backward(saved, grad=one, dx=bx[:, :96], dW=bw[:, :96])
     assert all(torch.equal(a, c) for a, c in zip(got, want))
     assert bool((bx[:, 96:] == 7).all()) and bool((bw[:, 96:] == 7).all())
-    only = ops.vocab_ce_backward(x, W, b, t, saved, grad=one, need=(False, False, True))
+    only = ops.vocab_ce_backward(saved, grad=one, need=(False, False, True))
     assert only[0] is None and only[1] is None and torch.equal(only[2], want[2])
-    only = ops.vocab_ce_backward(x, W, b, t, saved, grad=one, need=(False, True, False))
+    only = ops.vocab_ce_backward(saved, grad=one, need=(False, True, False))
     assert torch.equal(only[1], want[1])
 
 
@@ -289,7 +289,7 @@ def test_captured_and_replayed():
 
         def step(x=x, W=W, b=b, t=t):
             nll, loss, saved = ops.vocab_ce_forward(x, W, b, t)
-            return (loss,) + ops.vocab_ce_backward(x, W, b, t, saved, grad=one)
+            return (loss,) + ops.vocab_ce_backward(saved, grad=one)
         step()
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
