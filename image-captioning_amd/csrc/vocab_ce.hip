@@ -23,13 +23,25 @@ constexpr float L2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr int G_EXP = 14;                        // G is stored times 2^14
 constexpr size_t PIECE_BYTES = (size_t)512 << 20;
 
+// dx has as many row tiles as there are counted rows, which only the device knows: the number of parts for each possible
+// number of row tiles goes along (one part beyond 64 of them, 16384 rows, where there are tiles enough).
+struct Splits {
+    unsigned char s[64];
+};
+__host__ __device__ __forceinline__ int splits_of(const Splits& t, int tiles) {
+    return tiles < 1 || tiles > 64 ? 1 : t.s[tiles - 1];
+}
+
 // ---- memory plan (host and device agree through it) ------------------------------------------------------------------
 struct Plan {
     int M, V, K, Mp, Vp, Kp, split, elt;         // Mp: rows and Vp: words rounded up to 256, Kp: width to 32
     int xs;                                      // stored columns of the packed operands: Kp, or 2 Kp when split
     bool pack_w;
     int piece, pieces;                           // vocabulary words per piece (a multiple of 256)
-    int sx, sw;                                  // contraction splits of dx and dW
+    Splits sx;                                   // contraction splits of dx, by row tiles
+    int64_t dx_tiles;                            // most workgroups of a dx launch, and
+    int64_t dx_rows;                             // most rows of partial sums
+    int sw;                                      // contraction splits of dW
     bool wide_z, wide_dx, wide_dw;               // tiles of 256 x 256 for the logits, dx and dW
     size_t o_order, o_slot, o_tgt, o_lse, o_dlt, o_b2, o_x, o_w, saved;
     size_t o_part, o_amax, fwd;
@@ -43,12 +55,12 @@ size_t take(size_t& at, size_t bytes) {
 }
 
 // Contractions with few output tiles and a long sum are cut into s parts.  Workgroups run in rounds of `slots`; a part takes
-// 1 / s of the time, and each part costs about 6 k-tiles of time for its start, its partial sums and their addition.
+// 1 / s of the time.  Starting a tile costs about 6 k-tiles of time, writing partial sums and adding them later 16 more.
 int splits_for(int64_t tiles, int kt, int slots) {
     int best = 1;
     double least = 1e300;
     for (int s = 1; s <= 16 && kt / s >= 8; ++s) {
-        const double t = (double)((tiles * s + slots - 1) / slots) * ((kt + s - 1) / s + 6);
+        const double t = (double)((tiles * s + slots - 1) / slots) * ((kt + s - 1) / s + (s > 1 ? 22 : 6));
         if (t < least * 0.97) least = t, best = s;
     }
     return best;
@@ -102,12 +114,23 @@ bool make_plan(const capdec_vocab_ce* a, Plan& p) {
         split = wide ? s1 : s2;
         return wide;
     };
-    p.wide_dx = grad(row_tiles, p.piece / kt, p.sx);
+    int full;
+    p.wide_dx = grad(row_tiles, p.piece / kt, full);
     p.wide_dw = grad(word_tiles, p.Mp / kt, p.sw);
+    const int cols = p.wide_dx ? p.Kp / 256 : (p.Kp + 127) / 128;
+    p.dx_tiles = row_tiles * cols;
+    p.dx_rows = p.Mp;
+    for (int t = 1; t <= 64; ++t) {
+        p.sx.s[t - 1] = (unsigned char)splits_for((int64_t)t * cols, p.piece / kt, p.wide_dx ? 256 : 512);
+        if (t > row_tiles) continue;
+        const int64_t n = (int64_t)t * p.sx.s[t - 1];
+        if (n * cols > p.dx_tiles) p.dx_tiles = n * cols;
+        if (n * 256 > p.dx_rows) p.dx_rows = n * 256;
+    }
     at = 256;
     p.o_rw = take(at, (size_t)p.Mp * 4);
     p.o_g = take(at, (size_t)p.Mp * p.piece * es);
-    p.o_dx = take(at, (size_t)p.sx * p.Mp * p.Kp * 4);
+    p.o_dx = take(at, (size_t)p.dx_rows * p.Kp * 4);
     p.o_dw = p.sw > 1 ? take(at, (size_t)p.sw * p.piece * p.Kp * 4) : 0;
     p.o_db = a->bias ? take(at, (size_t)(p.Mp / 128) * p.piece * 4) : 0;
     p.bwd = at;
@@ -617,8 +640,9 @@ struct GradArgs {
     int rows_live;                 // dx: only the first count rows exist
     int k_live;                    // dW: the contraction runs over the counted rows; else over kt k-tiles
     int kt, nsplit;
+    Splits splits;                 // dx: instead of nsplit
     Map map;
-    float* part; int64_t ldp, plane; int add;
+    float* part; int64_t ldp, plane; int add;      // dx: plane is of the live row tiles
     void* out; int64_t ldo; int dtype;
 };
 __device__ __forceinline__ void store_as(void* p, int64_t i, float v, int dtype) {
@@ -630,11 +654,16 @@ template <class C, int ELT, bool TP, bool SPLIT, int OUT>
 __global__ __launch_bounds__(C::THREADS, C::EU) void grad_kernel(GradArgs a) {
     extern __shared__ __attribute__((aligned(16))) short lds[];
     int ti_, tj_, z;
-    if (!tile_of(a.map, blockIdx.x, ti_, tj_, z)) return;
     const int count = a.head->count;
+    if (a.rows_live) {
+        a.map.ni = (count + C::BI - 1) / C::BI;
+        a.map.nz = a.nsplit = splits_of(a.splits, a.map.ni);
+        a.map.per = (a.map.ni * a.map.nj * a.map.nz + 7) / 8;
+        a.plane = (int64_t)a.map.ni * C::BI * a.ldp;
+    }
+    if (!tile_of(a.map, blockIdx.x, ti_, tj_, z)) return;
     const int i0 = ti_ * C::BI, j0 = tj_ * C::BJ;
     const int nI = a.rows_live ? min(a.I, count) : a.I;
-    if (i0 >= nI) return;
     constexpr int KT = SPLIT ? 16 : 32;
     const int kt = a.k_live ? (count + KT - 1) / KT : a.kt;
     const int per = (kt + a.nsplit - 1) / a.nsplit;
@@ -667,10 +696,12 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void grad_kernel(GradArgs a) {
 }
 
 // dx[r] = factor * sum of the partial sums of r's slot; zero for rows that are not counted
-__global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part, int64_t plane, int nsplit, int Kp, int M,
+__global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part, Splits splits, int Kp, int M,
                                                  int K, const int* __restrict__ slot, const Head* __restrict__ head,
                                                  const BwdHead* __restrict__ bh, int split, void* out, int64_t ldo, int dtype) {
     const float f = bh->factor * (split ? pow2(-scale_exp(head->amax_w)) : 1.f);
+    const int tiles = (head->count + 255) / 256, nsplit = splits_of(splits, tiles);
+    const int64_t plane = (int64_t)tiles * 256 * Kp;
     const int cpr = (K + 3) / 4;
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < (int64_t)M * cpr; t += (int64_t)gridDim.x * 256) {
         const int r = (int)(t / cpr), c = (int)(t - (int64_t)r * cpr) * 4;
@@ -743,8 +774,9 @@ int launch_dlogits(LogitArgs a, int words, int rows, hipStream_t s) {
     return 0;
 }
 template <class C, int ELT, bool TP, bool SPLIT, int OUT>
-int launch_grad(GradArgs a, int I, int J, hipStream_t s) {
-    const unsigned grid = make_map(a.map, (I + C::BI - 1) / C::BI, (J + C::BJ - 1) / C::BJ, a.nsplit);
+int launch_grad(GradArgs a, int I, int J, int64_t most, hipStream_t s) {
+    unsigned grid = make_map(a.map, (I + C::BI - 1) / C::BI, (J + C::BJ - 1) / C::BJ, a.nsplit);
+    if (most) grid = (unsigned)((most + 7) / 8 * 8);          // dx: the kernel maps what is live
     CAPDEC_TRY(allow_lds(grad_kernel<C, ELT, TP, SPLIT, OUT>, C::LDS_BYTES));
     grad_kernel<C, ELT, TP, SPLIT, OUT><<<grid, C::THREADS, C::LDS_BYTES, s>>>(a);
     CAPDEC_LAUNCH_CHECK();
@@ -867,9 +899,9 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
             GradArgs d{};
             d.P = View{G, g.ldg, p.Mp, 0};
             d.Q = View{W + (int64_t)v0 * ldw, ldw, p.Kp, real};
-            d.head = head; d.bh = bh; d.I = p.Mp; d.J = p.Kp; d.rows_live = 1; d.kt = words / kt; d.nsplit = p.sx;
-            d.part = dxp; d.ldp = p.Kp; d.plane = (int64_t)p.Mp * p.Kp; d.add = v0 > 0;
-#define DX(E, S) (p.wide_dx ? launch_grad<Wide, E, false, S, 0>(d, p.Mp, p.Kp, s) : launch_grad<Big, E, false, S, 0>(d, p.Mp, p.Kp, s))
+            d.head = head; d.bh = bh; d.I = p.Mp; d.J = p.Kp; d.rows_live = 1; d.kt = words / kt; d.splits = p.sx;
+            d.part = dxp; d.ldp = p.Kp; d.add = v0 > 0;
+#define DX(E, S) (p.wide_dx ? launch_grad<Wide, E, false, S, 0>(d, p.Mp, p.Kp, p.dx_tiles, s) : launch_grad<Big, E, false, S, 0>(d, p.Mp, p.Kp, p.dx_tiles, s))
             CAPDEC_TRY(BY_TYPE(p, DX));
 #undef DX
         }
@@ -881,13 +913,13 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
             if (p.sw == 1) {
                 d.I = real; d.J = p.K;
                 d.out = (char*)dW + (int64_t)v0 * lddw * (p.split ? 4 : 2); d.ldo = lddw; d.dtype = a->dtype;
-#define DW(E, S) (p.wide_dw ? launch_grad<Wide, E, true, S, 1>(d, words, p.Kp, s) : launch_grad<Big, E, true, S, 1>(d, words, p.Kp, s))
+#define DW(E, S) (p.wide_dw ? launch_grad<Wide, E, true, S, 1>(d, words, p.Kp, 0, s) : launch_grad<Big, E, true, S, 1>(d, words, p.Kp, 0, s))
                 CAPDEC_TRY(BY_TYPE(p, DW));
 #undef DW
             } else {
                 d.I = real; d.J = p.Kp;
                 d.part = (float*)(ws + p.o_dw); d.ldp = p.Kp; d.plane = (int64_t)p.piece * p.Kp;
-#define DW(E, S) (p.wide_dw ? launch_grad<Wide, E, true, S, 0>(d, words, p.Kp, s) : launch_grad<Big, E, true, S, 0>(d, words, p.Kp, s))
+#define DW(E, S) (p.wide_dw ? launch_grad<Wide, E, true, S, 0>(d, words, p.Kp, 0, s) : launch_grad<Big, E, true, S, 0>(d, words, p.Kp, 0, s))
                 CAPDEC_TRY(BY_TYPE(p, DW));
 #undef DW
             }
@@ -903,7 +935,7 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
     }
     if (dx) {
         dx_kernel<<<blocks_for((int64_t)p.M * ((p.K + 3) / 4), 256, 8192), 256, 0, s>>>(
-            dxp, (int64_t)p.Mp * p.Kp, p.sx, p.Kp, p.M, p.K, slot, head, bh, p.split, dx, lddx, a->dtype);
+            dxp, p.sx, p.Kp, p.M, p.K, slot, head, bh, p.split, dx, lddx, a->dtype);
         CAPDEC_LAUNCH_CHECK();
     }
     return 0;
