@@ -31,11 +31,40 @@ struct Batch {
     Item it[MAX_BATCH];
 };
 
+// A and A^2 are symmetric: from 768 on, the upper triangle of 256 x 256 or 128 x 128 tiles, its contraction in parts where
+// that fills the CUs better.  Times in us from measurements of split operands (a k-tile takes a CU 1.36 with one 256 x 256
+// tile; 0.45, 0.80, 1.15 with one to three 128 x 128 tiles); the parts' sums go to memory and back at 4 TB/s.
+struct Symmetric {
+    bool on, wide;
+    int nsplit;
+    size_t slab;                   // bytes of partial sums for a batch
+};
+Symmetric symmetric_plan(int m, int kt, int nz) {
+    Symmetric best{false, false, 1, 0};
+    if (m < 768) return best;
+    auto mids = [](int64_t n) {
+        const int64_t per = (n + 255) / 256, left = per % 3;
+        return (double)(per / 3) * 1.15 + (left == 2 ? 0.80 : left == 1 ? 0.45 : 0.0);
+    };
+    const int64_t w = (m + 255) / 256, h = (m + 127) / 128;
+    // the whole square, by the rule of launch_sized
+    double least = 0.9 * (w * w * nz >= 256 ? (double)((w * w * nz + 255) / 256) * 1.36 : mids(h * h * nz)) * kt;
+    for (int wide = 0; wide < 2; ++wide)
+        for (int s = 1; s <= 8 && kt / s >= 8; ++s) {
+            const int64_t n = (wide ? w * (w + 1) / 2 : h * (h + 1) / 2) * nz * s;
+            const size_t slab = s > 1 ? (size_t)n * (wide ? 256 * 256 : 128 * 128) * 4 : 0;
+            if (slab > (size_t)512 << 20) break;
+            const double t = (wide ? (double)((n + 255) / 256) * 1.36 : mids(n)) * ((kt + s - 1) / s) + (s > 1 ? 5 + 2e-6 * slab / 4 : 0);
+            if (t < least) least = t, best = Symmetric{true, wide != 0, s, slab};
+        }
+    return best;
+}
+
 struct Dims {
     int rows, cols, rp, cp, m;            // rp, cp: rounded up to 32; m: the shorter of the two
     bool tall;
     size_t x_elems, a_elems;              // 16-bit elements of one matrix
-    size_t per, norm;                     // workspace bytes per matrix, and of the partial sums of a batch
+    size_t per, norm, slab;               // workspace bytes: per matrix, of a batch's sums of squares, of partial products
     int batch;
 };
 
@@ -54,6 +83,14 @@ bool make_dims(int count, int rows, int cols, Dims& d) {
     d.batch = b < 1 ? 1 : b > MAX_BATCH ? MAX_BATCH : (int)b;
     if (d.batch > count) d.batch = count;
     d.norm = (size_t)d.batch * NORM_BLOCKS * 8;
+    d.slab = 0;                           // the most that a product of this batch, or of the rest of the matrices, may take
+    const int n = d.tall ? d.rp : d.cp, rest = count % d.batch ? count % d.batch : d.batch;
+    for (int kdiv = 16; kdiv <= 32; kdiv += 16)
+        for (int nz : {d.batch, rest})
+            for (int k : {n, d.m}) {
+                const size_t b = symmetric_plan(d.m, k / kdiv, nz).slab;
+                if (b > d.slab) d.slab = b;
+            }
     return true;
 }
 
@@ -195,6 +232,8 @@ struct StepArgs {
     int64_t ldr;
     float alpha, beta;
     int I, J, kt;
+    int tri;                       // symmetric result: only the tiles on and above the diagonal, mirrored as they are stored
+    int nsplit; float* slab;       // contraction in parts: partial sums [matrix][part][tile][accumulator][thread]
     Map map;
     short* out; int64_t ldo; int out_split;       // inner products
     // last product of the last step
@@ -204,86 +243,143 @@ struct StepArgs {
 };
 enum { INNER = 0, RESULT = 1, UPDATE = 2 };
 
-template <class C, bool TP, bool TQ, bool SPLIT, int OUT>
+// WHOLE: contraction and epilogue.  PART: the contraction of one of nsplit parts, its sums to the slab.  JOIN: the parts'
+// sums added in order, then the epilogue; a workgroup per accumulator of a tile (blockIdx.y).
+enum { WHOLE = 0, PART = 1, JOIN = 2 };
+
+template <class C, bool TP, bool TQ, bool SPLIT, int OUT, int PHASE>
 __global__ __launch_bounds__(C::THREADS, C::EU) void step_kernel(StepArgs a) {
     extern __shared__ __attribute__((aligned(16))) short lds[];
     int ti_, tj_, z;
     if (!tile_of(a.map, blockIdx.x, ti_, tj_, z)) return;
+    const int tiles = a.map.ni * a.map.nj, tile = ti_ * a.map.nj + tj_;
+    if (a.tri) {                   // the map runs over the triangle's tiles along one axis: column tj_ of it holds tj_ + 1
+        tj_ = (int)((sqrtf(8.f * ti_ + 1.f) - 1.f) * 0.5f);
+        while ((tj_ + 1) * (tj_ + 2) / 2 <= ti_) ++tj_;
+        while (tj_ * (tj_ + 1) / 2 > ti_) --tj_;
+        ti_ -= tj_ * (tj_ + 1) / 2;
+    }
     const int i0 = ti_ * C::BI, j0 = tj_ * C::BJ;
-    View P = a.P, Q = a.Q;
-    P.p += z * a.strideP;
-    Q.p += z * a.strideQ;
+    const int mat = PHASE == PART ? z / a.nsplit : z;
+    constexpr int ACCS = C::TI * C::TJ;
     f32x16 acc[C::TI][C::TJ];
-    contract<C, F16, TP, TQ, SPLIT>(P, Q, i0, j0, 0, a.kt, lds, acc);
-    if (threadIdx.x >= C::GROUP) return;
+    if (PHASE != JOIN) {
+        View P = a.P, Q = a.Q;
+        P.p += mat * a.strideP;
+        Q.p += mat * a.strideQ;
+        const int part = z - mat * (PHASE == PART ? a.nsplit : 1), per = PHASE == PART ? (a.kt + a.nsplit - 1) / a.nsplit : a.kt;
+        contract<C, F16, TP, TQ, SPLIT>(P, Q, i0, j0, part * per, min(a.kt, (part + 1) * per), lds, acc);
+        if (threadIdx.x >= C::GROUP) return;
+    }
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));
+    if (PHASE == PART) {
+        float* d = a.slab + ((int64_t)z * tiles + tile) * (ACCS * 16 * C::GROUP) + tid;
+#pragma unroll
+        for (int e = 0; e < ACCS * 16; ++e) d[e * C::GROUP] = acc[e / 16 / C::TJ][e / 16 % C::TJ][e % 16];
+        return;
+    }
     const int lane = tid & 63, wave = tid >> 6, wi = wave / C::WJ, wj = wave % C::WJ, h = lane >> 5;
-    const short* R = a.R ? a.R + z * a.strideR : nullptr;
+    const short* R = a.R ? a.R + mat * a.strideR : nullptr;
     float lr = a.lr;
     if (OUT == UPDATE && a.st) lr = a.st->lr;
-#pragma unroll
-    for (int tj = 0; tj < C::TJ; ++tj) {
-        const int j = j0 + (wj * C::TJ + tj) * 32 + (lane & 31);
-        if (j >= a.J) continue;
+    auto finish = [&](int ti, int tj, const f32x16& sum) {
+        const int j = j0 + (wj * C::TJ + tj) * 32 + (lane & 31), ib = i0 + (wi * C::TI + ti) * 32;
+        if (j >= a.J) return;
         const int64_t js = SPLIT ? split_col(j) : j;
         const int64_t jo = a.out_split ? split_col(j) : j;
+        float v[16];
 #pragma unroll
-        for (int ti = 0; ti < C::TI; ++ti) {
-            float v[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = a.alpha * acc[ti][tj][e];
-            if (R) {                       // every load first, without branches: one round trip
-                short hi[16], lo[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const short* q = R + (int64_t)min(i0 + (wi * C::TI + ti) * 32 + acc_row(e, h), a.I - 1) * a.ldr + js;
-                    hi[e] = q[0];
-                    lo[e] = SPLIT ? q[16] : (short)0;
-                }
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    v[e] = fmaf(a.beta, from_bits<F16>(hi[e]) + (SPLIT ? from_bits<F16>(lo[e]) : 0.f), v[e]);
-            }
-            float old[16];
-            if (OUT == UPDATE) {
-                const Item& it = a.b.it[z];
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    old[e] = ((const float*)it.dst)[(int64_t)min(i0 + (wi * C::TI + ti) * 32 + acc_row(e, h), a.I - 1) * it.ldd + j];
-            }
+        for (int e = 0; e < 16; ++e) v[e] = a.alpha * sum[e];
+        if (R) {                       // every load first, without branches: one round trip
+            short hi[16], lo[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const int i = i0 + (wi * C::TI + ti) * 32 + acc_row(e, h);
+                const short* q = R + (int64_t)min(ib + acc_row(e, h), a.I - 1) * a.ldr + js;
+                hi[e] = q[0];
+                lo[e] = SPLIT ? q[16] : (short)0;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                v[e] = fmaf(a.beta, from_bits<F16>(hi[e]) + (SPLIT ? from_bits<F16>(lo[e]) : 0.f), v[e]);
+        }
+        if (OUT == INNER) {
+            short* out = a.out + mat * a.strideO;
+            s16x4 hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                short p, r;
+                split16(v[e], p, r);
+                hi[e / 4][e % 4] = p;
+                lo[e / 4][e % 4] = r;
+                const int i = ib + acc_row(e, h);
                 if (i >= a.I) continue;
-                if (OUT == INNER) {
-                    short* d = a.out + z * a.strideO + (int64_t)i * a.ldo + jo;
-                    short p, r;
-                    split16(v[e], p, r);
-                    d[0] = p;
-                    if (a.out_split) d[16] = r;
-                } else {
-                    const Item& it = a.b.it[z];
-                    const int64_t at = (int64_t)i * it.ldd + j;
-                    if (OUT == RESULT) {
-                        store_as(it.dst, at, v[e], a.dtype);
-                    } else {
-                        ((float*)it.dst)[at] = fmaf(-lr * a.scale, v[e], old[e] * (1.f - lr * a.decay));
-                    }
+                short* d = out + (int64_t)i * a.ldo + jo;
+                d[0] = p;
+                if (a.out_split) d[16] = r;
+            }
+            if (a.tri && ti_ != tj_) {
+                // row j of the mirrored tile: four neighbours at a time (I is a multiple of 32)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int i = ib + 8 * q + 4 * h;
+                    if (i >= a.I) continue;
+                    short* d = out + (int64_t)j * a.ldo + (a.out_split ? split_col(i) : i);
+                    *reinterpret_cast<s16x4*>(d) = hi[q];
+                    if (a.out_split) *reinterpret_cast<s16x4*>(d + 16) = lo[q];
                 }
             }
+            return;
         }
+        const Item& it = a.b.it[mat];
+        float old[16];
+        if (OUT == UPDATE) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                old[e] = ((const float*)it.dst)[(int64_t)min(ib + acc_row(e, h), a.I - 1) * it.ldd + j];
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int i = ib + acc_row(e, h);
+            if (i >= a.I) continue;
+            const int64_t at = (int64_t)i * it.ldd + j;
+            if (OUT == RESULT) store_as(it.dst, at, v[e], a.dtype);
+            else ((float*)it.dst)[at] = fmaf(-lr * a.scale, v[e], old[e] * (1.f - lr * a.decay));
+        }
+    };
+    if (PHASE == JOIN) {
+        const int ac = blockIdx.y;
+        f32x16 sum;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum[e] = 0.f;
+        for (int k = 0; k < a.nsplit; ++k) {
+            const float* d = a.slab + ((((int64_t)mat * a.nsplit + k) * tiles + tile) * ACCS + ac) * (16 * C::GROUP) + tid;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sum[e] += d[e * C::GROUP];
+        }
+        finish(ac / C::TJ, ac % C::TJ, sum);
+    } else {
+#pragma unroll
+        for (int tj = 0; tj < C::TJ; ++tj)
+#pragma unroll
+            for (int ti = 0; ti < C::TI; ++ti) finish(ti, tj, acc[ti][tj]);
     }
 }
 
-template <class C, bool TP, bool TQ, bool SPLIT, int OUT>
+template <class C, bool TP, bool TQ, bool SPLIT, int OUT, int PHASE>
 int launch(const StepArgs& a0, int nz, hipStream_t s) {
     StepArgs a = a0;
-    const unsigned grid = make_map(a.map, (a.I + C::BI - 1) / C::BI, (a.J + C::BJ - 1) / C::BJ, nz);
-    if (C::LDS_BYTES > 64 * 1024)
-        CAPDEC_TRY((int)hipFuncSetAttribute(reinterpret_cast<const void*>(step_kernel<C, TP, TQ, SPLIT, OUT>),
-                                            hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS_BYTES));
-    step_kernel<C, TP, TQ, SPLIT, OUT><<<grid, C::THREADS, C::LDS_BYTES, s>>>(a);
+    int ni = (a.I + C::BI - 1) / C::BI, nj = (a.J + C::BJ - 1) / C::BJ;
+    if (a.tri) {
+        ni = ni * (ni + 1) / 2;
+        nj = 1;
+    }
+    const unsigned grid = make_map(a.map, ni, nj, PHASE == PART ? nz * a.nsplit : nz);
+    constexpr int bytes = PHASE == JOIN ? 0 : C::LDS_BYTES;
+    if (bytes > 64 * 1024)
+        CAPDEC_TRY((int)hipFuncSetAttribute(reinterpret_cast<const void*>(step_kernel<C, TP, TQ, SPLIT, OUT, PHASE>),
+                                            hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    step_kernel<C, TP, TQ, SPLIT, OUT, PHASE><<<dim3(grid, PHASE == JOIN ? C::TI * C::TJ : 1), PHASE == JOIN ? C::GROUP : C::THREADS, bytes, s>>>(a);
     CAPDEC_LAUNCH_CHECK();
     return 0;
 }
@@ -292,15 +388,33 @@ int launch(const StepArgs& a0, int nz, hipStream_t s) {
 template <bool TP, bool TQ, bool SPLIT, int OUT>
 int launch_sized(const StepArgs& a, int nz, hipStream_t s) {
     auto tiles = [&](int bi, int bj) { return (int64_t)((a.I + bi - 1) / bi) * ((a.J + bj - 1) / bj) * nz; };
-    if (tiles(256, 256) >= 256) return launch<Wide, TP, TQ, SPLIT, OUT>(a, nz, s);
-    if (tiles(256, 128) >= 256) return launch<Big, TP, TQ, SPLIT, OUT>(a, nz, s);
-    if (tiles(128, 128) >= 256) return launch<Mid, TP, TQ, SPLIT, OUT>(a, nz, s);
-    if (tiles(64, 64) >= 512) return launch<Small, TP, TQ, SPLIT, OUT>(a, nz, s);
-    return launch<Deep, TP, TQ, SPLIT, OUT>(a, nz, s);
+    if (tiles(256, 256) >= 256) return launch<Wide, TP, TQ, SPLIT, OUT, WHOLE>(a, nz, s);
+    if (tiles(256, 128) >= 256) return launch<Big, TP, TQ, SPLIT, OUT, WHOLE>(a, nz, s);
+    if (tiles(128, 128) >= 256) return launch<Mid, TP, TQ, SPLIT, OUT, WHOLE>(a, nz, s);
+    if (tiles(64, 64) >= 512) return launch<Small, TP, TQ, SPLIT, OUT, WHOLE>(a, nz, s);
+    return launch<Deep, TP, TQ, SPLIT, OUT, WHOLE>(a, nz, s);
 }
 template <bool TP, bool TQ, int OUT>
 int launch_split(const StepArgs& a, bool split, int nz, hipStream_t s) {
     return split ? launch_sized<TP, TQ, true, OUT>(a, nz, s) : launch_sized<TP, TQ, false, OUT>(a, nz, s);
+}
+
+// A symmetric product of a batch, into planes of the operands' layout.
+template <bool T>
+int launch_symmetric(StepArgs a, bool split, int nz, float* slab, hipStream_t s) {
+    const Symmetric p = symmetric_plan(a.I, a.kt, nz);
+    a.tri = p.on; a.nsplit = p.nsplit; a.slab = slab;
+#define SYM(S)                                                                                   \
+    if (!p.on) return launch_sized<T, T, S, INNER>(a, nz, s);                                    \
+    if (p.nsplit == 1)                                                                           \
+        return p.wide ? launch<Wide, T, T, S, INNER, WHOLE>(a, nz, s) : launch<Mid, T, T, S, INNER, WHOLE>(a, nz, s); \
+    CAPDEC_TRY((p.wide ? launch<Wide, T, T, S, INNER, PART>(a, nz, s) : launch<Mid, T, T, S, INNER, PART>(a, nz, s))); \
+    return p.wide ? launch<Wide, T, T, S, INNER, JOIN>(a, nz, s) : launch<Mid, T, T, S, INNER, JOIN>(a, nz, s);
+    if (split) {
+        SYM(true)
+    }
+    SYM(false)
+#undef SYM
 }
 
 // Largest |p(x)| on [0, top] of a x + b x^3 + c x^5 (odd) or b x + c x^2: ends and stationary points.
@@ -350,6 +464,7 @@ int run_batch(const Batch& b, int nz, const Dims& d, const Iteration& n, int dty
     X[1] = X[0] + (size_t)d.batch * d.x_elems;
     short* A = X[1] + (size_t)d.batch * d.x_elems;
     short* B = A + (size_t)d.batch * d.a_elems;
+    float* slab = (float*)(B + (size_t)d.batch * d.a_elems);
     double sigma = 1.0;                           // bound of the iterate's singular values
     int sx = exponent_for(sigma);
     bool split = n.exact_steps > 0;
@@ -378,8 +493,8 @@ int run_batch(const Batch& b, int nz, const Dims& d, const Iteration& n, int dty
         g.alpha = ldexpf(1.f, sa - 2 * sx);
         g.I = g.J = d.m; g.kt = (d.tall ? d.rp : d.cp) / kdiv;
         g.out = A; g.ldo = lda; g.out_split = split; g.strideO = (int64_t)d.a_elems;
-        if (d.tall) CAPDEC_TRY((launch_split<true, true, INNER>(g, split, nz, s)));
-        else CAPDEC_TRY((launch_split<false, false, INNER>(g, split, nz, s)));
+        if (d.tall) CAPDEC_TRY(launch_symmetric<true>(g, split, nz, slab, s));
+        else CAPDEC_TRY(launch_symmetric<false>(g, split, nz, slab, s));
 
         g.strideP = g.strideQ = g.strideR = (int64_t)d.a_elems;
         g.P = g.Q = View{A, lda, d.m, d.m};
@@ -388,7 +503,7 @@ int run_batch(const Batch& b, int nz, const Dims& d, const Iteration& n, int dty
         g.beta = (float)ldexp((double)n.b, sb - sa);
         g.kt = d.m / kdiv;
         g.out = B;
-        CAPDEC_TRY((launch_split<false, false, INNER>(g, split, nz, s)));
+        CAPDEC_TRY(launch_symmetric<false>(g, split, nz, slab, s));
 
         const bool end = k + 1 == n.steps;
         const double next = top_of_step(n.a, n.b, n.c, sigma);
@@ -449,7 +564,7 @@ extern "C" {
 size_t capdec_orthogonalize_workspace_bytes(int count, int rows, int cols) {
     Dims d;
     if (!make_dims(count, rows, cols, d)) return 0;
-    return ((d.norm + 255) & ~(size_t)255) + d.per * d.batch;
+    return ((d.norm + 255) & ~(size_t)255) + d.per * d.batch + d.slab;
 }
 
 int capdec_orthogonalize(const capdec_matrix* mats, int count, int rows, int cols, int dtype, int steps, const float* coeffs,
