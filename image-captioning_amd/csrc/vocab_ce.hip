@@ -45,7 +45,7 @@ struct Plan {
     bool wide_z, wide_dx, wide_dw;               // tiles of 256 x 256 for the logits, dx and dW
     size_t o_order, o_slot, o_tgt, o_lse, o_dlt, o_b2, o_x, o_w, saved;
     size_t o_part, o_amax, fwd;
-    size_t o_rw, o_g, o_dx, o_dw, o_db, bwd;
+    size_t o_rw, o_rest, o_g, o_dx, o_dw, o_db, bwd;
 };
 
 size_t take(size_t& at, size_t bytes) {
@@ -129,6 +129,7 @@ bool make_plan(const capdec_vocab_ce* a, Plan& p) {
     }
     at = 256;
     p.o_rw = take(at, (size_t)p.Mp * 4);
+    p.o_rest = take(at, (size_t)p.Mp * 4);
     p.o_g = take(at, (size_t)p.Mp * p.piece * es);
     p.o_dx = take(at, (size_t)p.dx_rows * p.Kp * 4);
     p.o_dw = p.sw > 1 ? take(at, (size_t)p.sw * p.piece * p.Kp * 4) : 0;
@@ -362,6 +363,7 @@ struct LogitArgs {
     const int* tgt;
     short* g; int64_t ldg;                       // [slot][word of the piece]
     float* dbp;                                  // [row tile][word of the piece], nullable
+    float* rest;                                 // [slot] what rounding took off the target's entry (16-bit operands)
     int v0, piece;
 };
 
@@ -534,7 +536,8 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void dlogits_kernel(LogitArgs a)
     const float c1 = logit_scale<SPLIT>(a.head);
     constexpr int WORDS = 32 * C::TI;                     // of a wavefront
     constexpr int PL = SPLIT ? 2 : 1;
-    constexpr int LD = WORDS * PL + 8;                    // 16-bit elements per row of the turned tile
+    constexpr int LOW = SPLIT ? 16 : WORDS;               // from a value to its low part
+    constexpr int LD = WORDS * 2 + 8;                     // 16-bit elements per row of the turned tile: G, and its low parts
     // one 32-row block of the wavefront at a time
     short* tile = lds + wave * 32 * LD;
     float* colsum = reinterpret_cast<float*>(lds + C::WAVES * 32 * LD);      // [WJ][BI]
@@ -563,20 +566,25 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void dlogits_kernel(LogitArgs a)
                         hi[e] = p;
                         lo[e] = r;
                     } else {
+                        asm("" : "+v"(v));
                         hi[e] = to_bits<ELT>(v);
+                        lo[e] = to_bits<ELT>(v - from_bits<ELT>(hi[e]));
                     }
                 }
                 short* d = tile + (lane & 31) * LD + (SPLIT ? (int)split_col(wd) : wd);
                 *reinterpret_cast<s16x4*>(d) = hi;
-                if (SPLIT) *reinterpret_cast<s16x4*>(d + 16) = lo;
+                if (SPLIT || a.dbp) *reinterpret_cast<s16x4*>(d + LOW) = lo;
             }
             __builtin_amdgcn_sched_barrier(0);
         }
         // (the tile belongs to this wavefront alone: LDS operations of a wavefront complete in order)
+        // What rounding takes off a target's entry, usually its row's largest by far, is kept: dx gets it back, and dW of
+        // a batch too small for such errors to average out.
         if (h == 0 && live) {
             const int t = a.tgt[s] - (i0 + wi * WORDS);
             if (t >= 0 && t < WORDS) {
-                const float v = expm1f(a.dlt[s]) * w;
+                float v = expm1f(a.dlt[s]) * w;
+                asm("" : "+v"(v));
                 short* d = tile + lane * LD + (SPLIT ? (int)split_col(t) : t);
                 if (SPLIT) {
                     short p, r;
@@ -584,7 +592,11 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void dlogits_kernel(LogitArgs a)
                     d[0] = p;
                     d[16] = r;
                 } else {
-                    d[0] = to_bits<ELT>(v);
+                    const short q = to_bits<ELT>(v);
+                    const float rest = v - from_bits<ELT>(q);
+                    d[0] = q;
+                    d[LOW] = to_bits<ELT>(rest);
+                    a.rest[s] = rest;
                 }
             }
         }
@@ -608,8 +620,7 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void dlogits_kernel(LogitArgs a)
                 float sum = 0.f;
 #pragma unroll 8
                 for (int r = 0; r < 32; ++r) {
-                    sum += from_bits<ELT>(d[r * LD]);
-                    if (SPLIT) sum += from_bits<ELT>(d[r * LD + 16]);
+                    sum += from_bits<ELT>(d[r * LD]) + from_bits<ELT>(d[r * LD + LOW]);
                 }
                 sums[k] += sum;
             }
@@ -632,6 +643,7 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void dlogits_kernel(LogitArgs a)
 
 // dx and dW of one piece.  OUT 0: fp32 partial sums [split][i][j], added onto what earlier pieces left when `add`;
 // OUT 1: times the factor, in the weights' type.
+constexpr int REST_ROWS = 64;
 struct GradArgs {
     View P, Q;
     const Head* head;
@@ -642,6 +654,7 @@ struct GradArgs {
     int kt, nsplit;
     Splits splits;                 // dx: instead of nsplit
     Map map;
+    const int* tgt; const float* rest; int v0;     // dW of at most REST_ROWS rows
     float* part; int64_t ldp, plane; int add;      // dx: plane is of the live row tiles
     void* out; int64_t ldo; int dtype;
 };
@@ -670,6 +683,24 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void grad_kernel(GradArgs a) {
     f32x16 acc[C::TI][C::TJ];
     contract<C, ELT, TP, true, SPLIT>(a.P, a.Q, i0, j0, z * per, min(kt, (z + 1) * per), lds, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave / C::WJ, wj = wave % C::WJ, h = lane >> 5;
+    if (TP && !SPLIT && z == 0 && count <= REST_ROWS) {
+        // row m adds rest[m] x[m] to its target's row of dW
+        for (int m = 0; m < count; ++m) {
+            const int at = a.tgt[m] - a.v0 - i0;
+            if (a.tgt[m] < a.v0 || at < 0 || at >= C::BI) continue;
+            const float q = a.rest[m];
+#pragma unroll
+            for (int tj = 0; tj < C::TJ; ++tj) {
+                const int j = min(j0 + (wj * C::TJ + tj) * 32 + (lane & 31), a.Q.n - 1);
+                const float x = q * from_bits<ELT>(a.Q.p[(int64_t)m * a.Q.ld + j]);
+#pragma unroll
+                for (int ti = 0; ti < C::TI; ++ti)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if ((wi * C::TI + ti) * 32 + acc_row(e, h) == at) acc[ti][tj][e] += x;
+            }
+        }
+    }
     float f = 1.f;
     if (OUT == 1) {
         f = a.bh->factor;
@@ -695,10 +726,13 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void grad_kernel(GradArgs a) {
     }
 }
 
-// dx[r] = factor * sum of the partial sums of r's slot; zero for rows that are not counted
-__global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part, Splits splits, int Kp, int M,
-                                                 int K, const int* __restrict__ slot, const Head* __restrict__ head,
-                                                 const BwdHead* __restrict__ bh, int split, void* out, int64_t ldo, int dtype) {
+// dx[r] = factor * (sum of the partial sums of r's slot + what rounding took off its target's entry of G times the target's
+// row of W); zero for rows that are not counted
+__global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part, Splits splits, int Kp, int M, int K,
+                                                 const int* __restrict__ slot, const int* __restrict__ tgt,
+                                                 const float* __restrict__ rest, const void* W, int64_t ldw,
+                                                 const Head* __restrict__ head, const BwdHead* __restrict__ bh, int split,
+                                                 void* out, int64_t ldo, int dtype) {
     const float f = bh->factor * (split ? pow2(-scale_exp(head->amax_w)) : 1.f);
     const int tiles = (head->count + 255) / 256, nsplit = splits_of(splits, tiles);
     const int64_t plane = (int64_t)tiles * 256 * Kp;
@@ -709,6 +743,13 @@ __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part,
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
         if (s >= 0) {
             for (int k = 0; k < nsplit; ++k) v += *reinterpret_cast<const f32x4*>(part + k * plane + (int64_t)s * Kp + c);
+            const int w = tgt[s];
+            if (!split && w >= 0) {
+                const float q = rest[s];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < K) v[e] = fmaf(q, load_as_f32(W, (int64_t)w * ldw + c + e, dtype), v[e]);
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] *= f;
         }
@@ -765,7 +806,7 @@ int launch_lse(LogitArgs a, int words, int rows, hipStream_t s) {
 }
 template <class C, int ELT, bool SPLIT>
 int launch_dlogits(LogitArgs a, int words, int rows, hipStream_t s) {
-    constexpr int turned = C::WAVES * 32 * (32 * C::TI * (SPLIT ? 2 : 1) + 8) * 2 + C::WJ * C::BI * 4;
+    constexpr int turned = C::WAVES * 32 * (32 * C::TI * 2 + 8) * 2 + C::WJ * C::BI * 4;
     constexpr int bytes = turned > C::LDS_BYTES ? turned : C::LDS_BYTES;
     const unsigned grid = make_map(a.map, words / C::BI, rows / C::BJ, 1);
     CAPDEC_TRY(allow_lds(dlogits_kernel<C, ELT, SPLIT>, bytes));
@@ -875,6 +916,7 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
     const int* slot = (const int*)(sv + p.o_slot);
     BwdHead* bh = (BwdHead*)ws;
     float* rw = (float*)(ws + p.o_rw);
+    float* rest = (float*)(ws + p.o_rest);
     weights_kernel<<<1, 1024, 0, s>>>(row_grad, grad, mean, head, order, p.Mp, rw, bh);
     CAPDEC_LAUNCH_CHECK();
     const short* px = (const short*)(sv + p.o_x);
@@ -891,7 +933,7 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
         g.X = View{px, (int64_t)p.xs, p.Mp, 0};
         g.b2 = (const float*)(sv + p.o_b2); g.head = head; g.kt = p.xs / 32; g.Mp = p.Mp;
         g.lse = (const float*)(sv + p.o_lse); g.dlt = (const float*)(sv + p.o_dlt); g.rw = rw; g.tgt = (const int*)(sv + p.o_tgt);
-        g.g = G; g.ldg = (int64_t)p.piece * pl; g.dbp = dbias ? (float*)(ws + p.o_db) : nullptr; g.v0 = v0; g.piece = p.piece;
+        g.g = G; g.ldg = (int64_t)p.piece * pl; g.rest = rest; g.dbp = dbias ? (float*)(ws + p.o_db) : nullptr; g.v0 = v0; g.piece = p.piece;
 #define DL(E, S) (p.wide_z ? launch_dlogits<Wide, E, S>(g, words, p.Mp, s) : launch_dlogits<Big, E, S>(g, words, p.Mp, s))
         CAPDEC_TRY(BY_TYPE(p, DL));
 #undef DL
@@ -910,6 +952,7 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
             d.P = View{G, g.ldg, words, p.Mp};
             d.Q = View{px, (int64_t)p.xs, p.Kp, p.Mp};
             d.head = head; d.bh = bh; d.k_live = 1; d.nsplit = p.sw;
+            d.tgt = g.tgt; d.rest = rest; d.v0 = v0;
             if (p.sw == 1) {
                 d.I = real; d.J = p.K;
                 d.out = (char*)dW + (int64_t)v0 * lddw * (p.split ? 4 : 2); d.ldo = lddw; d.dtype = a->dtype;
@@ -935,7 +978,7 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
     }
     if (dx) {
         dx_kernel<<<blocks_for((int64_t)p.M * ((p.K + 3) / 4), 256, 8192), 256, 0, s>>>(
-            dxp, p.sx, p.Kp, p.M, p.K, slot, head, bh, p.split, dx, lddx, a->dtype);
+            dxp, p.sx, p.Kp, p.M, p.K, slot, (const int*)(sv + p.o_tgt), rest, a->W, a->ldw, head, bh, p.split, dx, lddx, a->dtype);
         CAPDEC_LAUNCH_CHECK();
     }
     return 0;
