@@ -542,17 +542,6 @@ def vocab_logits_bwd(dec, x, dlogits, grads):
     return _lin_bwd(grads, "fc2", dec.fc2, dlogits, x)
 
 
-_ONES = {}
-
-
-def _one(device):
-    """The constant 1.0 of a device: the upstream gradient of a loss that is differentiated itself."""
-    t = _ONES.get(device)
-    if t is None:
-        t = _ONES[device] = torch.ones(1, device=device)
-    return t
-
-
 def vocab_loss(dec, x, targets, ignore_index=0, materialize=True, skip_ignored=True, rows=None, pieces=False):
     """Projection + CrossEntropyLoss(ignore_index) (reference train.py:216,254-256).
     Returns (loss [1] device tensor, saved state for ``vocab_loss_bwd``).
@@ -607,7 +596,7 @@ def vocab_loss_bwd(dec, x, saved, grads):
     the others add to them)."""
     if saved[0] == "pieces":
         W, b = dec.fc2.weight, dec.fc2.bias
-        return ops.vocab_ce_backward(saved[1], grad=_one(x.device), dW=_new(grads, "fc2.weight", W),
+        return ops.vocab_ce_backward(saved[1], dW=_new(grads, "fc2.weight", W),
                                      db=None if b is None else _new(grads, "fc2.bias", b))[0]
     if saved[0] == "rows":
         _, dlogits, rows = saved

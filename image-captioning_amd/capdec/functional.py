@@ -78,7 +78,7 @@ def vocab_cross_entropy(x, weight, bias, targets, ignore_index=0, reduction="mea
     if x.dim() < 1 or x.shape[:-1] != targets.shape:
         raise RuntimeError(f"capdec: x {tuple(x.shape)} and targets {tuple(targets.shape)} do not fit")
     x2, t = x.reshape(-1, x.shape[-1]), targets.reshape(-1)
-    if x2.stride(1) != 1 and x2.shape[1] > 1:
-        x2 = x2.contiguous()
+    if (x2.stride(1) != 1 and x2.shape[1] > 1) or (x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]):
+        x2 = x2.contiguous()                       # columns apart, or rows that share memory (a broadcast x)
     loss = AG.vocab_cross_entropy(x2, weight, bias, t.contiguous(), ignore_index, reduction)
     return loss.view(targets.shape) if reduction == "none" else loss

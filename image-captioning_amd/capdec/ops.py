@@ -1038,13 +1038,14 @@ def vocab_ce_forward(x, W, b, targets, ignore_index=0, want_loss=True):
 
 def vocab_ce_backward(state, grad=None, row_grad=None, mean=True, dx=None, dW=None, db=None, need=(True, True, True)):
     """Gradients of ``vocab_ce_forward``.  The upstream gradient is ``row_grad`` [M] fp32 (of nll) or ``grad``, a one-element
-    fp32 tensor (of the mean, or with ``mean=False`` of the sum).  Returns (dx, dW, db) in the operands' type, written into
+    fp32 tensor (of the mean, or with ``mean=False`` of the sum; None: 1).  Returns (dx, dW, db) in the operands' type, written into
     the tensors given for them, or None where ``need`` says so."""
     lib = _lib.load()
-    if (grad is None) == (row_grad is None):
-        raise RuntimeError("capdec vocab_ce_backward: exactly one of grad and row_grad")
-    g = _chk(grad if grad is not None else row_grad, name="upstream gradient")
-    if g.numel() != (1 if grad is not None else state.args.M) or not g.is_contiguous():
+    if grad is not None and row_grad is not None:
+        raise RuntimeError("capdec vocab_ce_backward: at most one of grad and row_grad")
+    g = grad if grad is not None else row_grad
+    if g is not None and (_chk(g, name="upstream gradient").numel() != (1 if grad is not None else state.args.M) or
+                          not g.is_contiguous()):
         raise RuntimeError(f"capdec vocab_ce_backward: upstream gradient {tuple(g.shape)} does not fit {state.args.M} rows")
     outs = []
     for given, like, want, name in ((dx, state.x, need[0], "dx"), (dW, state.W, need[1], "dW"), (db, state.b, need[2], "db")):
@@ -1060,7 +1061,7 @@ def vocab_ce_backward(state, grad=None, row_grad=None, mean=True, dx=None, dW=No
     dx, dW, db = outs
     r = byref(state.args)
     ws_bytes = lib.capdec_vocab_ce_backward_workspace_bytes(r)
-    ws = _bytes(ws_bytes, g.device)
+    ws = _bytes(ws_bytes, state.saved.device)
     _lib.check(lib.capdec_vocab_ce_backward(r, state.saved.data_ptr(), state.saved.numel(), ws.data_ptr(), ws_bytes,
                                             _ptr(row_grad), _ptr(grad), 1 if mean else 0, _ptr(dx),
                                             0 if dx is None else _row_stride(dx, "dx"), _ptr(dW),
@@ -1098,13 +1099,29 @@ def _matrices(what, ts, dtypes):
     return ts
 
 
-def _distinct(what, ts):
-    """Outputs of one call must not share memory."""
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.element_size() * (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1))
-                   for t in ts)
-    for (_, end), (start, _) in zip(spans, spans[1:]):
-        if start < end:
-            raise RuntimeError(f"capdec {what}: two of the matrices written overlap in memory")
+def _overlap(a, b):
+    """Whether two row-contiguous matrices share memory; columns of one wider matrix side by side do not."""
+    ea, eb = a.element_size(), b.element_size()
+    pa, pb = a.data_ptr(), b.data_ptr()
+    la, lb = a.stride(0) * ea, b.stride(0) * eb
+    if pa + (a.shape[0] - 1) * la + a.shape[1] * ea <= pb or pb + (b.shape[0] - 1) * lb + b.shape[1] * eb <= pa:
+        return False
+    off = (pb - pa) % la if la == lb and la > 0 else 0
+    return not (off >= a.shape[1] * ea and off + b.shape[1] * eb <= la)
+
+
+def _check_overlap(what, written, read=()):
+    """No matrix written may share memory with another one of the call.  In address order, neighbours tell: a matrix that
+    reaches past the next one's start overlaps it or lies beside it in one wider matrix."""
+    ts = sorted([(t.data_ptr(), i, t, True) for i, t in enumerate(written)] +
+                [(t.data_ptr(), i, t, False) for i, t in enumerate(read)], key=lambda q: q[0])
+    for k, (p, _, t, w) in enumerate(ts):
+        end = p + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
+        for q, _, u, x in ts[k + 1:]:
+            if q >= end:
+                break
+            if (w or x) and _overlap(t, u):
+                raise RuntimeError(f"capdec {what}: a matrix that is written overlaps another one in memory")
 
 
 def orthogonalize(mats, steps=5, coeffs=NS_COEFFS, eps=1e-7, out=None):
@@ -1122,8 +1139,7 @@ def orthogonalize(mats, steps=5, coeffs=NS_COEFFS, eps=1e-7, out=None):
     if [(t.shape, t.dtype) for t in src] != [(t.shape, t.dtype) for t in dst]:
         raise RuntimeError("capdec orthogonalize: out must match the matrices in shape and type")
     _same_device("orthogonalize", src + dst)
-    if len(dst) > 1:
-        _distinct("orthogonalize", dst)
+    _check_overlap("orthogonalize", dst, [t for t, d in zip(src, dst) if t.data_ptr() != d.data_ptr() or t.stride() != d.stride()])
     co = _ns_coeffs(coeffs)
     for (rows, cols), idx in _by_shape(src).items():
         arr = (_lib.Matrix * len(idx))()
@@ -1159,7 +1175,7 @@ def muon_step(params, grads, momenta, lr=None, state=None, momentum=0.95, nester
     if not ([t.shape for t in p] == [t.shape for t in g] == [t.shape for t in m]):
         raise RuntimeError("capdec muon_step: params, grads and momenta must match in number and shape")
     _same_device("muon_step", p + g + m)
-    _distinct("muon_step", p + m)
+    _check_overlap("muon_step", p + m, g)
     co = _ns_coeffs(coeffs)
     for (rows, cols), idx in _by_shape(p).items():
         arr = (_lib.MuonParam * len(idx))()

@@ -183,7 +183,7 @@ __global__ __launch_bounds__(256) void normalise_kernel(Batch b, int rows, int c
     for (int k = threadIdx.x & 63; k < nparts; k += 64) s += part[blockIdx.y * NORM_BLOCKS + k];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    const float inv = (float)((double)scale / (sqrt(s) + (double)eps));
+    const float inv = s == 0.0 ? 0.f : (float)((double)scale / (sqrt(s) + (double)eps));
     short* x = X + blockIdx.y * x_elems;
     const int cpr = cp / 8;
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < (int64_t)rp * cpr; t += (int64_t)gridDim.x * 256) {
@@ -448,7 +448,7 @@ int exponent_for(double top) {
     if (!(top > 0)) return 14;
     int e;
     frexp(top * 1.01, &e);                        // top < 2^e
-    return 15 - e;
+    return e < -45 ? 60 : 15 - e;                 // an iterate that shrinks away needs no more
 }
 
 struct Iteration {

@@ -73,6 +73,7 @@ bool wide_pays(int64_t wide_tiles, int kt) { return kt >= 48 && wide_tiles >= 25
 bool make_plan(const capdec_vocab_ce* a, Plan& p) {
     if (!a || a->M < 1 || a->V < 1 || a->K < 1 || a->dtype < 0 || a->dtype > 2) return false;
     if (a->M > (1 << 24) || a->V > (1 << 24) || a->K > (1 << 20)) return false;
+    if ((int64_t)a->M * a->V > (int64_t)1 << 42) return false;          // tiles are counted in 32 bits
     p = Plan{};
     p.M = a->M; p.V = a->V; p.K = a->K;
     p.Mp = (a->M + 255) / 256 * 256;
@@ -485,7 +486,8 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ nl
 
 // ---- backward -----------------------------------------------------------------------------------------------------
 // What each row of G is multiplied by, brought to [2^13, 2^14] at most by a power of two, and the factor that undoes it.
-// row_grad: the rows' own upstream gradients; else one scalar for all of them (divided by the count when `mean`).
+// row_grad: the rows' own upstream gradients; else one scalar for all of them, 1 where there is none (divided by the count
+// when `mean`).
 __global__ __launch_bounds__(1024) void weights_kernel(const float* __restrict__ row_grad, const float* __restrict__ grad,
                                                        int mean, const Head* __restrict__ head,
                                                        const int* __restrict__ order, int Mp, float* __restrict__ rw,
@@ -512,7 +514,7 @@ __global__ __launch_bounds__(1024) void weights_kernel(const float* __restrict__
         rw[s] = s >= count ? 0.f : row_grad ? row_grad[order[s]] * scale : scale;
     if (threadIdx.x == 0) {
         float f = 1.f / scale;
-        if (!row_grad) f *= grad[0] / (mean ? (float)count : 1.f);
+        if (!row_grad) f *= (grad ? grad[0] : 1.f) / (mean ? (float)count : 1.f);
         bh->factor = count > 0 ? f : 0.f;
     }
 }
@@ -901,7 +903,7 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
                              size_t workspace_bytes, const float* row_grad, const float* grad, int mean, void* dx,
                              int64_t lddx, void* dW, int64_t lddw, void* dbias, void* stream) {
     Plan p;
-    CAPDEC_REQUIRE(valid(a) && make_plan(a, p) && saved && workspace && (row_grad || grad));
+    CAPDEC_REQUIRE(valid(a) && make_plan(a, p) && saved && workspace && !(row_grad && grad));
     CAPDEC_REQUIRE(!dx || p.M == 1 || lddx >= p.K);
     CAPDEC_REQUIRE(!dW || p.V == 1 || lddw >= p.K);
     CAPDEC_REQUIRE(!dbias || a->bias);

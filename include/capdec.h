@@ -621,13 +621,13 @@ int capdec_satt_greedy_decode(const capdec_satt_model* m, const float* enc, cons
  *   z = x W^T + bias;  nll[r] = log(sum_v exp z[r,v]) - z[r, targets[r]], 0 where targets[r] == ignore_index
  * x [M,K] and W [V,K] have unit column stride and row strides ldx, ldw (elements); x, W, bias and their gradients share
  * one type.  Rows whose target is ignore_index are not read at all.  A counted target outside [0, V) makes its loss and
- * the gradients it enters NaN.  M, V <= 2^24, K <= 2^20.
+ * the gradients it enters NaN.  M, V <= 2^24, M V <= 2^42, K <= 2^20.
  * `saved` (capdec_vocab_ce_saved_bytes) carries packed operands and row statistics from the forward call to the backward
  * call, which reads W again: neither W nor `saved` may change in between.  `workspace` is scratch of one call.  Both are
  * 16-byte aligned.  Sums run in fixed orders: results repeat bit for bit.
  * forward: nll [M] fp32; loss (nullable) [3] fp32 = (mean over the counted rows, NaN without any; sum; their number).
- * backward: the upstream gradient is row_grad [M] (fp32, d/d nll) or, where that is NULL, grad[0] for the sum of nll
- * (mean == 0) or for its mean (mean != 0); dx, dW, dbias are written (not added to), any of them may be NULL.
+ * backward: the upstream gradient is row_grad [M] (fp32, d/d nll) or, where that is NULL, grad[0] (NULL: 1) for the sum of
+ * nll (mean == 0) or for its mean (mean != 0); dx, dW, dbias are written (not added to), any of them may be NULL.
  * ------------------------------------------------------------------------------------------ */
 #define CAPDEC_F32 0
 #define CAPDEC_BF16 1

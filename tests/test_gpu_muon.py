@@ -90,6 +90,17 @@ def test_strided_matrices():
     assert bool((out[:, 0] == 7).all()) and bool((out[:, 71:] == 7).all())
 
 
+def test_columns_of_one_wider_matrix():
+    """Three projections side by side in one matrix, updated in place."""
+    from capdec import ops
+    w = gradient_like((64, 150)) * 1e3
+    parts, want = [w[:, 50 * k:50 * k + 50] for k in range(3)], [w[:, 50 * k:50 * k + 50].contiguous() for k in range(3)]
+    g, m = [gradient_like((64, 50), k) for k in range(3)], [torch.zeros(64, 50, device="cuda") for _ in range(6)]
+    ops.muon_step(parts, g, m[:3], lr=0.1)
+    ops.muon_step(want, g, m[3:], lr=0.1)
+    assert all(torch.equal(a, b) for a, b in zip(parts, want))
+
+
 def test_steps_coefficients_and_spectra():
     """Other iterations, and spectra from one direction to six orders of magnitude."""
     from capdec import ops
@@ -111,7 +122,10 @@ def test_scale_does_not_matter_and_zero_stays_zero():
     want = definition(G, eps=0.0)
     for s in (1e-25, 1e-10, 1e10, 1e30):
         near(ops.orthogonalize(G * s, eps=0.0), want, torch.float32)
-    assert int(ops.orthogonalize(torch.zeros(3, 40, 50, device="cuda")).count_nonzero()) == 0
+    for eps in (1e-7, 0.0):
+        assert int(ops.orthogonalize(torch.zeros(3, 40, 50, device="cuda"), eps=eps).count_nonzero()) == 0
+    out = ops.orthogonalize(G, coeffs=(1e-9, 0.0, 0.0))            # an iterate that shrinks away
+    assert bool(out.isfinite().all()) and float(out.norm()) < 1e-30
     bad = torch.stack([G, G, G])
     bad[1, 5, 5] = float("nan")
     out = ops.orthogonalize(bad)
@@ -185,7 +199,11 @@ def test_refusals_on_the_gpu():
     with pytest.raises(RuntimeError, match="overlap"):
         ops.muon_step([G, G], [G, G], [G.clone(), G.clone()], lr=0.1)
     with pytest.raises(RuntimeError, match="overlap"):
-        ops.muon_step([G], [G], [G], lr=0.1)
+        ops.muon_step([G], [G.clone()], [G], lr=0.1)
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.muon_step([G.clone()], [G], [G], lr=0.1)
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.orthogonalize([G, G.clone()], out=[G.clone(), G])
     with pytest.raises(RuntimeError, match="2-D|rows"):
         ops.orthogonalize(G.t())
     with pytest.raises(RuntimeError, match="type"):

@@ -217,6 +217,27 @@ def test_strides_and_alignment(dt):
     assert got.shape == (10, 13) and torch.equal(got.sum(), F.vocab_cross_entropy(x, W, b, t, reduction="none").view(10, 13).sum())
 
 
+def test_broadcast_inputs():
+    """Rows of x that are one row: its gradient is the sum of theirs."""
+    from capdec import functional as F
+    x, W, b, t = make(40, 300, 64, torch.float32, seed=13, ignored=0.3)
+    row = x[:1].detach().requires_grad_()
+    g, = torch.autograd.grad(F.vocab_cross_entropy(row.expand(40, 64), W, b, t), (row,))
+    (nll, dx, _, _), (_, tol, _, _) = definition(row.detach().expand(40, 64), W, b, t, torch.full((40,), 1 / int((t != 0).sum()), device="cuda"))
+    near(g, dx.sum(0, keepdim=True), tol.sum(0, keepdim=True) + 40 * 2.0 ** -24 * dx.abs().sum(0, keepdim=True), "dx")
+
+
+def test_operands_changed_in_between_are_noticed():
+    from capdec import functional as F
+    x, W, b, t = make(40, 300, 64, torch.float32, seed=14)
+    W.requires_grad_()
+    loss = F.vocab_cross_entropy(x, W, b, t)
+    with torch.no_grad():
+        W += 1
+    with pytest.raises(RuntimeError, match="modified"):
+        loss.backward()
+
+
 def test_gradients_written_into_given_buffers_with_strides():
     from capdec import ops
     x, W, b, t = make(130, 520, 96, torch.float32, seed=8)
@@ -227,6 +248,7 @@ def test_gradients_written_into_given_buffers_with_strides():
     got = ops.vocab_ce_backward(saved, grad=one, dx=bx[:, :96], dW=bw[:, :96])
     assert all(torch.equal(a, c) for a, c in zip(got, want))
     assert bool((bx[:, 96:] == 7).all()) and bool((bw[:, 96:] == 7).all())
+    assert all(torch.equal(a, c) for a, c in zip(ops.vocab_ce_backward(saved), want))        # no upstream gradient: 1
     only = ops.vocab_ce_backward(saved, grad=one, need=(False, False, True))
     assert only[0] is None and only[1] is None and torch.equal(only[2], want[2])
     only = ops.vocab_ce_backward(saved, grad=one, need=(False, True, False))

@@ -26,7 +26,8 @@ def test_vocab_ce_sizes():
         big = ce(dtype=dtype, M=100000, V=200000)
         assert lib.capdec_vocab_ce_backward_workspace_bytes(big) < (512 << 20) + 17 * 100096 * 64 * 4 + 17 * 200192 * 64 * 4
     assert lib.capdec_vocab_ce_saved_bytes(ce(dtype=1, K=50, ldw=50)) > 1000 * 64 * 2      # odd widths are packed
-    for bad in (dict(M=0), dict(V=0), dict(K=0), dict(dtype=3), dict(dtype=-1), dict(M=1 << 25), dict(V=1 << 25), dict(K=1 << 21)):
+    for bad in (dict(M=0), dict(V=0), dict(K=0), dict(dtype=3), dict(dtype=-1), dict(M=1 << 25), dict(V=1 << 25), dict(K=1 << 21),
+                dict(M=1 << 24, V=1 << 19)):
         a = ce(**bad)
         assert lib.capdec_vocab_ce_saved_bytes(a) == 0 and lib.capdec_vocab_ce_backward_workspace_bytes(a) == 0
     assert lib.capdec_vocab_ce_saved_bytes(None) == 0
@@ -50,7 +51,7 @@ def test_vocab_ce_refusals():
     assert fwd(a, saved=BASE + 4) == EALIGN and fwd(a, ws=BASE + 8) == EALIGN
     assert fwd(a, ns=lib.capdec_vocab_ce_saved_bytes(a) - 1) == ENOMEM
     assert fwd(a, nw=lib.capdec_vocab_ce_forward_workspace_bytes(a) - 1) == ENOMEM
-    assert bwd(a, g=None) == EINVAL and bwd(a, ldx=63) == EINVAL and bwd(a, ldw=60) == EINVAL
+    assert bwd(a, row=BASE) == EINVAL and bwd(a, ldx=63) == EINVAL and bwd(a, ldw=60) == EINVAL
     assert bwd(a, db=BASE) == EINVAL                                       # a bias gradient without a bias
     assert bwd(a, ns=100) == ENOMEM and bwd(a, nw=lib.capdec_vocab_ce_backward_workspace_bytes(a) - 1) == ENOMEM
     assert bwd(a, ws=BASE + 4) == EALIGN
@@ -87,6 +88,20 @@ def test_orthogonalize_and_muon_refusals():
                 dict(steps=-1), dict(ws=None), dict(c=None)):
         assert muon(**bad) == EINVAL, bad
     assert muon(ws=BASE + 4) == EALIGN and muon(nw=16) == ENOMEM
+
+
+def test_overlapping_matrices_are_told_apart():
+    """Rows of one matrix, columns of one wider matrix and separate ones do not overlap; anything shared does."""
+    from capdec import ops
+    w = torch.zeros(20, 60)
+    ops._check_overlap("t", [w[:10], w[10:]])
+    ops._check_overlap("t", [w[:, :20], w[:, 20:40], w[:, 40:], torch.zeros(20, 60)])
+    ops._check_overlap("t", [w[3:9, 40:50]], [w[3:9, 50:]])
+    ops._check_overlap("t", [torch.zeros(4, 4)], [w, w, w[:5]])            # what is only read may be the same twice
+    for written, read in (([w, w], []), ([w[:11], w[10:]], []), ([w[:, :21], w[:, 20:40]], []), ([w], [w]),
+                          ([w[:, 10:30]], [w[5:6, 29:35]]), ([w[:10]], [w[9:, :1]]), ([w[2:4]], [w]), ([w[0:1], w[0:1]], [])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops._check_overlap("t", written, read)
 
 
 def test_python_wrappers_refuse_what_they_cannot_take():
