@@ -691,9 +691,17 @@ class _VocabCrossEntropyFn(torch.autograd.Function):
         if ctx.state is None:
             return tuple(torch.zeros_like(t) if t is not None and n else None
                          for t, n in zip((x, W, b), ctx.needs_input_grad)) + (None, None, None)
-        g = g.float().contiguous()
-        up = dict(row_grad=g) if ctx.reduction == "none" else dict(grad=g, mean=ctx.reduction == "mean")
-        dx, dW, db = ops.vocab_ce_backward(ctx.state, need=ctx.needs_input_grad[:3], **up)
+        # (the gradient of an fp32 loss is fp32; a row's may come expanded)
+        rows = ctx.reduction == "none"
+        if rows:
+            g = g.contiguous()
+        nx, nw, nb = ctx.needs_input_grad[:3]
+        st = ctx.state
+        K = x.shape[1]
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if nx else None
+        dW = torch.empty(W.shape, device=x.device, dtype=x.dtype) if nw else None
+        db = torch.empty(b.shape, device=x.device, dtype=x.dtype) if nb else None
+        ops._vocab_ce_backward(st, g if rows else None, None if rows else g, ctx.reduction == "mean", dx, K, dW, K, db)
         return dx, dW, db, None, None, None
 
 

@@ -979,7 +979,7 @@ _DTYPE_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16
 
 def _same_device(what, tensors):
     """Every tensor on the current GPU (the wrappers launch on its current stream)."""
-    here = torch.cuda.current_device() if torch.cuda.is_available() else None
+    here = torch.cuda.current_device() if torch.cuda.is_initialized() or torch.cuda.is_available() else None
     for t in tensors:
         if t.get_device() != here:
             raise RuntimeError(f"capdec {what}: every tensor must be on the current GPU (HIP device {here}), got {t.device}; "
@@ -993,7 +993,7 @@ def _bytes(n, device):
 class VocabCEState:
     """What ``vocab_ce_forward`` leaves for ``vocab_ce_backward``: the operands (neither of them may change in between), the
     call's arguments, and the packed operands and row statistics in device memory."""
-    __slots__ = ("x", "W", "b", "targets", "args", "saved")
+    __slots__ = ("x", "W", "b", "targets", "args", "ref", "saved", "ws_bytes")
 
 
 def vocab_ce_forward(x, W, b, targets, ignore_index=0, want_loss=True):
@@ -1006,41 +1006,53 @@ def vocab_ce_forward(x, W, b, targets, ignore_index=0, want_loss=True):
         if not isinstance(t, torch.Tensor):
             raise RuntimeError(f"capdec vocab_ce: tensors expected, got {type(t).__name__}")
     _same_device("vocab_ce", ts)
-    code = _DTYPE_CODE.get(x.dtype)
-    if code is None or W.dtype != x.dtype or (b is not None and b.dtype != x.dtype):
+    dtype, code = x.dtype, _DTYPE_CODE.get(x.dtype)
+    if code is None or W.dtype != dtype or (b is not None and b.dtype != dtype):
         raise RuntimeError("capdec vocab_ce: x, W and bias must share one type, float32, bfloat16 or float16; got "
-                           f"{x.dtype}, {W.dtype}" + (f", {b.dtype}" if b is not None else ""))
-    if x.dim() != 2 or W.dim() != 2:
-        raise RuntimeError(f"capdec vocab_ce: x [M,K] and W [V,K] expected, got {tuple(x.shape)} and {tuple(W.shape)}")
-    (M, K), (V, k) = x.shape, W.shape
-    if k != K or min(M, K, V) < 1:
-        raise RuntimeError(f"capdec vocab_ce: x [M,K] and W [V,K] expected, got {tuple(x.shape)} and {tuple(W.shape)}")
-    if targets.dtype != torch.int64 or targets.dim() != 1 or targets.shape[0] != M or not targets.is_contiguous():
+                           f"{dtype}, {W.dtype}" + (f", {b.dtype}" if b is not None else ""))
+    xs, wsh = x.shape, W.shape
+    if len(xs) != 2 or len(wsh) != 2 or xs[1] != wsh[1] or min(xs[0], xs[1], wsh[0]) < 1:
+        raise RuntimeError(f"capdec vocab_ce: x [M,K] and W [V,K] expected, got {tuple(xs)} and {tuple(wsh)}")
+    (M, K), V = xs, wsh[0]
+    if targets.dtype != torch.int64 or targets.shape != (M,) or not targets.is_contiguous():
         raise RuntimeError(f"capdec vocab_ce: targets must be {M} contiguous int64 values, got {targets.dtype} "
                            f"{tuple(targets.shape)}")
-    if b is not None and (b.dim() != 1 or b.shape[0] != V or not b.is_contiguous()):
+    if b is not None and (b.shape != (V,) or not b.is_contiguous()):
         raise RuntimeError(f"capdec vocab_ce: bias must hold {V} contiguous values, got {tuple(b.shape)}")
-    a = _lib.VocabCE(x.data_ptr(), W.data_ptr(), _ptr(b), targets.data_ptr(), _row_stride(x, "x"), _row_stride(W, "W"),
-                     ignore_index, M, V, K, code)
-    r = byref(a)
+    st = VocabCEState()
+    st.x, st.W, st.b, st.targets = x, W, b, targets
+    st.args = a = _lib.VocabCE(x.data_ptr(), W.data_ptr(), _ptr(b), targets.data_ptr(), _row_stride(x, "x"),
+                               _row_stride(W, "W"), ignore_index, M, V, K, code)
+    st.ref = r = byref(a)
     saved_bytes, ws_bytes = lib.capdec_vocab_ce_saved_bytes(r), lib.capdec_vocab_ce_forward_workspace_bytes(r)
     if not saved_bytes:
         raise RuntimeError(f"capdec vocab_ce: unsupported sizes M={M} V={V} K={K}")
-    saved, ws = _bytes(saved_bytes, x.device), _bytes(ws_bytes, x.device)
-    out = torch.empty(M + 3, device=x.device, dtype=torch.float32)
+    st.ws_bytes = None
+    dev = x.device
+    st.saved = saved = _bytes(saved_bytes, dev)
+    ws, out = _bytes(ws_bytes, dev), torch.empty(M + 3, device=dev, dtype=torch.float32)
     p = out.data_ptr()
     _lib.check(lib.capdec_vocab_ce_forward(r, saved.data_ptr(), saved_bytes, ws.data_ptr(), ws_bytes, p,
                                            p + 4 * M if want_loss else None, _stream()), "capdec_vocab_ce_forward")
-    state = VocabCEState()
-    state.x, state.W, state.b, state.targets, state.args, state.saved = x, W, b, targets, a, saved
-    return out[:M], out[M:] if want_loss else None, state
+    return out[:M], out[M:] if want_loss else None, st
+
+
+def _vocab_ce_backward(st, row_grad, grad, mean, dx, lddx, dW, lddw, db):
+    """The launch of ``vocab_ce_backward`` on checked tensors (None: not wanted, or no upstream gradient)."""
+    lib = _lib.load()
+    if st.ws_bytes is None:
+        st.ws_bytes = lib.capdec_vocab_ce_backward_workspace_bytes(st.ref)
+    n, saved = st.ws_bytes, st.saved
+    ws = _bytes(n, saved.device)
+    _lib.check(lib.capdec_vocab_ce_backward(st.ref, saved.data_ptr(), saved.numel(), ws.data_ptr(), n, _ptr(row_grad),
+                                            _ptr(grad), 1 if mean else 0, _ptr(dx), lddx, _ptr(dW), lddw, _ptr(db),
+                                            _stream()), "capdec_vocab_ce_backward")
 
 
 def vocab_ce_backward(state, grad=None, row_grad=None, mean=True, dx=None, dW=None, db=None, need=(True, True, True)):
     """Gradients of ``vocab_ce_forward``.  The upstream gradient is ``row_grad`` [M] fp32 (of nll) or ``grad``, a one-element
-    fp32 tensor (of the mean, or with ``mean=False`` of the sum; None: 1).  Returns (dx, dW, db) in the operands' type, written into
-    the tensors given for them, or None where ``need`` says so."""
-    lib = _lib.load()
+    fp32 tensor (of the mean, or with ``mean=False`` of the sum; None: 1).  Returns (dx, dW, db) in the operands' type,
+    written into the tensors given for them, or None where ``need`` says so."""
     if grad is not None and row_grad is not None:
         raise RuntimeError("capdec vocab_ce_backward: at most one of grad and row_grad")
     g = grad if grad is not None else row_grad
@@ -1059,14 +1071,8 @@ def vocab_ce_backward(state, grad=None, row_grad=None, mean=True, dx=None, dW=No
         outs.append(given)
     _same_device("vocab_ce_backward", [t for t in (g, state.saved, *outs) if t is not None])
     dx, dW, db = outs
-    r = byref(state.args)
-    ws_bytes = lib.capdec_vocab_ce_backward_workspace_bytes(r)
-    ws = _bytes(ws_bytes, state.saved.device)
-    _lib.check(lib.capdec_vocab_ce_backward(r, state.saved.data_ptr(), state.saved.numel(), ws.data_ptr(), ws_bytes,
-                                            _ptr(row_grad), _ptr(grad), 1 if mean else 0, _ptr(dx),
-                                            0 if dx is None else _row_stride(dx, "dx"), _ptr(dW),
-                                            0 if dW is None else _row_stride(dW, "dW"), _ptr(db), _stream()),
-               "capdec_vocab_ce_backward")
+    _vocab_ce_backward(state, row_grad, grad, mean, dx, 0 if dx is None else _row_stride(dx, "dx"), dW,
+                       0 if dW is None else _row_stride(dW, "dW"), db)
     return dx, dW, db
 
 

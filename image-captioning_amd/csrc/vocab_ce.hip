@@ -143,9 +143,19 @@ struct Head {               // first 256 bytes of the saved buffer
     int count;              // rows with a counted target
     unsigned amax_x, amax_w;   // bits of the largest finite magnitude (split operands)
 };
-struct BwdHead {            // first 256 bytes of the backward workspace
+struct BwdHead {            // first 256 bytes of the backward workspace (upstream gradients of the rows)
     float factor;           // what dx, dW and db are to be multiplied by
 };
+struct Upstream {           // where that factor comes from: a BwdHead, or one scalar (NULL: 1) for the sum or mean of the rows
+    const BwdHead* bh;
+    const float* grad;
+    int mean;
+};
+__device__ __forceinline__ float factor_of(const Upstream& u, const Head* head) {
+    if (u.bh) return u.bh->factor;
+    if (head->count == 0) return 0.f;
+    return ldexpf((u.grad ? u.grad[0] : 1.f) / (u.mean ? (float)head->count : 1.f), -G_EXP);
+}
 
 // power of two that brings amax to [2^14, 2^15); the operands' scales are undone in fp32
 __device__ __forceinline__ int scale_exp(unsigned amax_bits) {
@@ -485,38 +495,28 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ nl
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------
-// What each row of G is multiplied by, brought to [2^13, 2^14] at most by a power of two, and the factor that undoes it.
-// row_grad: the rows' own upstream gradients; else one scalar for all of them, 1 where there is none (divided by the count
-// when `mean`).
-__global__ __launch_bounds__(1024) void weights_kernel(const float* __restrict__ row_grad, const float* __restrict__ grad,
-                                                       int mean, const Head* __restrict__ head,
+// The rows' own upstream gradients, brought to [2^13, 2^14] at most by a power of two, and the factor that undoes it.  (One
+// scalar for all rows needs no kernel: G is stored times 2^14, and factor_of() has the rest.)
+__global__ __launch_bounds__(1024) void weights_kernel(const float* __restrict__ row_grad, const Head* __restrict__ head,
                                                        const int* __restrict__ order, int Mp, float* __restrict__ rw,
                                                        BwdHead* __restrict__ bh) {
     const int count = head->count;
-    float scale = pow2(G_EXP);
     __shared__ float wm[16];
-    if (row_grad) {
-        float m = 0.f;
-        for (int s = threadIdx.x; s < count; s += 1024) {
-            const float v = fabsf(row_grad[order[s]]);
-            if (v < INFINITY) m = fmaxf(m, v);
-        }
-        m = wave_max(m);
-        if ((threadIdx.x & 63) == 0) wm[threadIdx.x >> 6] = m;
-        __syncthreads();
-        m = 0.f;
-        for (int w = 0; w < 16; ++w) m = fmaxf(m, wm[w]);
-        // amax * scale in [2^13, 2^14)
-        const int e = (int)(__float_as_uint(m) >> 23) - 127;
-        scale = m > 0.f ? pow2(min(G_EXP - 1 - e, 126)) : 1.f;
+    float m = 0.f;
+    for (int s = threadIdx.x; s < count; s += 1024) {
+        const float v = fabsf(row_grad[order[s]]);
+        if (v < INFINITY) m = fmaxf(m, v);
     }
-    for (int s = threadIdx.x; s < Mp; s += 1024)
-        rw[s] = s >= count ? 0.f : row_grad ? row_grad[order[s]] * scale : scale;
-    if (threadIdx.x == 0) {
-        float f = 1.f / scale;
-        if (!row_grad) f *= (grad ? grad[0] : 1.f) / (mean ? (float)count : 1.f);
-        bh->factor = count > 0 ? f : 0.f;
-    }
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) wm[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = 0.f;
+    for (int w = 0; w < 16; ++w) m = fmaxf(m, wm[w]);
+    // m * scale in [2^13, 2^14)
+    const int e = (int)(__float_as_uint(m) >> 23) - 127;
+    const float scale = m > 0.f ? pow2(min(G_EXP - 1 - e, 126)) : 1.f;
+    for (int s = threadIdx.x; s < Mp; s += 1024) rw[s] = s < count ? row_grad[order[s]] * scale : 0.f;
+    if (threadIdx.x == 0) bh->factor = count > 0 ? 1.f / scale : 0.f;
 }
 
 // G of one piece of the vocabulary.  The tile is turned through LDS (a wavefront's 64 rows x 128 words at a time), so
@@ -549,7 +549,7 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void dlogits_kernel(LogitArgs a)
         const int s = j0 + (wj * C::TJ + tj) * 32 + (lane & 31);
         const bool live = s < count;
         const float l2 = live ? a.lse[s] : 0.f;
-        const float w = live ? a.rw[s] : 0.f;
+        const float w = live ? (a.rw ? a.rw[s] : pow2(G_EXP)) : 0.f;
         const float* b2 = a.b2 + i0 + wi * WORDS;
 #pragma unroll
         for (int ti = 0; ti < C::TI; ++ti) {
@@ -649,7 +649,7 @@ constexpr int REST_ROWS = 64;
 struct GradArgs {
     View P, Q;
     const Head* head;
-    const BwdHead* bh;
+    Upstream up;
     int I, J;                      // rows and columns stored
     int rows_live;                 // dx: only the first count rows exist
     int k_live;                    // dW: the contraction runs over the counted rows; else over kt k-tiles
@@ -705,7 +705,7 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void grad_kernel(GradArgs a) {
     }
     float f = 1.f;
     if (OUT == 1) {
-        f = a.bh->factor;
+        f = factor_of(a.up, a.head);
         if (SPLIT) f *= pow2(-scale_exp(a.head->amax_x));
     }
 #pragma unroll
@@ -733,9 +733,9 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void grad_kernel(GradArgs a) {
 __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part, Splits splits, int Kp, int M, int K,
                                                  const int* __restrict__ slot, const int* __restrict__ tgt,
                                                  const float* __restrict__ rest, const void* W, int64_t ldw,
-                                                 const Head* __restrict__ head, const BwdHead* __restrict__ bh, int split,
-                                                 void* out, int64_t ldo, int dtype) {
-    const float f = bh->factor * (split ? pow2(-scale_exp(head->amax_w)) : 1.f);
+                                                 const Head* __restrict__ head, Upstream up, int split, void* out,
+                                                 int64_t ldo, int dtype) {
+    const float f = factor_of(up, head) * (split ? pow2(-scale_exp(head->amax_w)) : 1.f);
     const int tiles = (head->count + 255) / 256, nsplit = splits_of(splits, tiles);
     const int64_t plane = (int64_t)tiles * 256 * Kp;
     const int cpr = (K + 3) / 4;
@@ -763,10 +763,9 @@ __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part,
 
 // dW of one piece from its partial sums, and db from the row tiles' column sums
 __global__ __launch_bounds__(256) void dw_kernel(const float* __restrict__ part, int64_t plane, int nsplit, int Kp, int rows,
-                                                 int K, const Head* __restrict__ head, const BwdHead* __restrict__ bh,
-                                                 int split, void* dW, int64_t ldw, int dtype, const float* __restrict__ dbp,
+                                                 int K, const Head* __restrict__ head, Upstream up, int split, void* dW, int64_t ldw, int dtype, const float* __restrict__ dbp,
                                                  int piece, int row_tile, void* db, int v0) {
-    const float fb = bh->factor;
+    const float fb = factor_of(up, head);
     const float f = fb * (split ? pow2(-scale_exp(head->amax_x)) : 1.f);
     const int cpr = (K + 3) / 4;
     const int64_t nw = nsplit > 1 ? (int64_t)rows * cpr : 0;
@@ -916,11 +915,13 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
     const Head* head = (const Head*)sv;
     const int* order = (const int*)(sv + p.o_order);
     const int* slot = (const int*)(sv + p.o_slot);
-    BwdHead* bh = (BwdHead*)ws;
-    float* rw = (float*)(ws + p.o_rw);
+    float* rw = row_grad ? (float*)(ws + p.o_rw) : nullptr;
+    const Upstream up{row_grad ? (const BwdHead*)ws : nullptr, grad, mean};
     float* rest = (float*)(ws + p.o_rest);
-    weights_kernel<<<1, 1024, 0, s>>>(row_grad, grad, mean, head, order, p.Mp, rw, bh);
-    CAPDEC_LAUNCH_CHECK();
+    if (row_grad) {
+        weights_kernel<<<1, 1024, 0, s>>>(row_grad, head, order, p.Mp, rw, (BwdHead*)ws);
+        CAPDEC_LAUNCH_CHECK();
+    }
     const short* px = (const short*)(sv + p.o_x);
     const short* W = p.pack_w ? (const short*)(sv + p.o_w) : (const short*)a->W;
     const int64_t ldw = p.pack_w ? p.xs : a->ldw;
@@ -943,7 +944,7 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
             GradArgs d{};
             d.P = View{G, g.ldg, p.Mp, 0};
             d.Q = View{W + (int64_t)v0 * ldw, ldw, p.Kp, real};
-            d.head = head; d.bh = bh; d.I = p.Mp; d.J = p.Kp; d.rows_live = 1; d.kt = words / kt; d.splits = p.sx;
+            d.head = head; d.up = up; d.I = p.Mp; d.J = p.Kp; d.rows_live = 1; d.kt = words / kt; d.splits = p.sx;
             d.part = dxp; d.ldp = p.Kp; d.add = v0 > 0;
 #define DX(E, S) (p.wide_dx ? launch_grad<Wide, E, false, S, 0>(d, p.Mp, p.Kp, p.dx_tiles, s) : launch_grad<Big, E, false, S, 0>(d, p.Mp, p.Kp, p.dx_tiles, s))
             CAPDEC_TRY(BY_TYPE(p, DX));
@@ -953,7 +954,7 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
             GradArgs d{};
             d.P = View{G, g.ldg, words, p.Mp};
             d.Q = View{px, (int64_t)p.xs, p.Kp, p.Mp};
-            d.head = head; d.bh = bh; d.k_live = 1; d.nsplit = p.sw;
+            d.head = head; d.up = up; d.k_live = 1; d.nsplit = p.sw;
             d.tgt = g.tgt; d.rest = rest; d.v0 = v0;
             if (p.sw == 1) {
                 d.I = real; d.J = p.K;
@@ -973,14 +974,14 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
         if (slabs > 1 || dbias) {
             const int64_t items = (slabs > 1 ? (int64_t)real * ((p.K + 3) / 4) : 0) + (dbias ? real : 0);
             dw_kernel<<<blocks_for(items, 256, 8192), 256, 0, s>>>((const float*)(ws + p.o_dw), (int64_t)p.piece * p.Kp, slabs,
-                                                                   p.Kp, real, p.K, head, bh, p.split, dW, lddw, a->dtype,
+                                                                   p.Kp, real, p.K, head, up, p.split, dW, lddw, a->dtype,
                                                                    g.dbp, p.piece, p.wide_z ? Wide::BJ : Big::BJ, dbias, v0);
             CAPDEC_LAUNCH_CHECK();
         }
     }
     if (dx) {
         dx_kernel<<<blocks_for((int64_t)p.M * ((p.K + 3) / 4), 256, 8192), 256, 0, s>>>(
-            dxp, p.sx, p.Kp, p.M, p.K, slot, (const int*)(sv + p.o_tgt), rest, a->W, a->ldw, head, bh, p.split, dx, lddx, a->dtype);
+            dxp, p.sx, p.Kp, p.M, p.K, slot, (const int*)(sv + p.o_tgt), rest, a->W, a->ldw, head, up, p.split, dx, lddx, a->dtype);
         CAPDEC_LAUNCH_CHECK();
     }
     return 0;
