@@ -72,7 +72,6 @@ def vocab_cross_entropy(x, weight, bias, targets, ignore_index=0, reduction="mea
 
     A backward pass that is to be captured in a HIP graph must not run while an eager graph of the same leaves is alive:
     drop the losses of earlier eager passes first."""
-    from . import autograd as AG
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"capdec: reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
     if x.dim() < 1 or x.shape[:-1] != targets.shape:
@@ -80,5 +79,12 @@ def vocab_cross_entropy(x, weight, bias, targets, ignore_index=0, reduction="mea
     x2, t = x.reshape(-1, x.shape[-1]), targets.reshape(-1)
     if (x2.stride(1) != 1 and x2.shape[1] > 1) or (x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]):
         x2 = x2.contiguous()                       # columns apart, or rows that share memory (a broadcast x)
-    loss = AG.vocab_cross_entropy(x2, weight, bias, t.contiguous(), ignore_index, reduction)
+    t = t.contiguous()
+    if x2.shape[0] == 0 or (torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad or
+                                                          (bias is not None and bias.requires_grad))):
+        from . import autograd as AG
+        loss = AG.vocab_cross_entropy(x2, weight, bias, t, ignore_index, reduction)
+    else:
+        nll, loss, _ = ops.vocab_ce_forward(x2, weight, bias, t, ignore_index, want_loss=reduction != "none")
+        loss = nll if reduction == "none" else loss[0 if reduction == "mean" else 1]
     return loss.view(targets.shape) if reduction == "none" else loss

@@ -43,6 +43,8 @@ struct Plan {
     int64_t dx_rows;                             // most rows of partial sums
     int sw;                                      // contraction splits of dW
     bool wide_z, wide_dx, wide_dw;               // tiles of 256 x 256 for the logits, dx and dW
+    bool few_z;                                  // tiles of 128 x 128 for the logits
+    int z_words, z_rows;                         // the logits' tile
     size_t o_order, o_slot, o_tgt, o_lse, o_dlt, o_b2, o_x, o_w, saved;
     size_t o_part, o_amax, fwd;
     size_t o_rw, o_rest, o_g, o_dx, o_dw, o_db, bwd;
@@ -96,7 +98,11 @@ bool make_plan(const capdec_vocab_ce* a, Plan& p) {
     p.saved = at;
 
     at = 256;
-    p.o_part = take(at, (size_t)(p.Vp / 256) * p.Mp * 8);
+    p.wide_z = wide_pays((int64_t)(p.Mp / 256) * (p.Vp / 256), p.xs / 32);
+    p.few_z = !p.wide_z && (int64_t)(p.Mp / 128) * (p.Vp / 256) < 512;
+    p.z_words = p.few_z ? Mid::BI : p.wide_z ? Wide::BI : Big::BI;
+    p.z_rows = p.few_z ? Mid::BJ : p.wide_z ? Wide::BJ : Big::BJ;
+    p.o_part = take(at, (size_t)(p.Vp / p.z_words) * p.Mp * 8);
     p.o_amax = take(at, 2 * 512 * 4);
     p.fwd = at;
 
@@ -108,7 +114,6 @@ bool make_plan(const capdec_vocab_ce* a, Plan& p) {
     p.pieces = (p.Vp + p.piece - 1) / p.piece;
     const int kt = p.split ? 16 : 32;
     const int64_t row_tiles = p.Mp / 256, word_tiles = p.piece / 256;
-    p.wide_z = wide_pays(row_tiles * word_tiles, p.xs / 32);
     auto grad = [&](int64_t tiles, int n, int& split) {      // tiles of 256 along the first axis
         const int s2 = splits_for(tiles * ((p.Kp + 127) / 128), n, 512), s1 = splits_for(tiles * ((p.Kp + 255) / 256), n, 256);
         const bool wide = p.Kp % 256 == 0 && wide_pays(tiles * (p.Kp / 256) * s1, n / s1);
@@ -166,21 +171,38 @@ __device__ __forceinline__ int scale_exp(unsigned amax_bits) {
 __device__ __forceinline__ float pow2(int e) { return ldexpf(1.f, e); }
 
 // ---- rows with a counted target -------------------------------------------------------------------------------------
-// One workgroup: stable compaction, 4096 targets per round.
-__global__ __launch_bounds__(1024) void compact_kernel(const int64_t* __restrict__ targets, int M, int V, int64_t ignore,
-                                                       Head* __restrict__ head, int* __restrict__ order,
-                                                       int* __restrict__ slot, int* __restrict__ tgt) {
+__device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int dtype) {
+    if (dtype == CAPDEC_F32) return ((const float*)p)[i];
+    const short b = ((const short*)p)[i];
+    return dtype == CAPDEC_BF16 ? from_bits<BF16>(b) : from_bits<F16>(b);
+}
+
+constexpr int AMAX_BLOCKS = 256;
+struct ScanArgs {
+    const int64_t* targets;
+    int M, V, K;
+    int64_t ignore;
+    Head* head;
+    int *order, *slot, *tgt;
+    const float* x; int64_t ldx;          // split operands: also the largest finite magnitudes of x (counted rows) and W
+    const float* W; int64_t ldw;
+    int nparts, vec;
+    float* part;                          // [2][AMAX_BLOCKS]
+};
+
+// The first workgroup compacts the rows: stable, 4096 targets per round.
+__device__ void compact(const ScanArgs& a) {
     __shared__ int wsum[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int done = 0;
-    for (int base = 0; base < M; base += 4096) {
+    for (int base = 0; base < a.M; base += 4096) {
         int64_t t[4];
         int n = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int r = base + threadIdx.x * 4 + k;
-            t[k] = r < M ? targets[r] : ignore;
-            n += t[k] != ignore;
+            t[k] = r < a.M ? a.targets[r] : a.ignore;
+            n += t[k] != a.ignore;
         }
         int pre = n;
 #pragma unroll
@@ -200,73 +222,75 @@ __global__ __launch_bounds__(1024) void compact_kernel(const int64_t* __restrict
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int r = base + threadIdx.x * 4 + k;
-            if (r >= M) break;
-            if (t[k] != ignore) {
-                order[s] = r;
-                tgt[s] = (t[k] >= 0 && t[k] < V) ? (int)t[k] : -1;    // -1: outside the vocabulary, the row's loss is NaN
-                slot[r] = s++;
+            if (r >= a.M) break;
+            if (t[k] != a.ignore) {
+                a.order[s] = r;
+                a.tgt[s] = (t[k] >= 0 && t[k] < a.V) ? (int)t[k] : -1;    // -1: outside the vocabulary, the row's loss is NaN
+                a.slot[r] = s++;
             } else {
-                slot[r] = -1;
+                a.slot[r] = -1;
             }
         }
         done += all;
         __syncthreads();
     }
     if (threadIdx.x == 0) {
-        head->count = done;
-        head->amax_x = head->amax_w = 0;
+        a.head->count = done;
+        a.head->amax_x = a.head->amax_w = 0;
     }
 }
 
-__device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int dtype) {
-    if (dtype == CAPDEC_F32) return ((const float*)p)[i];
-    const short b = ((const short*)p)[i];
-    return dtype == CAPDEC_BF16 ? from_bits<BF16>(b) : from_bits<F16>(b);
-}
-
-// Largest finite magnitude of x (counted rows) and W, one partial per block; blockIdx.y picks the operand.  A wavefront
-// reads four rows at a time.
-constexpr int AMAX_BLOCKS = 512;
-__global__ __launch_bounds__(256) void amax_kernel(const float* __restrict__ x, int64_t ldx, const float* __restrict__ W,
-                                                   int64_t ldw, int V, int K, const Head* __restrict__ head,
-                                                   const int* __restrict__ order, int vec, float* __restrict__ part) {
-    const bool isw = blockIdx.y != 0;
-    const int rows = isw ? V : head->count;
+// The others take the maxima, one partial each: a wavefront reads four rows at a time.
+__device__ void partial_max(const ScanArgs& a, int block) {
+    const bool isw = block >= a.nparts;
+    const int rows = isw ? a.V : a.M, nw = a.nparts * 16;
     float m = 0.f;
-    const int wave = (blockIdx.x * 256 + threadIdx.x) >> 6, nw = gridDim.x * 4, lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     auto see = [&](float v) {
         v = fabsf(v);
         if (v < INFINITY) m = fmaxf(m, v);
     };
-    for (int r = wave; r < rows; r += 4 * nw) {
+    for (int r = (block - (isw ? a.nparts : 0)) * 16 + wave; r < rows; r += 4 * nw) {
         const float* row[4];
+        bool use[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int q = min(r + k * nw, rows - 1);             // the last row again past the end
-            row[k] = isw ? W + (int64_t)q * ldw : x + (int64_t)order[q] * ldx;
+            use[k] = isw || a.targets[q] != a.ignore;
+            row[k] = isw ? a.W + (int64_t)q * a.ldw : a.x + (int64_t)q * a.ldx;
         }
-        if (vec) {
-            for (int c = lane * 4; c < K; c += 256) {
-                f32x4 v[4];
+        if (a.vec) {
+            for (int c = lane * 4; c < a.K; c += 256) {
+                f32x4 v[4] = {};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const f32x4*>(row[k] + c);
+                for (int k = 0; k < 4; ++k)
+                    if (use[k]) v[k] = *reinterpret_cast<const f32x4*>(row[k] + c);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) see(v[k][e]);
             }
         } else {
-            for (int c = lane; c < K; c += 64) {
+            for (int c = lane; c < a.K; c += 64) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) see(row[k][c]);
+                for (int k = 0; k < 4; ++k)
+                    if (use[k]) see(row[k][c]);
             }
         }
     }
     m = wave_max(m);
-    __shared__ float wm[4];
-    if (lane == 0) wm[threadIdx.x >> 6] = m;
+    __shared__ float wm[16];
+    if (lane == 0) wm[wave] = m;
     __syncthreads();
-    if (threadIdx.x == 0) part[blockIdx.y * AMAX_BLOCKS + blockIdx.x] = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) m = fmaxf(m, wm[w]);
+        a.part[(isw ? AMAX_BLOCKS - a.nparts : 0) + block] = m;
+    }
+}
+
+__global__ __launch_bounds__(1024) void scan_kernel(ScanArgs a) {
+    if (blockIdx.x == 0) compact(a);
+    else partial_max(a, blockIdx.x - 1);
 }
 
 // Packed operands: rows of whole k-tiles, zero beyond the width; x by slot (zero rows up to the next multiple of 32
@@ -863,16 +887,15 @@ int capdec_vocab_ce_forward(const capdec_vocab_ce* a, void* saved, size_t saved_
     int* order = (int*)(sv + p.o_order);
     int* slot = (int*)(sv + p.o_slot);
     int* tgt = (int*)(sv + p.o_tgt);
-    compact_kernel<<<1, 1024, 0, s>>>(a->targets, a->M, a->V, a->ignore_index, head, order, slot, tgt);
     const int esz = p.split ? 4 : 2;
     const int vec = capdec_aligned16(a->x) && capdec_aligned16(a->W) && a->ldx * esz % 16 == 0 && a->ldw * esz % 16 == 0;
     PackArgs k{};
-    if (p.split) {
-        k.nparts = (int)blocks_for((int64_t)(p.V > p.M ? p.V : p.M), 4, AMAX_BLOCKS);
-        k.part = (const float*)((char*)workspace + p.o_amax);
-        amax_kernel<<<dim3(k.nparts, 2), 256, 0, s>>>((const float*)a->x, a->ldx, (const float*)a->W, a->ldw, p.V, p.K, head,
-                                                      order, vec && p.K % 4 == 0, (float*)((char*)workspace + p.o_amax));
-    }
+    ScanArgs sc{a->targets, p.M, p.V, p.K, a->ignore_index, head, order, slot, tgt, (const float*)a->x, a->ldx, (const float*)a->W,
+                a->ldw, 0, vec && p.K % 4 == 0, (float*)((char*)workspace + p.o_amax)};
+    if (p.split) sc.nparts = (int)blocks_for((int64_t)(p.V > p.M ? p.V : p.M), 16, AMAX_BLOCKS);
+    scan_kernel<<<1 + 2 * sc.nparts, 1024, 0, s>>>(sc);
+    k.nparts = sc.nparts;
+    k.part = sc.part;
     k.x = a->x; k.ldx = a->ldx; k.W = a->W; k.ldw = a->ldw; k.bias = a->bias;
     k.M = p.M; k.V = p.V; k.K = p.K; k.Kp = p.Kp; k.xs = p.xs; k.dtype = a->dtype; k.split = p.split; k.Vp = p.Vp;
     k.pack_w = p.pack_w; k.vec = vec;
@@ -888,10 +911,10 @@ int capdec_vocab_ce_forward(const capdec_vocab_ce* a, void* saved, size_t saved_
     g.X = View{k.px, (int64_t)p.xs, p.Mp, 0};
     g.b2 = k.b2; g.head = head; g.kt = p.xs / 32; g.Mp = p.Mp;
     g.part = (float2*)((char*)workspace + p.o_part);
-#define LSE(E, S) (p.wide_z ? launch_lse<Wide, E, S>(g, p.Vp, p.Mp, s) : launch_lse<Big, E, S>(g, p.Vp, p.Mp, s))
+#define LSE(E, S) (p.few_z ? launch_lse<Mid, E, S>(g, p.Vp, p.Mp, s) : p.wide_z ? launch_lse<Wide, E, S>(g, p.Vp, p.Mp, s) : launch_lse<Big, E, S>(g, p.Vp, p.Mp, s))
     CAPDEC_TRY(BY_TYPE(p, LSE));
 #undef LSE
-    nll_kernel<<<(p.M + 3) / 4, 256, 0, s>>>(g.part, p.Vp / 256, p.Mp, a->x, a->ldx, a->W, a->ldw, a->bias, a->dtype, p.M, p.K,
+    nll_kernel<<<(p.M + 3) / 4, 256, 0, s>>>(g.part, p.Vp / p.z_words, p.Mp, a->x, a->ldx, a->W, a->ldw, a->bias, a->dtype, p.M, p.K,
                                              slot, tgt, (float*)(sv + p.o_lse), (float*)(sv + p.o_dlt), nll);
     if (loss) loss_kernel<<<1, 1024, 0, s>>>(nll, p.M, head, loss);
     CAPDEC_LAUNCH_CHECK();
@@ -937,7 +960,7 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
         g.b2 = (const float*)(sv + p.o_b2); g.head = head; g.kt = p.xs / 32; g.Mp = p.Mp;
         g.lse = (const float*)(sv + p.o_lse); g.dlt = (const float*)(sv + p.o_dlt); g.rw = rw; g.tgt = (const int*)(sv + p.o_tgt);
         g.g = G; g.ldg = (int64_t)p.piece * pl; g.rest = rest; g.dbp = dbias ? (float*)(ws + p.o_db) : nullptr; g.v0 = v0; g.piece = p.piece;
-#define DL(E, S) (p.wide_z ? launch_dlogits<Wide, E, S>(g, words, p.Mp, s) : launch_dlogits<Big, E, S>(g, words, p.Mp, s))
+#define DL(E, S) (p.few_z ? launch_dlogits<Mid, E, S>(g, words, p.Mp, s) : p.wide_z ? launch_dlogits<Wide, E, S>(g, words, p.Mp, s) : launch_dlogits<Big, E, S>(g, words, p.Mp, s))
         CAPDEC_TRY(BY_TYPE(p, DL));
 #undef DL
         if (dx) {
@@ -975,7 +998,7 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
             const int64_t items = (slabs > 1 ? (int64_t)real * ((p.K + 3) / 4) : 0) + (dbias ? real : 0);
             dw_kernel<<<blocks_for(items, 256, 8192), 256, 0, s>>>((const float*)(ws + p.o_dw), (int64_t)p.piece * p.Kp, slabs,
                                                                    p.Kp, real, p.K, head, up, p.split, dW, lddw, a->dtype,
-                                                                   g.dbp, p.piece, p.wide_z ? Wide::BJ : Big::BJ, dbias, v0);
+                                                                   g.dbp, p.piece, p.z_rows, dbias, v0);
             CAPDEC_LAUNCH_CHECK();
         }
     }
