@@ -61,7 +61,7 @@ size_t take(size_t& at, size_t bytes) {
 int splits_for(int64_t tiles, int kt, int slots) {
     int best = 1;
     double least = 1e300;
-    for (int s = 1; s <= 16 && kt / s >= 8; ++s) {
+    for (int s = 1; s <= 128 && kt / s >= 8; s += s < 16 ? 1 : 16) {
         const double t = (double)((tiles * s + slots - 1) / slots) * ((kt + s - 1) / s + (s > 1 ? 22 : 6));
         if (t < least * 0.97) least = t, best = s;
     }
@@ -683,6 +683,7 @@ struct GradArgs {
     const int* tgt; const float* rest; int v0;     // dW of at most REST_ROWS rows
     float* part; int64_t ldp, plane; int add;      // dx: plane is of the live row tiles
     void* out; int64_t ldo; int dtype;
+    int vec;                       // 16-bit results: rows of whole aligned 16-byte pieces
 };
 __device__ __forceinline__ void store_as(void* p, int64_t i, float v, int dtype) {
     if (dtype == CAPDEC_F32) ((float*)p)[i] = v;
@@ -732,23 +733,53 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void grad_kernel(GradArgs a) {
         f = factor_of(a.up, a.head);
         if (SPLIT) f *= pow2(-scale_exp(a.head->amax_x));
     }
+    if (OUT == 1 && !SPLIT && a.vec) {
+        // 16-bit results go through LDS, 32 rows of the wavefront at a time: stores of 16 bytes a lane instead of 2
+        constexpr int COLS = 32 * C::TJ, LD = COLS + 8, CH = COLS / 8;
+        short* tile = lds + wave * 32 * LD;
+#pragma unroll
+        for (int ti = 0; ti < C::TI; ++ti) {
+#pragma unroll
+            for (int tj = 0; tj < C::TJ; ++tj)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) tile[acc_row(e, h) * LD + tj * 32 + (lane & 31)] = to_bits<ELT>(acc[ti][tj][e] * f);
+            __builtin_amdgcn_wave_barrier();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            const int j = j0 + wj * COLS + (lane % CH) * 8;
+#pragma unroll
+            for (int r = 0; r < 32; r += 64 / CH) {
+                const int i = i0 + (wi * C::TI + ti) * 32 + r + lane / CH;
+                const s16x8 v = *reinterpret_cast<const s16x8*>(tile + (r + lane / CH) * LD + (lane % CH) * 8);
+                if (i < nI && j < a.J) *reinterpret_cast<s16x8*>((short*)a.out + (int64_t)i * a.ldo + j) = v;
+            }
+            __builtin_amdgcn_wave_barrier();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+        return;
+    }
 #pragma unroll
     for (int tj = 0; tj < C::TJ; ++tj) {
         const int j = j0 + (wj * C::TJ + tj) * 32 + (lane & 31);
         if (j >= a.J) continue;
 #pragma unroll
-        for (int ti = 0; ti < C::TI; ++ti)
+        for (int ti = 0; ti < C::TI; ++ti) {
+            const int ib = i0 + (wi * C::TI + ti) * 32;
+            float* d = a.part + (int64_t)z * a.plane + j;
+            if (OUT == 0 && a.add) {
+                float old[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) old[e] = d[(int64_t)min(ib + acc_row(e, h), nI - 1) * a.ldp];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[ti][tj][e] += old[e];
+            }
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const int i = i0 + (wi * C::TI + ti) * 32 + acc_row(e, h);
+                const int i = ib + acc_row(e, h);
                 if (i >= nI) continue;
-                if (OUT == 0) {
-                    float* d = a.part + (int64_t)z * a.plane + (int64_t)i * a.ldp + j;
-                    *d = a.add ? *d + acc[ti][tj][e] : acc[ti][tj][e];
-                } else {
-                    store_as(a.out, (int64_t)i * a.ldo + j, acc[ti][tj][e] * f, a.dtype);
-                }
+                if (OUT == 0) d[(int64_t)i * a.ldp] = acc[ti][tj][e];
+                else store_as(a.out, (int64_t)i * a.ldo + j, acc[ti][tj][e] * f, a.dtype);
             }
+        }
     }
 }
 
@@ -768,6 +799,7 @@ __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part,
         const int s = slot[r];
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
         if (s >= 0) {
+#pragma unroll 16
             for (int k = 0; k < nsplit; ++k) v += *reinterpret_cast<const f32x4*>(part + k * plane + (int64_t)s * Kp + c);
             const int w = tgt[s];
             if (!split && w >= 0) {
@@ -803,6 +835,7 @@ __global__ __launch_bounds__(256) void dw_kernel(const float* __restrict__ part,
         }
         const int r = (int)(t / cpr), c = (int)(t - (int64_t)r * cpr) * 4;
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
         for (int k = 0; k < nsplit; ++k) v += *reinterpret_cast<const f32x4*>(part + k * plane + (int64_t)r * Kp + c);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -982,6 +1015,7 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
             if (p.sw == 1) {
                 d.I = real; d.J = p.K;
                 d.out = (char*)dW + (int64_t)v0 * lddw * (p.split ? 4 : 2); d.ldo = lddw; d.dtype = a->dtype;
+                d.vec = capdec_aligned16(dW) && lddw % 8 == 0 && p.K % 8 == 0;
 #define DW(E, S) (p.wide_dw ? launch_grad<Wide, E, true, S, 1>(d, words, p.Kp, 0, s) : launch_grad<Big, E, true, S, 1>(d, words, p.Kp, 0, s))
                 CAPDEC_TRY(BY_TYPE(p, DW));
 #undef DW

@@ -620,7 +620,7 @@ int capdec_satt_greedy_decode(const capdec_satt_model* m, const float* enc, cons
  * reference, which materialises [B,T,V] logits: transformer.py:137 + train.py:216,254-256).
  *   z = x W^T + bias;  nll[r] = log(sum_v exp z[r,v]) - z[r, targets[r]], 0 where targets[r] == ignore_index
  * x [M,K] and W [V,K] have unit column stride and row strides ldx, ldw (elements); x, W, bias and their gradients share
- * one type.  Rows whose target is ignore_index are not read at all.  A counted target outside [0, V) makes its loss and
+ * one type.  Rows of x whose target is ignore_index are not read.  A counted target outside [0, V) makes its loss and
  * the gradients it enters NaN.  M, V <= 2^24, M V <= 2^42, K <= 2^20.
  * `saved` (capdec_vocab_ce_saved_bytes) carries packed operands and row statistics from the forward call to the backward
  * call, which reads W again: neither W nor `saved` may change in between.  `workspace` is scratch of one call.  Both are

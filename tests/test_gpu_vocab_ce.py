@@ -217,6 +217,37 @@ def test_strides_and_alignment(dt):
     assert got.shape == (10, 13) and torch.equal(got.sum(), F.vocab_cross_entropy(x, W, b, t, reduction="none").view(10, 13).sum())
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("M,V,K,bias", [(1, 5000, 512, True), (7, 70001, 100, False), (100, 300, 33, True), (192, 1000, 64, True),
+                                         (193, 1000, 64, False), (700, 2000, 128, True)])
+def test_loss_alone(M, V, K, bias, dt):
+    """The loss where nothing asks for gradients."""
+    from capdec import functional as F
+    x, W, b, t = make(M, V, K, dt, seed=15, bias=bias, ignored=0.3)
+    t[0] = V - 1
+    (nll, *_), (tol, *_) = definition(x, W, b, t, torch.zeros(M, device="cuda"))
+    got = F.vocab_cross_entropy(x, W, b, t, reduction="none")
+    near(got, nll, torch.full_like(nll, tol), "loss")
+    n = int((t != 0).sum())
+    for red, want in (("sum", nll.sum()), ("mean", nll.sum() / n)):
+        got = F.vocab_cross_entropy(x, W, b, t, reduction=red)
+        near(got, want, (tol * n + 2.0 ** -22 * nll.sum()) / (n if red == "mean" else 1), red)
+        assert torch.equal(got, F.vocab_cross_entropy(x, W, b, t, reduction=red))
+    if M > 2:
+        y = x.clone()
+        y[t == 0] = float("nan")
+        assert torch.equal(F.vocab_cross_entropy(y, W, b, t, reduction="sum"), F.vocab_cross_entropy(x, W, b, t, reduction="sum"))
+        t[1] = V
+        assert math.isnan(F.vocab_cross_entropy(x, W, b, t).item())
+        t[:] = 0
+        assert math.isnan(F.vocab_cross_entropy(x, W, b, t).item()) and F.vocab_cross_entropy(x, W, b, t, reduction="sum").item() == 0
+    if bias:
+        b[:V // 2] = float("-inf")
+        t[:] = torch.randint(V // 2, V, (M,), device="cuda")
+        (nll, *_), (tol, *_) = definition(x, W, b, t, torch.zeros(M, device="cuda"), ignore=-1)
+        near(F.vocab_cross_entropy(x, W, b, t, ignore_index=-1, reduction="none"), nll, torch.full_like(nll, tol), "loss")
+
+
 def test_broadcast_inputs():
     """Rows of x that are one row: its gradient is the sum of theirs."""
     from capdec import functional as F
