@@ -539,7 +539,7 @@ int run_batch(const Batch& b, int nz, const Dims& d, const Iteration& n, int dty
     return 0;
 }
 
-// A bfloat16 result is rounded by 2^-9: its last two steps take one fp16 number per value, a third of the products.  Their
+// A bfloat16 result is rounded by up to 2^-8: its last two steps take one fp16 number per value, a third of the products.  Their
 // error, about 2^-12 a value and grown once by a, stays below that rounding (6.5e-4 against 1.7e-3 in norm for gradients
 // of a few strong directions over noise; 2.5e-3 where all but 16 of 512 directions are a thousandth of those).
 int exact_steps(int steps, int dtype) { return dtype == CAPDEC_BF16 ? (steps > 2 ? steps - 2 : 0) : steps; }

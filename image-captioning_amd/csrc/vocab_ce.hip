@@ -7,10 +7,12 @@
 // leaves (max, sum of exp) per row.  Backward: G is rebuilt for one piece of the vocabulary at a time from x, W and the
 // rows' log-sum-exp, and contracted with W and x while it is in the caches.  Four products of 2 M V K flops in all for
 // loss and gradients, bound by the matrix cores at large sizes and by reading W at few rows.
-// fp32 operands are split into two fp16 numbers (mma16.h); 16-bit operands are multiplied as they are.  Sums, softmax
+// fp32 operands are split into two fp16 numbers (mma16.h), but for batches of at most 64 rows, which have kernels of their
+// own that read W as it is; 16-bit operands are multiplied as they are.  Sums, softmax
 // statistics and the partial sums of the gradients are fp32.  G takes the operands' 16-bit type (scaled by 2^14, so
-// that probabilities down to 2^-28 stay normal in fp16): its rounding is that of the gradients themselves, and averages
-// out in sums over rows or words.
+// that probabilities down to 2^-28 stay normal in fp16).  That rounding averages out in sums over rows or words, except
+// at the targets, whose entries are near -g_r: what it takes off them is carried beside G and added to dx, and to dW up to
+// 64 rows, and db sums the unrounded values.  Against rounding of the results alone: dx and db 1.0, dW 1.0 - 1.3 times.
 // Every sum has a fixed order: results repeat bit for bit.
 #include "mma16.h"
 #include <math.h>
@@ -22,6 +24,8 @@ namespace {
 constexpr float L2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr int G_EXP = 14;                        // G is stored times 2^14
 constexpr size_t PIECE_BYTES = (size_t)512 << 20;
+constexpr int FEW = 64;
+constexpr int AMAX_BLOCKS = 256;
 
 // dx has as many row tiles as there are counted rows, which only the device knows: the number of parts for each possible
 // number of row tiles goes along (one part beyond 64 of them, 16384 rows, where there are tiles enough).
@@ -44,8 +48,11 @@ struct Plan {
     int sw;                                      // contraction splits of dW
     bool wide_z, wide_dx, wide_dw;               // tiles of 256 x 256 for the logits, dx and dW
     bool few_z;                                  // tiles of 128 x 128 for the logits
+    bool few;                                    // fp32 and at most 64 rows: kernels of their own
+    int few_rows;                                // rows of z and G there: 16, 32 or 64
+    int few_split, few_words;                    // parts of the dx contraction, and words of a part
     int z_words, z_rows;                         // the logits' tile
-    size_t o_order, o_slot, o_tgt, o_lse, o_dlt, o_b2, o_x, o_w, saved;
+    size_t o_order, o_slot, o_tgt, o_lse, o_dlt, o_b2, o_x, o_w, o_z, saved;
     size_t o_part, o_amax, fwd;
     size_t o_rw, o_rest, o_g, o_dx, o_dw, o_db, bwd;
 };
@@ -92,6 +99,27 @@ bool make_plan(const capdec_vocab_ce* a, Plan& p) {
     p.o_tgt = take(at, (size_t)p.Mp * 4);
     p.o_lse = take(at, (size_t)p.Mp * 4);
     p.o_dlt = take(at, (size_t)p.Mp * 4);
+    if (p.split && p.M <= FEW) {
+        p.few = true;
+        p.few_rows = p.M <= 16 ? 16 : p.M <= 32 ? 32 : 64;
+        p.o_x = take(at, (size_t)p.few_rows * p.Kp * 4);
+        p.o_z = take(at, (size_t)p.few_rows * p.Vp * 4);
+        p.saved = at;
+        at = 256;
+        p.o_part = take(at, (size_t)p.few_rows * (p.Vp / 32) * 8);
+        p.fwd = at;
+        // about 1024 workgroups for dx, each of them 64 columns by at least 128 words
+        const int cols = (p.Kp + 63) / 64;
+        int n = 1024 / cols < 1 ? 1 : 1024 / cols > 255 ? 255 : 1024 / cols;
+        p.few_words = ((p.Vp + n - 1) / n + 127) / 128 * 128;
+        p.few_split = (p.Vp + p.few_words - 1) / p.few_words;
+        at = 256;
+        p.o_rw = take(at, (size_t)p.Mp * 4);
+        p.o_g = take(at, (size_t)p.few_rows * p.Vp * 4);
+        p.o_dx = take(at, (size_t)p.few_split * p.few_rows * p.Kp * 4);
+        p.bwd = at;
+        return true;
+    }
     p.o_b2 = take(at, (size_t)p.Vp * 4);
     p.o_x = take(at, (size_t)p.Mp * p.xs * 2);
     p.o_w = p.pack_w ? take(at, (size_t)p.V * p.xs * 2) : 0;
@@ -103,7 +131,7 @@ bool make_plan(const capdec_vocab_ce* a, Plan& p) {
     p.z_words = p.few_z ? Mid::BI : p.wide_z ? Wide::BI : Big::BI;
     p.z_rows = p.few_z ? Mid::BJ : p.wide_z ? Wide::BJ : Big::BJ;
     p.o_part = take(at, (size_t)(p.Vp / p.z_words) * p.Mp * 8);
-    p.o_amax = take(at, 2 * 512 * 4);
+    p.o_amax = take(at, 2 * AMAX_BLOCKS * 4);
     p.fwd = at;
 
     const int es = p.split ? 4 : 2;
@@ -177,7 +205,6 @@ __device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int dtype
     return dtype == CAPDEC_BF16 ? from_bits<BF16>(b) : from_bits<F16>(b);
 }
 
-constexpr int AMAX_BLOCKS = 256;
 struct ScanArgs {
     const int64_t* targets;
     int M, V, K;
@@ -458,7 +485,7 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void lse_kernel(LogitArgs a) {
 
 // Per slot: the tiles' statistics joined, the target's logit (a dot product of the original operands), and the loss.
 // A wavefront per row of the batch; rows that are not counted get loss 0.
-__global__ __launch_bounds__(256) void nll_kernel(const float2* __restrict__ part, int ntiles, int Mp, const void* x,
+__global__ __launch_bounds__(256) void nll_kernel(const float2* __restrict__ part, int ntiles, int64_t ts, int64_t rs, const void* x,
                                                   int64_t ldx, const void* W, int64_t ldw, const void* bias, int dtype,
                                                   int M, int K, const int* __restrict__ slot, const int* __restrict__ tgt,
                                                   float* __restrict__ lse, float* __restrict__ dlt, float* __restrict__ nll) {
@@ -470,8 +497,9 @@ __global__ __launch_bounds__(256) void nll_kernel(const float2* __restrict__ par
         return;
     }
     float m = -INFINITY, sum = 0.f;
+#pragma unroll 4
     for (int t = lane; t < ntiles; t += 64) {
-        const float2 v = part[(int64_t)t * Mp + s];
+        const float2 v = part[t * ts + s * rs];
         const float mm = fmaxf(m, v.x), mz = mm == -INFINITY ? 0.f : mm;
         sum = sum * __builtin_amdgcn_exp2f(m - mz) + v.y * __builtin_amdgcn_exp2f(v.x - mz);
         m = mm;
@@ -785,14 +813,14 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void grad_kernel(GradArgs a) {
 
 // dx[r] = factor * (sum of the partial sums of r's slot + what rounding took off its target's entry of G times the target's
 // row of W); zero for rows that are not counted
-__global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part, Splits splits, int Kp, int M, int K,
+__global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part, Splits splits, int rows, int Kp, int M, int K,
                                                  const int* __restrict__ slot, const int* __restrict__ tgt,
                                                  const float* __restrict__ rest, const void* W, int64_t ldw,
                                                  const Head* __restrict__ head, Upstream up, int split, void* out,
                                                  int64_t ldo, int dtype) {
     const float f = factor_of(up, head) * (split ? pow2(-scale_exp(head->amax_w)) : 1.f);
     const int tiles = (head->count + 255) / 256, nsplit = splits_of(splits, tiles);
-    const int64_t plane = (int64_t)tiles * 256 * Kp;
+    const int64_t plane = (int64_t)(rows ? rows : tiles * 256) * Kp;
     const int cpr = (K + 3) / 4;
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < (int64_t)M * cpr; t += (int64_t)gridDim.x * 256) {
         const int r = (int)(t / cpr), c = (int)(t - (int64_t)r * cpr) * 4;
@@ -802,7 +830,7 @@ __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part,
 #pragma unroll 16
             for (int k = 0; k < nsplit; ++k) v += *reinterpret_cast<const f32x4*>(part + k * plane + (int64_t)s * Kp + c);
             const int w = tgt[s];
-            if (!split && w >= 0) {
+            if (rest && w >= 0) {
                 const float q = rest[s];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -819,8 +847,8 @@ __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part,
 
 // dW of one piece from its partial sums, and db from the row tiles' column sums
 __global__ __launch_bounds__(256) void dw_kernel(const float* __restrict__ part, int64_t plane, int nsplit, int Kp, int rows,
-                                                 int K, const Head* __restrict__ head, Upstream up, int split, void* dW, int64_t ldw, int dtype, const float* __restrict__ dbp,
-                                                 int piece, int row_tile, void* db, int v0) {
+                                                 int K, const Head* __restrict__ head, Upstream up, int split, void* dW,
+                                                 int64_t ldw, int dtype, const float* __restrict__ dbp, int piece, int row_tile, void* db, int v0) {
     const float fb = factor_of(up, head);
     const float f = fb * (split ? pow2(-scale_exp(head->amax_x)) : 1.f);
     const int cpr = (K + 3) / 4;
@@ -841,6 +869,296 @@ __global__ __launch_bounds__(256) void dw_kernel(const float* __restrict__ part,
         for (int e = 0; e < 4; ++e)
             if (c + e < K) store_as(dW, (int64_t)(v0 + r) * ldw + c + e, v[e] * f, dtype);
     }
+}
+
+// ---- fp32 batches of at most 64 rows ------------------------------------------------------------------------------------
+// There reading W and writing dW is nearly all of the work, and packing W would read it twice and write it once more.  So
+// W goes from memory into fp32 matrix instructions (16 x 16 x 4), which keep up with memory for so few rows, and the logits,
+// of which there are fewer than W has elements, are kept for the backward call instead of a packed W.  Slots in groups of
+// 16, R groups; lane (r, g) = (lane & 15, lane >> 4) holds row or column r and, of 16 terms of a sum, terms 4 g to 4 g + 3:
+// operands agree on the order of the terms, so that it may be any.
+// W of 131072 x 512 (54 us a pass at the rate of a large copy): one row takes 60 us for the loss and 230 for loss and gradients (few_lse 83,
+// 55 where W stays in the caches; few_dx 55, few_dw 51); 64 rows 154 and 476, where the split operands take 227 and 598 for
+// 65 rows.  From 32 rows on the matrix instructions count (64 rows: 55 us of each product) and the kernels are bound by the
+// two together; a split in registers, three 16-bit products, would be the next step.
+__device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+template <bool VEC>
+__device__ __forceinline__ f32x4 load4(const float* p) {
+    if (VEC) return *reinterpret_cast<const f32x4*>(p);
+    return f32x4{p[0], p[1], p[2], p[3]};
+}
+// the first n of 4 values, zeros behind them
+__device__ __forceinline__ f32x4 load_some(const float* p, int n) {
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = e < n ? p[e] : 0.f;
+    return v;
+}
+
+struct FewArgs {
+    const float* x; int64_t ldx;
+    const float* W; int64_t ldw;
+    const float* bias;
+    int M, V, K, Vp;
+    const Head* head;
+    const int* order;
+    int Kp;
+    float* xs;                 // [slot][Kp], a copy of x for the backward call, zero behind the width and the counted rows
+    float* z;                  // [slot][Vp], in units of log 2, -inf behind the vocabulary
+    float2* part;              // [slot][Vp / 32]
+};
+// A workgroup makes the logits of 32 words; its wavefronts share out the sum over the width.
+template <int R, bool VEC>
+__global__ __launch_bounds__(256) void few_lse_kernel(FewArgs a) {
+    const int count = a.head->count;
+    for (int k = blockIdx.x; k < 16 * R; k += gridDim.x)
+        for (int c = threadIdx.x; c < a.Kp; c += 256)
+            a.xs[(int64_t)k * a.Kp + c] = k < count && c < a.K ? a.x[(int64_t)a.order[k] * a.ldx + c] : 0.f;
+    if (count == 0) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int w0 = blockIdx.x * 32;
+    const float *wp[2], *xp[R];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) wp[t] = a.W + (int64_t)min(w0 + 16 * t + r, a.V - 1) * a.ldw + 4 * g;
+#pragma unroll
+    for (int i = 0; i < R; ++i) xp[i] = a.x + (int64_t)a.order[min(16 * i + r, count - 1)] * a.ldx + 4 * g;
+    f32x4 acc[2][R] = {};
+    auto multiply = [&](const auto& wv, const auto& xv, int u) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < R; ++i) acc[t][i] = mfma4(wv[t][u][e], xv[i][u][e], acc[t][i]);
+    };
+    constexpr int U = R == 4 ? 2 : 4, COLS = 16 * U;
+    const int full = a.K / COLS;
+    for (int q = wave; q < full; q += 4) {
+        f32x4 wv[2][U], xv[R][U];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int u = 0; u < U; ++u) wv[t][u] = load4<VEC>(wp[t] + q * COLS + 16 * u);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int u = 0; u < U; ++u) xv[i][u] = load4<VEC>(xp[i] + q * COLS + 16 * u);
+#pragma unroll
+        for (int u = 0; u < U; ++u) multiply(wv, xv, u);
+    }
+    if (full * COLS < a.K && wave == (full & 3)) {
+        f32x4 wv[2][U], xv[R][U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = full * COLS + 16 * u, n = a.K - c - 4 * g;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) wv[t][u] = load_some(wp[t] + c, n);
+#pragma unroll
+            for (int i = 0; i < R; ++i) xv[i][u] = load_some(xp[i] + c, n);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) multiply(wv, xv, u);
+    }
+    __shared__ f32x4 sum[4][2][R][64];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < R; ++i) sum[wave][t][i][lane] = acc[t][i];
+    __syncthreads();
+    if (wave >= R) return;
+    // wavefront i has slots 16 i to 16 i + 15: lane (r, g) words 4 g to 4 g + 3 of both groups for slot r
+    const int slot = 16 * wave + r;
+    float v[2][4], m = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        f32x4 d = sum[0][t][wave][lane];
+#pragma unroll
+        for (int k = 1; k < 4; ++k) d += sum[k][t][wave][lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int w = w0 + 16 * t + 4 * g + e;
+            const float b = a.bias ? a.bias[min(w, a.V - 1)] : 0.f;
+            v[t][e] = w < a.V ? fmaf(d[e], L2E, b * L2E) : -INFINITY;
+            m = fmaxf(m, v[t][e]);
+        }
+        *reinterpret_cast<f32x4*>(a.z + (int64_t)slot * a.Vp + w0 + 16 * t + 4 * g) = f32x4{v[t][0], v[t][1], v[t][2], v[t][3]};
+    }
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    const float m0 = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(v[t][e] - m0);
+    s += __shfl_xor(s, 16, 64);
+    s += __shfl_xor(s, 32, 64);
+    if (g == 0) a.part[(int64_t)slot * (a.Vp / 32) + blockIdx.x] = make_float2(m, s);
+}
+
+struct FewGrad {
+    const float* xs;           // [slot][Kp]
+    const float* W; int64_t ldw;
+    int M, V, K, Kp, Vp;
+    const Head* head;
+    const int* tgt;
+    const float *z, *lse, *dlt, *rw;
+    Upstream up;
+    float* G;                  // [slot][Vp], zero behind the counted rows and behind the vocabulary
+    int rows;                  // slots of z and G
+    int words;                 // of a part of the dx contraction, a multiple of 128
+    float* part;               // [part][slot][Kp]
+    float* dW; int64_t lddw;
+    float* db;
+};
+// G from the logits, and the bias gradient.  A thread has four words, a wavefront every fourth slot.
+__global__ __launch_bounds__(256) void few_g_kernel(FewGrad a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int w = (blockIdx.x * 64 + lane) * 4;               // Vp is a multiple of 256
+    const int count = a.head->count;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = wave; s < a.rows; s += 4) {
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (s < count) {
+            const float l2 = a.lse[s], f = a.rw ? a.rw[s] : pow2(G_EXP);
+            const int t = a.tgt[s] - w;
+            const f32x4 z = *reinterpret_cast<const f32x4*>(a.z + (int64_t)s * a.Vp + w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (t == e && a.tgt[s] >= 0 ? expm1f(a.dlt[s]) : __builtin_amdgcn_exp2f(z[e] - l2)) * f;
+            sum += v;
+        }
+        *reinterpret_cast<f32x4*>(a.G + (int64_t)s * a.Vp + w) = v;
+    }
+    if (!a.db) return;
+    __shared__ f32x4 part[4][64];
+    part[wave][lane] = sum;
+    __syncthreads();
+    const float f = factor_of(a.up, a.head);
+    const float* p = reinterpret_cast<const float*>(part);
+    const int v = blockIdx.x * 256 + threadIdx.x;
+    if (v < a.V) a.db[v] = ((p[threadIdx.x] + p[256 + threadIdx.x]) + (p[512 + threadIdx.x] + p[768 + threadIdx.x])) * f;
+}
+
+// Partial sums of dx = G W: a workgroup has 64 columns and one part of the words, of which its wavefronts take 16 at a time
+// in turn.  A lane reads 4 columns of a word at once, which go to four products: column 4 r + c is column r of product c.
+template <int R, bool VEC>
+__global__ __launch_bounds__(256) void few_dx_kernel(FewGrad a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int c0 = blockIdx.x * 64 + 4 * r, first = blockIdx.y * a.words, last = min(a.Vp, first + a.words);
+    f32x4 acc[R][4] = {};
+    f32x4 b[2][4], v[2][R];                                   // the next words are on their way during a product
+    auto load = [&](int k, int w) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float* row = a.W + (int64_t)min(w + 4 * g + e, a.V - 1) * a.ldw;      // G is zero behind the vocabulary
+            if (VEC) b[k][e] = *reinterpret_cast<const f32x4*>(row + min(c0, a.K - 4));
+            else
+#pragma unroll
+                for (int c = 0; c < 4; ++c) b[k][e][c] = row[min(c0 + c, a.K - 1)];
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) v[k][i] = *reinterpret_cast<const f32x4*>(a.G + (int64_t)(16 * i + r) * a.Vp + w + 4 * g);
+    };
+    auto multiply = [&](int k) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int i = 0; i < R; ++i) acc[i][c] = mfma4(v[k][i][e], b[k][e][c], acc[i][c]);
+    };
+    load(0, first + 16 * wave);                               // a part has a multiple of 128 words
+    for (int w = first + 16 * wave; w < last; w += 128) {
+        load(1, w + 64);
+        multiply(0);
+        if (w + 128 < last) load(0, w + 128);
+        multiply(1);
+    }
+    __shared__ f32x4 sum[4][R][4][64];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[wave][i][c][lane] = acc[i][c];
+    __syncthreads();
+    if (wave >= R || c0 >= a.Kp) return;
+    f32x4 d[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        d[c] = sum[0][wave][c][lane];
+#pragma unroll
+        for (int k = 1; k < 4; ++k) d[c] += sum[k][wave][c][lane];
+    }
+    float* out = a.part + ((int64_t)blockIdx.y * a.rows + 16 * wave + 4 * g) * a.Kp + c0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) *reinterpret_cast<f32x4*>(out + (int64_t)e * a.Kp) = f32x4{d[0][e], d[1][e], d[2][e], d[3][e]};
+}
+
+// dW = G^T x: a wavefront has T groups of 16 words and goes through the columns, 64 at a time.
+template <int R, int T, bool VEC>
+__global__ __launch_bounds__(256) void few_dw_kernel(FewGrad a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int w0 = (blockIdx.x * 4 + wave) * 16 * T;          // Vp is a multiple of 256
+    const float f = factor_of(a.up, a.head);
+    float v[T][4 * R];
+#pragma unroll
+    for (int st = 0; st < 4 * R; ++st)
+#pragma unroll
+        for (int t = 0; t < T; ++t) v[t][st] = a.G[(int64_t)(4 * st + g) * a.Vp + w0 + 16 * t + r];
+    for (int c0 = blockIdx.y * 64 + 4 * r; c0 - 4 * r < a.K; c0 += 64 * gridDim.y) {
+        f32x4 acc[T][4] = {};
+#pragma unroll
+        for (int st = 0; st < 4 * R; ++st) {
+            const f32x4 b = *reinterpret_cast<const f32x4*>(a.xs + (int64_t)(4 * st + g) * a.Kp + min(c0, a.Kp - 4));
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int t = 0; t < T; ++t) acc[t][c] = mfma4(v[t][st], b[c], acc[t][c]);
+        }
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int w = w0 + 16 * t + 4 * g + e;
+                if (w >= a.V) continue;
+                float* out = a.dW + (int64_t)w * a.lddw + c0;
+                if (VEC) {
+                    if (c0 < a.K) *reinterpret_cast<f32x4*>(out) = f32x4{acc[t][0][e] * f, acc[t][1][e] * f, acc[t][2][e] * f, acc[t][3][e] * f};
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (c0 + c < a.K) out[c] = acc[t][c][e] * f;
+                }
+            }
+    }
+}
+
+template <int R>
+int few_backward(const FewGrad& a, int split, const int* slot, void* dx, int64_t lddx, hipStream_t s) {
+    few_g_kernel<<<a.Vp / 256, 256, 0, s>>>(a);
+    const bool even = a.K % 4 == 0;
+    if (dx) {
+        const dim3 grid((a.Kp + 63) / 64, split);
+        if (even && capdec_aligned16(a.W) && a.ldw % 4 == 0) few_dx_kernel<R, true><<<grid, 256, 0, s>>>(a);
+        else few_dx_kernel<R, false><<<grid, 256, 0, s>>>(a);
+        Splits one;
+        one.s[0] = (unsigned char)split;
+        int64_t blocks = ((int64_t)a.M * ((a.K + 3) / 4) + 255) / 256;
+        dx_kernel<<<(unsigned)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>(a.part, one, a.rows, a.Kp, a.M, a.K, slot, a.tgt, nullptr,
+                                                                          a.W, a.ldw, a.head, a.up, 0, dx, lddx, CAPDEC_F32);
+    }
+    if (a.dW) {
+        // at least 2048 wavefronts where the columns allow it
+        constexpr int T = 2;
+        const int blocks = a.Vp / (64 * T), cols = (a.K + 63) / 64;
+        const int y = blocks >= 512 ? 1 : 512 / blocks < cols ? 512 / blocks : cols;
+        const dim3 grid(blocks, y);
+        if (even && capdec_aligned16(a.dW) && a.lddw % 4 == 0) few_dw_kernel<R, T, true><<<grid, 256, 0, s>>>(a);
+        else few_dw_kernel<R, T, false><<<grid, 256, 0, s>>>(a);
+    }
+    CAPDEC_LAUNCH_CHECK();
+    return 0;
 }
 
 unsigned blocks_for(int64_t items, int64_t per, unsigned most) {
@@ -922,6 +1240,23 @@ int capdec_vocab_ce_forward(const capdec_vocab_ce* a, void* saved, size_t saved_
     int* tgt = (int*)(sv + p.o_tgt);
     const int esz = p.split ? 4 : 2;
     const int vec = capdec_aligned16(a->x) && capdec_aligned16(a->W) && a->ldx * esz % 16 == 0 && a->ldw * esz % 16 == 0;
+    if (p.few) {
+        ScanArgs sc{a->targets, p.M, p.V, p.K, a->ignore_index, head, order, slot, tgt, nullptr, 0, nullptr, 0, 0, 0, nullptr};
+        scan_kernel<<<1, 1024, 0, s>>>(sc);
+        float2* part = (float2*)((char*)workspace + p.o_part);
+        const FewArgs f{(const float*)a->x, a->ldx, (const float*)a->W, a->ldw, (const float*)a->bias, p.M, p.V, p.K, p.Vp, head,
+                        order, p.Kp, (float*)(sv + p.o_x), (float*)(sv + p.o_z), part};
+        const bool v4 = vec && p.K % 4 == 0;
+        const unsigned grid = p.Vp / 32;
+        if (p.few_rows == 16) v4 ? few_lse_kernel<1, true><<<grid, 256, 0, s>>>(f) : few_lse_kernel<1, false><<<grid, 256, 0, s>>>(f);
+        else if (p.few_rows == 32) v4 ? few_lse_kernel<2, true><<<grid, 256, 0, s>>>(f) : few_lse_kernel<2, false><<<grid, 256, 0, s>>>(f);
+        else v4 ? few_lse_kernel<4, true><<<grid, 256, 0, s>>>(f) : few_lse_kernel<4, false><<<grid, 256, 0, s>>>(f);
+        nll_kernel<<<(p.M + 3) / 4, 256, 0, s>>>(part, p.Vp / 32, 1, p.Vp / 32, a->x, a->ldx, a->W, a->ldw, a->bias, a->dtype, p.M,
+                                                 p.K, slot, tgt, (float*)(sv + p.o_lse), (float*)(sv + p.o_dlt), nll);
+        if (loss) loss_kernel<<<1, 1024, 0, s>>>(nll, p.M, head, loss);
+        CAPDEC_LAUNCH_CHECK();
+        return 0;
+    }
     PackArgs k{};
     ScanArgs sc{a->targets, p.M, p.V, p.K, a->ignore_index, head, order, slot, tgt, (const float*)a->x, a->ldx, (const float*)a->W,
                 a->ldw, 0, vec && p.K % 4 == 0, (float*)((char*)workspace + p.o_amax)};
@@ -944,11 +1279,14 @@ int capdec_vocab_ce_forward(const capdec_vocab_ce* a, void* saved, size_t saved_
     g.X = View{k.px, (int64_t)p.xs, p.Mp, 0};
     g.b2 = k.b2; g.head = head; g.kt = p.xs / 32; g.Mp = p.Mp;
     g.part = (float2*)((char*)workspace + p.o_part);
-#define LSE(E, S) (p.few_z ? launch_lse<Mid, E, S>(g, p.Vp, p.Mp, s) : p.wide_z ? launch_lse<Wide, E, S>(g, p.Vp, p.Mp, s) : launch_lse<Big, E, S>(g, p.Vp, p.Mp, s))
+#define LSE(E, S)                                                  \
+    (p.few_z    ? launch_lse<Mid, E, S>(g, p.Vp, p.Mp, s)          \
+     : p.wide_z ? launch_lse<Wide, E, S>(g, p.Vp, p.Mp, s)         \
+                : launch_lse<Big, E, S>(g, p.Vp, p.Mp, s))
     CAPDEC_TRY(BY_TYPE(p, LSE));
 #undef LSE
-    nll_kernel<<<(p.M + 3) / 4, 256, 0, s>>>(g.part, p.Vp / p.z_words, p.Mp, a->x, a->ldx, a->W, a->ldw, a->bias, a->dtype, p.M, p.K,
-                                             slot, tgt, (float*)(sv + p.o_lse), (float*)(sv + p.o_dlt), nll);
+    nll_kernel<<<(p.M + 3) / 4, 256, 0, s>>>(g.part, p.Vp / p.z_words, p.Mp, 1, a->x, a->ldx, a->W, a->ldw, a->bias, a->dtype,
+                                             p.M, p.K, slot, tgt, (float*)(sv + p.o_lse), (float*)(sv + p.o_dlt), nll);
     if (loss) loss_kernel<<<1, 1024, 0, s>>>(nll, p.M, head, loss);
     CAPDEC_LAUNCH_CHECK();
     return 0;
@@ -978,6 +1316,15 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
         weights_kernel<<<1, 1024, 0, s>>>(row_grad, head, order, p.Mp, rw, (BwdHead*)ws);
         CAPDEC_LAUNCH_CHECK();
     }
+    if (p.few) {
+        const FewGrad f{(const float*)(sv + p.o_x), (const float*)a->W, a->ldw, p.M, p.V, p.K, p.Kp, p.Vp, head,
+                        (const int*)(sv + p.o_tgt), (const float*)(sv + p.o_z), (const float*)(sv + p.o_lse),
+                        (const float*)(sv + p.o_dlt), rw, up, (float*)(ws + p.o_g), p.few_rows, p.few_words,
+                        (float*)(ws + p.o_dx), (float*)dW, lddw, (float*)dbias};
+        return p.few_rows == 16 ? few_backward<1>(f, p.few_split, slot, dx, lddx, s)
+             : p.few_rows == 32 ? few_backward<2>(f, p.few_split, slot, dx, lddx, s)
+                                : few_backward<4>(f, p.few_split, slot, dx, lddx, s);
+    }
     const short* px = (const short*)(sv + p.o_x);
     const short* W = p.pack_w ? (const short*)(sv + p.o_w) : (const short*)a->W;
     const int64_t ldw = p.pack_w ? p.xs : a->ldw;
@@ -993,7 +1340,10 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
         g.b2 = (const float*)(sv + p.o_b2); g.head = head; g.kt = p.xs / 32; g.Mp = p.Mp;
         g.lse = (const float*)(sv + p.o_lse); g.dlt = (const float*)(sv + p.o_dlt); g.rw = rw; g.tgt = (const int*)(sv + p.o_tgt);
         g.g = G; g.ldg = (int64_t)p.piece * pl; g.rest = rest; g.dbp = dbias ? (float*)(ws + p.o_db) : nullptr; g.v0 = v0; g.piece = p.piece;
-#define DL(E, S) (p.few_z ? launch_dlogits<Mid, E, S>(g, words, p.Mp, s) : p.wide_z ? launch_dlogits<Wide, E, S>(g, words, p.Mp, s) : launch_dlogits<Big, E, S>(g, words, p.Mp, s))
+#define DL(E, S)                                                   \
+    (p.few_z    ? launch_dlogits<Mid, E, S>(g, words, p.Mp, s)     \
+     : p.wide_z ? launch_dlogits<Wide, E, S>(g, words, p.Mp, s)    \
+                : launch_dlogits<Big, E, S>(g, words, p.Mp, s))
         CAPDEC_TRY(BY_TYPE(p, DL));
 #undef DL
         if (dx) {
@@ -1038,7 +1388,8 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
     }
     if (dx) {
         dx_kernel<<<blocks_for((int64_t)p.M * ((p.K + 3) / 4), 256, 8192), 256, 0, s>>>(
-            dxp, p.sx, p.Kp, p.M, p.K, slot, (const int*)(sv + p.o_tgt), rest, a->W, a->ldw, head, up, p.split, dx, lddx, a->dtype);
+            dxp, p.sx, 0, p.Kp, p.M, p.K, slot, (const int*)(sv + p.o_tgt), p.split ? nullptr : rest, a->W, a->ldw, head, up,
+            p.split, dx, lddx, a->dtype);
         CAPDEC_LAUNCH_CHECK();
     }
     return 0;

@@ -622,8 +622,8 @@ int capdec_satt_greedy_decode(const capdec_satt_model* m, const float* enc, cons
  * x [M,K] and W [V,K] have unit column stride and row strides ldx, ldw (elements); x, W, bias and their gradients share
  * one type.  Rows of x whose target is ignore_index are not read.  A counted target outside [0, V) makes its loss and
  * the gradients it enters NaN.  M, V <= 2^24, M V <= 2^42, K <= 2^20.
- * `saved` (capdec_vocab_ce_saved_bytes) carries packed operands and row statistics from the forward call to the backward
- * call, which reads W again: neither W nor `saved` may change in between.  `workspace` is scratch of one call.  Both are
+ * `saved` (capdec_vocab_ce_saved_bytes) carries packed operands (for up to 64 rows of fp32: x and the logits) and row
+ * statistics from the forward call to the backward call, which reads W again: neither W nor `saved` may change in between.  `workspace` is scratch of one call.  Both are
  * 16-byte aligned.  Sums run in fixed orders: results repeat bit for bit.
  * forward: nll [M] fp32; loss (nullable) [3] fp32 = (mean over the counted rows, NaN without any; sum; their number).
  * backward: the upstream gradient is row_grad [M] (fp32, d/d nll) or, where that is NULL, grad[0] (NULL: 1) for the sum of
@@ -655,9 +655,10 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a /*host*/, const void* save
  * Orthogonalised updates of weight matrices (no counterpart in the reference, whose optimizer is Adam, train.py:217).
  *   X = U / (|U|_F + eps);  steps times:  A = X X^T, X <- a X + (b A + c A^2) X      (coeffs = {a, b, c}, host)
  * which drives the singular values of U towards 1.  `count` matrices of one shape per call, rows x cols with unit column
- * stride, rows * cols <= 2^31, any of 16 bits or fp32; sums and intermediate values carry fp32's precision.  Coefficients
- * under which singular values in [0, 1] could grow beyond 64 within the steps are refused (CAPDEC_EINVAL), as are more
- * than 32 steps.  A zero matrix stays zero.  Sums run in fixed orders: results repeat bit for bit.
+ * stride, rows * cols <= 2^31, any of 16 bits or fp32.  Sums are fp32, intermediate values pairs of fp16 numbers (22 bits),
+ * in the last two steps towards a bfloat16 result single fp16 numbers.  Coefficients under which singular values in
+ * [0, 1] could grow beyond 64 within the steps are refused (CAPDEC_EINVAL), as are more than 32 steps.  A zero matrix stays
+ * zero.  Sums run in fixed orders: results repeat bit for bit.
  * capdec_orthogonalize: dst = the last X; dst may be src.
  * capdec_muon_step: g <- grad_scale g;  m <- momentum m + g;  U = nesterov ? g + momentum m : m;
  *   p <- p (1 - lr weight_decay) - lr update_scale X.   fp32; g itself is not written.  lr comes from st->lr (device) when st

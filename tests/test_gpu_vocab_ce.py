@@ -397,3 +397,97 @@ def test_offsets_past_32_bits():
         ref += G[:, i:i + 100000] @ w
         mag += G[:, i:i + 100000].abs() @ w.abs()
     near(dx, ref, (1 + 1 / 16) * u * (mag + ref.abs()), "dx")
+
+
+@pytest.mark.parametrize("M,V,K", [(1, 300, 512), (2, 1, 4), (16, 1000, 36), (17, 4097, 30), (32, 515, 65), (33, 2000, 200), (48, 30, 1),
+                                   (63, 6000, 515), (64, 777, 96), (64, 70000, 64)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_few_rows(M, V, K, reduction):
+    """Batches of at most 64 rows of fp32, in groups of 16 slots: counted rows below and at the ends of the groups."""
+    for ignored in (0.0, 0.4):
+        x, W, b, t = make(M, V, K, torch.float32, seed=21, ignored=ignored, ignore=-100)
+        if reduction == "mean" and bool((t == -100).all()):          # (one row, ignored: the mean over none)
+            assert run(x, W, b, t, "mean", None, -100)[0].isnan()
+            continue
+        check(x, W, b if M % 3 else None, t, reduction, ignore=-100)
+
+
+def test_few_rows_upstream_gradients_far_apart():
+    """Rows whose upstream gradient is 1e-12 of the largest keep their accuracy in dx: bound of the row alone."""
+    x, W, b, t = make(40, 900, 72, torch.float32, seed=22, ignored=0.0, ignore=-100)
+    w = torch.logspace(0, -12, 40, device="cuda")
+    _, (dx, *_) = run(x, W, b, t, "none", w, -100)
+    (_, want, *_), (_, tol, *_) = definition(x, W, b, t, w, -100)
+    floor = 2.0 ** -38 * W.double().abs().sum(0)              # of the largest gradient, which these rows need not allow for
+    near(dx, want, tol - floor, "dx")
+
+
+@pytest.mark.parametrize("M", [5, 24, 64])
+def test_few_rows_layouts(M):
+    """Rows of x, W and the gradients at any stride and offset; what lies beside and behind them stays; a second backward."""
+    from capdec import ops
+    V, K = 530, 100
+    x, W, b, t = make(M, V, K, torch.float32, seed=23, ignored=0.3)
+    t[M - 1] = V - 1
+    one = torch.ones((), device="cuda")
+    want = None
+    for off in (0, 1, 4):
+        xs, ws, gx, gw = (torch.full((r + 2, K + 30 + off), 7.0, device="cuda") for r in (M, V, M, V))
+        xv, wv, dx, dW = (a[1:-1, off:off + K] for a in (xs, ws, gx, gw))
+        xv.copy_(x), wv.copy_(W)
+        nll, loss, state = ops.vocab_ce_forward(xv, wv, b, t)
+        xs.fill_(float("nan"))                                # the backward call has a copy of x, and reads W again
+        for _ in range(2):
+            dx.zero_(), dW.zero_()
+            db = torch.zeros_like(b)
+            ops.vocab_ce_backward(state, grad=one, mean=True, dx=dx, dW=dW, db=db)
+            got = [v.clone() for v in (nll, loss, dx, dW, db)]
+            want = got if want is None else want
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
+        for a, v in ((gx, dx), (gw, dW)):
+            v.fill_(7.0)
+            assert bool((a == 7.0).all())
+
+
+def test_few_rows_masked_and_out_of_range():
+    from capdec import functional as F
+    x, W, b, t = make(20, 700, 64, torch.float32, seed=24, ignored=0.0)
+    t[:] = 650
+    b[:600] = float("-inf")
+    loss, (dx, dW, db) = check(x, W, b, t, "sum", ignore=-100)
+    assert bool((dW[:600] == 0).all()) and bool((db[:600] == 0).all())
+    t[3:] = -100
+    y = x.clone()
+    y[3:] = float("nan")                                      # rows that are not counted are not read
+    _, grads = run(y, W, b, t, "mean", None, -100)
+    assert bool(grads[0][:3].isfinite().all()) and bool((grads[0][3:] == 0).all()) and bool(grads[1].isfinite().all())
+    t[:] = -100
+    _, grads = run(y, W, b, t, "sum", None, -100)
+    assert all(bool((g == 0).all()) for g in grads)
+    t[1] = 700
+    assert math.isnan(F.vocab_cross_entropy(x, W, b, t, ignore_index=-100).item())
+
+
+def test_few_rows_captured():
+    """Loss and gradients in a graph, replayed with other values between eager calls."""
+    from capdec import ops
+    x, W, b, t = make(30, 3000, 128, torch.float32, seed=25)
+    dx, dW, db = torch.empty_like(x), torch.empty_like(W), torch.empty_like(b)
+
+    def step():
+        nll, loss, state = ops.vocab_ce_forward(x, W, b, t)
+        ops.vocab_ce_backward(state, grad=None, mean=True, dx=dx, dW=dW, db=db)
+        return loss
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = step()
+    for k in range(4):
+        x.copy_(torch.randn_like(x) * (k + 1))
+        t.copy_(torch.randint(0, 3000, t.shape, device="cuda"))
+        graph.replay()
+        got = [v.clone() for v in (loss, dx, dW, db)]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, (want, dx, dW, db)))
