@@ -166,6 +166,45 @@ int main() {
     capdec_satt_model sm{};
     EXPECT(capdec_satt_decode_workspace_bytes(&sm, 4, 8), 0);
 
+    // vocabulary cross entropy: null operands, an unknown type, short row strides, both kinds of upstream gradient, small buffers
+    capdec_vocab_ce ce{};
+    EXPECT(capdec_vocab_ce_saved_bytes(nullptr), 0);
+    EXPECT(capdec_vocab_ce_saved_bytes(&ce), 0);
+    EXPECT(capdec_vocab_ce_forward(&ce, a, 1 << 20, a, 1 << 20, a, nullptr, nullptr), CAPDEC_EINVAL);
+    ce.x = a; ce.W = a; ce.targets = al; ce.M = 8; ce.V = 100; ce.K = 16; ce.ldx = 16; ce.ldw = 16;
+    for (int dtype = 0; dtype < 3; ++dtype) {
+        ce.dtype = dtype;
+        const size_t n = capdec_vocab_ce_saved_bytes(&ce), f = capdec_vocab_ce_forward_workspace_bytes(&ce),
+                     b = capdec_vocab_ce_backward_workspace_bytes(&ce);
+        EXPECT(n > 0 && f > 0 && b > 0, 1);
+        EXPECT(capdec_vocab_ce_forward(&ce, a, n - 1, a, f, a, nullptr, nullptr), CAPDEC_ENOMEM);
+        EXPECT(capdec_vocab_ce_forward(&ce, una, n, a, f, a, nullptr, nullptr), CAPDEC_EALIGN);
+        EXPECT(capdec_vocab_ce_backward(&ce, a, n, a, b - 1, nullptr, a, 1, a, 16, a, 16, nullptr, nullptr), CAPDEC_ENOMEM);
+        EXPECT(capdec_vocab_ce_backward(&ce, a, n, a, b, a, a, 1, a, 16, a, 16, nullptr, nullptr), CAPDEC_EINVAL);
+        EXPECT(capdec_vocab_ce_backward(&ce, a, n, a, b, a, nullptr, 1, a, 15, a, 16, nullptr, nullptr), CAPDEC_EINVAL);
+        EXPECT(capdec_vocab_ce_backward(&ce, a, n, a, b, a, nullptr, 1, a, 16, a, 16, a, nullptr), CAPDEC_EINVAL);   // no bias
+    }
+    ce.dtype = 3;
+    EXPECT(capdec_vocab_ce_saved_bytes(&ce), 0);
+    ce.dtype = 0; ce.ldw = 15;
+    EXPECT(capdec_vocab_ce_forward(&ce, a, 1 << 20, a, 1 << 20, a, nullptr, nullptr), CAPDEC_EINVAL);
+
+    // orthogonalised updates: null arrays, sizes, coefficients that grow without bound, small and misaligned workspaces
+    const float co[3] = {3.4445f, -4.7750f, 2.0315f}, wild[3] = {1e4f, 0.f, 0.f};
+    capdec_matrix mat{a, a, 16, 16};
+    const size_t nw = capdec_orthogonalize_workspace_bytes(1, 16, 16);
+    EXPECT(nw > 0, 1);
+    EXPECT(capdec_orthogonalize_workspace_bytes(0, 16, 16), 0);
+    EXPECT(capdec_orthogonalize(nullptr, 1, 16, 16, 0, 5, co, 1e-7f, a, nw, nullptr), CAPDEC_EINVAL);
+    EXPECT(capdec_orthogonalize(&mat, 1, 16, 16, 0, 5, nullptr, 1e-7f, a, nw, nullptr), CAPDEC_EINVAL);
+    EXPECT(capdec_orthogonalize(&mat, 1, 16, 16, 0, 5, wild, 1e-7f, a, nw, nullptr), CAPDEC_EINVAL);
+    EXPECT(capdec_orthogonalize(&mat, 1, 16, 16, 0, 33, co, 1e-7f, a, nw, nullptr), CAPDEC_EINVAL);
+    EXPECT(capdec_orthogonalize(&mat, 1, 16, 17, 0, 5, co, 1e-7f, a, (size_t)1 << 30, nullptr), CAPDEC_EINVAL);      // ld < cols
+    EXPECT(capdec_orthogonalize(&mat, 1, 16, 16, 0, 5, co, 1e-7f, a, nw - 1, nullptr), CAPDEC_ENOMEM);
+    EXPECT(capdec_orthogonalize(&mat, 1, 16, 16, 0, 5, co, 1e-7f, una, nw, nullptr), CAPDEC_EALIGN);
+    capdec_muon_param mp{a, a, nullptr, 16, 16, 16};
+    EXPECT(capdec_muon_step(&mp, 1, 16, 16, 0.1f, nullptr, 0.9f, 1, 0.f, 1.f, 1.f, 5, co, 1e-7f, a, nw, nullptr), CAPDEC_EINVAL);
+
     if (failures) {
         std::printf("%d validation checks failed\n", failures);
         return 1;
