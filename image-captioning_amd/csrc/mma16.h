@@ -10,8 +10,8 @@
 //
 // SPLIT operands carry 32-bit values as two fp16 numbers, v * s = hi + lo with s a power of two: 22 significant bits.
 // They are stored with twice the columns, [row][col / 16][hi, lo][16], which serves both orientations; a k-tile is then
-// 16 wide and feeds three products, lo*hi + hi*lo + hi*hi (lo*lo is below 2^-22 of the result).  Three MFMA passes
-// against sixteen for the fp32 matrix instruction at the same flops.
+// 16 wide and feeds three products, lo*hi + hi*lo + hi*hi (lo*lo is below 2^-22 of the result; tiles of 64 x 64, which wait
+// for memory, take it along).  Three MFMA passes against sixteen for the fp32 matrix instruction at the same flops.
 //
 // Bounds: rows of an N operand past its end are copies of its last row, columns of a T operand past its end are copies
 // of its last 8 (both feed only outputs that are not stored); k-tiles are whole, so operands are padded to 32 columns
@@ -69,7 +69,8 @@ __device__ __forceinline__ int acc_row(int e, int h) { return (e & 3) + 8 * (e >
 
 // 16 bytes per lane from `src` to 1 KiB of LDS at `dst` (wave-uniform), asynchronously.  Written as assembly because the
 // compiler, where it knows of such loads, waits for all of them before every transposing LDS read; it has no output
-// registers, and contract() waits for it by count.
+// registers, and contract() waits for it by count.  m0 has no other user: a kernel's tiles all come this way, or all through
+// the builtin.
 __device__ __forceinline__ void dma16(const short* src, short* dst) {
     const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) short*)dst);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src) : "memory");
