@@ -24,7 +24,8 @@ namespace {
 constexpr float L2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr int G_EXP = 14;                        // G is stored times 2^14
 constexpr size_t PIECE_BYTES = (size_t)512 << 20;
-constexpr int FEW = 64;
+constexpr int FEW = 64;                          // rows of fp32 up to which W is read as it is
+constexpr int FEW_WAVES = 1024;                  // from so many words / 32 on, no sum is shared by wavefronts
 constexpr int AMAX_BLOCKS = 256;
 
 // dx has as many row tiles as there are counted rows, which only the device knows: the number of parts for each possible
@@ -877,10 +878,10 @@ __global__ __launch_bounds__(256) void dw_kernel(const float* __restrict__ part,
 // of which there are fewer than W has elements, are kept for the backward call instead of a packed W.  Slots in groups of
 // 16, R groups; lane (r, g) = (lane & 15, lane >> 4) holds row or column r and, of 16 terms of a sum, terms 4 g to 4 g + 3:
 // operands agree on the order of the terms, so that it may be any.
-// W of 131072 x 512 (54 us a pass at the rate of a large copy): one row takes 60 us for the loss and 230 for loss and gradients (few_lse 83,
-// 55 where W stays in the caches; few_dx 55, few_dw 51); 64 rows 154 and 476, where the split operands take 227 and 598 for
-// 65 rows.  From 32 rows on the matrix instructions count (64 rows: 55 us of each product) and the kernels are bound by the
-// two together; a split in registers, three 16-bit products, would be the next step.
+// W of 131072 x 512 (54 us a pass at the rate of a large copy): one row takes 60 us for the loss and 230 for loss and
+// gradients (few_lse 86, 55 where W stays in the caches; few_dx 55, few_dw 51); 64 rows 149 and 470, where the split operands
+// take 227 and 600 for 65 rows.  From 32 rows on the matrix instructions count (64 rows: 55 us of each product) and the
+// kernels are bound by the two together.
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
 template <bool VEC>
@@ -908,8 +909,10 @@ struct FewArgs {
     float* z;                  // [slot][Vp], in units of log 2, -inf behind the vocabulary
     float2* part;              // [slot][Vp / 32]
 };
-// A workgroup makes the logits of 32 words; its wavefronts share out the sum over the width.
-template <int R, bool VEC>
+// A wavefront makes the logits of 32 words, the four of a workgroup reading the same columns of x at about the same time; or,
+// where that would leave CUs idle, a workgroup has 32 words and its wavefronts share out the sum over the width (SHARE; taken
+// throughout, 64 x 50000 x 1024 is 125 instead of 110 us, 64 x 131072 x 512 154 instead of 149, one row the same).
+template <int R, bool SHARE, bool VEC>
 __global__ __launch_bounds__(256) void few_lse_kernel(FewArgs a) {
     const int count = a.head->count;
     for (int k = blockIdx.x; k < 16 * R; k += gridDim.x)
@@ -917,7 +920,9 @@ __global__ __launch_bounds__(256) void few_lse_kernel(FewArgs a) {
             a.xs[(int64_t)k * a.Kp + c] = k < count && c < a.K ? a.x[(int64_t)a.order[k] * a.ldx + c] : 0.f;
     if (count == 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int w0 = blockIdx.x * 32;
+    const int tile = SHARE ? blockIdx.x : blockIdx.x * 4 + wave, w0 = tile * 32;
+    const int q0 = SHARE ? wave : 0;
+    constexpr int QS = SHARE ? 4 : 1;
     const float *wp[2], *xp[R];
 #pragma unroll
     for (int t = 0; t < 2; ++t) wp[t] = a.W + (int64_t)min(w0 + 16 * t + r, a.V - 1) * a.ldw + 4 * g;
@@ -934,7 +939,7 @@ __global__ __launch_bounds__(256) void few_lse_kernel(FewArgs a) {
     };
     constexpr int U = R == 4 ? 2 : 4, COLS = 16 * U;
     const int full = a.K / COLS;
-    for (int q = wave; q < full; q += 4) {
+    for (int q = q0; q < full; q += QS) {
         f32x4 wv[2][U], xv[R][U];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -947,7 +952,7 @@ __global__ __launch_bounds__(256) void few_lse_kernel(FewArgs a) {
 #pragma unroll
         for (int u = 0; u < U; ++u) multiply(wv, xv, u);
     }
-    if (full * COLS < a.K && wave == (full & 3)) {
+    if (full * COLS < a.K && (!SHARE || wave == (full & 3))) {
         f32x4 wv[2][U], xv[R][U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -960,41 +965,61 @@ __global__ __launch_bounds__(256) void few_lse_kernel(FewArgs a) {
 #pragma unroll
         for (int u = 0; u < U; ++u) multiply(wv, xv, u);
     }
-    __shared__ f32x4 sum[4][2][R][64];
+    // lane (r, g) has words 4 g to 4 g + 3 of both groups for slot r of row group i
+    auto finish = [&](int i, const f32x4 (&d)[2]) {
+        const int slot = 16 * i + r;
+        float v[2][4], m = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int w = w0 + 16 * t + 4 * g + e;
+                const float b = a.bias ? a.bias[min(w, a.V - 1)] : 0.f;
+                v[t][e] = w < a.V ? fmaf(d[t][e], L2E, b * L2E) : -INFINITY;
+                m = fmaxf(m, v[t][e]);
+            }
+            *reinterpret_cast<f32x4*>(a.z + (int64_t)slot * a.Vp + w0 + 16 * t + 4 * g) = f32x4{v[t][0], v[t][1], v[t][2], v[t][3]};
+        }
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        const float m0 = m == -INFINITY ? 0.f : m;
+        float s = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(v[t][e] - m0);
+        s += __shfl_xor(s, 16, 64);
+        s += __shfl_xor(s, 32, 64);
+        if (g == 0) a.part[(int64_t)slot * (a.Vp / 32) + tile] = make_float2(m, s);
+    };
+    if (!SHARE) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) finish(i, {acc[0][i], acc[1][i]});
+        return;
+    }
+    __shared__ f32x4 sum[SHARE ? 4 : 1][2][R][64];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < R; ++i) sum[wave][t][i][lane] = acc[t][i];
     __syncthreads();
     if (wave >= R) return;
-    // wavefront i has slots 16 i to 16 i + 15: lane (r, g) words 4 g to 4 g + 3 of both groups for slot r
-    const int slot = 16 * wave + r;
-    float v[2][4], m = -INFINITY;
+    f32x4 d[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        f32x4 d = sum[0][t][wave][lane];
+        d[t] = sum[0][t][wave][lane];
 #pragma unroll
-        for (int k = 1; k < 4; ++k) d += sum[k][t][wave][lane];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int w = w0 + 16 * t + 4 * g + e;
-            const float b = a.bias ? a.bias[min(w, a.V - 1)] : 0.f;
-            v[t][e] = w < a.V ? fmaf(d[e], L2E, b * L2E) : -INFINITY;
-            m = fmaxf(m, v[t][e]);
-        }
-        *reinterpret_cast<f32x4*>(a.z + (int64_t)slot * a.Vp + w0 + 16 * t + 4 * g) = f32x4{v[t][0], v[t][1], v[t][2], v[t][3]};
+        for (int k = 1; k < 4; ++k) d[t] += sum[k][t][wave][lane];
     }
-    m = fmaxf(m, __shfl_xor(m, 16, 64));
-    m = fmaxf(m, __shfl_xor(m, 32, 64));
-    const float m0 = m == -INFINITY ? 0.f : m;
-    float s = 0.f;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(v[t][e] - m0);
-    s += __shfl_xor(s, 16, 64);
-    s += __shfl_xor(s, 32, 64);
-    if (g == 0) a.part[(int64_t)slot * (a.Vp / 32) + blockIdx.x] = make_float2(m, s);
+    finish(wave, d);
+}
+
+template <int R>
+void launch_few_lse(const FewArgs& a, bool vec, hipStream_t s) {
+    const bool share = a.Vp / 32 < FEW_WAVES;
+    const unsigned grid = share ? a.Vp / 32 : a.Vp / 128;
+    if (share) vec ? few_lse_kernel<R, true, true><<<grid, 256, 0, s>>>(a) : few_lse_kernel<R, true, false><<<grid, 256, 0, s>>>(a);
+    else vec ? few_lse_kernel<R, false, true><<<grid, 256, 0, s>>>(a) : few_lse_kernel<R, false, false><<<grid, 256, 0, s>>>(a);
 }
 
 struct FewGrad {
@@ -1247,10 +1272,9 @@ int capdec_vocab_ce_forward(const capdec_vocab_ce* a, void* saved, size_t saved_
         const FewArgs f{(const float*)a->x, a->ldx, (const float*)a->W, a->ldw, (const float*)a->bias, p.M, p.V, p.K, p.Vp, head,
                         order, p.Kp, (float*)(sv + p.o_x), (float*)(sv + p.o_z), part};
         const bool v4 = vec && p.K % 4 == 0;
-        const unsigned grid = p.Vp / 32;
-        if (p.few_rows == 16) v4 ? few_lse_kernel<1, true><<<grid, 256, 0, s>>>(f) : few_lse_kernel<1, false><<<grid, 256, 0, s>>>(f);
-        else if (p.few_rows == 32) v4 ? few_lse_kernel<2, true><<<grid, 256, 0, s>>>(f) : few_lse_kernel<2, false><<<grid, 256, 0, s>>>(f);
-        else v4 ? few_lse_kernel<4, true><<<grid, 256, 0, s>>>(f) : few_lse_kernel<4, false><<<grid, 256, 0, s>>>(f);
+        if (p.few_rows == 16) launch_few_lse<1>(f, v4, s);
+        else if (p.few_rows == 32) launch_few_lse<2>(f, v4, s);
+        else launch_few_lse<4>(f, v4, s);
         nll_kernel<<<(p.M + 3) / 4, 256, 0, s>>>(part, p.Vp / 32, 1, p.Vp / 32, a->x, a->ldx, a->W, a->ldw, a->bias, a->dtype, p.M,
                                                  p.K, slot, tgt, (float*)(sv + p.o_lse), (float*)(sv + p.o_dlt), nll);
         if (loss) loss_kernel<<<1, 1024, 0, s>>>(nll, p.M, head, loss);

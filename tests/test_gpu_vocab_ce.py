@@ -400,7 +400,7 @@ def test_offsets_past_32_bits():
 
 
 @pytest.mark.parametrize("M,V,K", [(1, 300, 512), (2, 1, 4), (16, 1000, 36), (17, 4097, 30), (32, 515, 65), (33, 2000, 200), (48, 30, 1),
-                                   (63, 6000, 515), (64, 777, 96), (64, 70000, 64)])
+                                   (63, 6000, 515), (64, 777, 96), (64, 70000, 64), (20, 40000, 52)])
 @pytest.mark.parametrize("reduction", ["mean", "none"])
 def test_few_rows(M, V, K, reduction):
     """Batches of at most 64 rows of fp32, in groups of 16 slots: counted rows below and at the ends of the groups."""
