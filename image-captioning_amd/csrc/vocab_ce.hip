@@ -421,6 +421,7 @@ struct LogitArgs {
     int kt, Mp;
     Map map;
     float2* part;                                // forward: [tile][slot]
+    float* zt;                                   // forward: [slot] the target's logit, from the tile that has its word
     // dlogits
     const float *lse, *dlt, *rw;
     const int* tgt;
@@ -443,9 +444,15 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void lse_kernel(LogitArgs a) {
     const int count = a.head->count;
     const int i0 = ti_ * C::BI, j0 = tj_ * C::BJ;
     if (j0 >= count) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave / C::WJ, wj = wave % C::WJ, h = lane >> 5;
+    int at[C::TJ];                                // the targets among the wavefront's words
+#pragma unroll
+    for (int tj = 0; tj < C::TJ; ++tj) {
+        const int slot = j0 + (wj * C::TJ + tj) * 32 + (lane & 31);
+        at[tj] = slot < count ? a.tgt[slot] - i0 - wi * C::TI * 32 : -1;
+    }
     f32x16 acc[C::TI][C::TJ];
     contract<C, ELT, false, false, SPLIT>(a.W, a.X, i0, j0, 0, a.kt, lds, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave / C::WJ, wj = wave % C::WJ, h = lane >> 5;
     const float c1 = logit_scale<SPLIT>(a.head);
     float2* red = reinterpret_cast<float2*>(lds);
 #pragma unroll
@@ -463,6 +470,15 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void lse_kernel(LogitArgs a) {
                     m = fmaxf(m, v);
                 }
             }
+        const int to = at[tj];
+        if (__any(to >= 0 && to < C::TI * 32)) {
+            float zt = 0.f;
+#pragma unroll
+            for (int ti = 0; ti < C::TI; ++ti)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) zt = to - 4 * h == ti * 32 + acc_row(e, 0) ? acc[ti][tj][e] : zt;
+            if (to >= 0 && to < C::TI * 32 && ((to >> 2) & 1) == h) a.zt[j0 + (wj * C::TJ + tj) * 32 + (lane & 31)] = zt;
+        }
         const float m0 = m == -INFINITY ? 0.f : m;          // a tile whose words are all masked by the bias
         float s = 0.f;
 #pragma unroll
@@ -484,48 +500,48 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void lse_kernel(LogitArgs a) {
     }
 }
 
-// Per slot: the tiles' statistics joined, the target's logit (a dot product of the original operands), and the loss.
-// A wavefront per row of the batch; rows that are not counted get loss 0.
-__global__ __launch_bounds__(256) void nll_kernel(const float2* __restrict__ part, int ntiles, int64_t ts, int64_t rs, const void* x,
-                                                  int64_t ldx, const void* W, int64_t ldw, const void* bias, int dtype,
-                                                  int M, int K, const int* __restrict__ slot, const int* __restrict__ tgt,
-                                                  float* __restrict__ lse, float* __restrict__ dlt, float* __restrict__ nll) {
-    const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (r >= M) return;
-    const int s = slot[r];
-    if (s < 0) {
-        if (lane == 0) nll[r] = 0.f;
-        return;
-    }
+// Per slot: the tiles' statistics joined, and the loss.  The target's logit is the very number that went into the sum, so
+// that a row which is sure of its target loses 0 and not the rounding of two sums (the logit as a dot product of its own:
+// +-4e-6 at a logit of 64).  dlt: the target's logit in, the log of its probability out.  Rows that are not counted get
+// loss 0.  A workgroup has 64 slots, whose statistics lie side by side, or (ROW) one, whose tiles do.
+template <bool ROW>
+__global__ __launch_bounds__(1024) void nll_kernel(const float2* __restrict__ part, int ntiles, int Mp, int M,
+                                                   const Head* __restrict__ head, const int* __restrict__ order,
+                                                   const int* __restrict__ slot, const int* __restrict__ tgt,
+                                                   float* __restrict__ lse, float* __restrict__ dlt, float* __restrict__ nll) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int s = ROW ? blockIdx.x : blockIdx.x * 64 + lane, count = head->count;
+    if (s < M && threadIdx.x < 64 && slot[s] < 0 && (!ROW || lane == 0)) nll[s] = 0.f;         // as a row
     float m = -INFINITY, sum = 0.f;
-#pragma unroll 4
-    for (int t = lane; t < ntiles; t += 64) {
-        const float2 v = part[t * ts + s * rs];
-        const float mm = fmaxf(m, v.x), mz = mm == -INFINITY ? 0.f : mm;
-        sum = sum * __builtin_amdgcn_exp2f(m - mz) + v.y * __builtin_amdgcn_exp2f(v.x - mz);
-        m = mm;
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float mo = __shfl_xor(m, o, 64), so = __shfl_xor(sum, o, 64);
+    auto join = [&](float mo, float so) {
         const float mm = fmaxf(m, mo), mz = mm == -INFINITY ? 0.f : mm;
         sum = sum * __builtin_amdgcn_exp2f(m - mz) + so * __builtin_amdgcn_exp2f(mo - mz);
         m = mm;
+    };
+    if (s < count) {
+#pragma unroll 4
+        for (int t = ROW ? threadIdx.x : wave; t < ntiles; t += ROW ? 1024 : 16) {
+            const float2 v = ROW ? part[(int64_t)s * ntiles + t] : part[(int64_t)t * Mp + s];
+            join(v.x, v.y);
+        }
     }
-    const int t = tgt[s];
-    float dot = 0.f;
-    if (t >= 0)
-        for (int c = lane; c < K; c += 64)
-            dot = fmaf(load_as_f32(x, (int64_t)r * ldx + c, dtype), load_as_f32(W, (int64_t)t * ldw + c, dtype), dot);
-    dot = wave_sum(dot);
-    if (lane == 0) {
-        const float l2 = t >= 0 ? m + __log2f(sum) : NAN;
-        const float zt = t < 0 ? NAN : dot + (bias ? load_as_f32(bias, t, dtype) : 0.f);
-        const float d = fmaf(-l2, LN2, zt);            // log of the target's probability
-        lse[s] = l2;
-        dlt[s] = d;
-        nll[r] = -d;
+    if (ROW) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const float mo = __shfl_xor(m, o, 64), so = __shfl_xor(sum, o, 64);
+            join(mo, so);
+        }
     }
+    __shared__ float2 st[16][64];
+    st[wave][lane] = make_float2(m, sum);
+    __syncthreads();
+    if (wave > 0 || s >= count || (ROW && lane > 0)) return;
+    for (int w = 1; w < 16; ++w) join(st[w][lane].x, st[w][lane].y);
+    const bool known = tgt[s] >= 0;
+    const float l = __log2f(sum), d = known ? ((dlt[s] - m) - l) * LN2 : NAN;       // log of the target's probability
+    lse[s] = known ? m + l : NAN;
+    dlt[s] = d;
+    nll[order[s]] = -d;
 }
 
 // loss[0] = mean over the counted rows, loss[1] = sum, loss[2] = number of counted rows; one workgroup, fixed order
@@ -878,9 +894,9 @@ __global__ __launch_bounds__(256) void dw_kernel(const float* __restrict__ part,
 // of which there are fewer than W has elements, are kept for the backward call instead of a packed W.  Slots in groups of
 // 16, R groups; lane (r, g) = (lane & 15, lane >> 4) holds row or column r and, of 16 terms of a sum, terms 4 g to 4 g + 3:
 // operands agree on the order of the terms, so that it may be any.
-// W of 131072 x 512 (54 us a pass at the rate of a large copy): one row takes 60 us for the loss and 230 for loss and
-// gradients (few_lse 86, 55 where W stays in the caches; few_dx 55, few_dw 51); 64 rows 149 and 470, where the split operands
-// take 227 and 600 for 65 rows.  From 32 rows on the matrix instructions count (64 rows: 55 us of each product) and the
+// W of 131072 x 512 (54 us a pass at the rate of a large copy): one row takes 56 us for the loss and 225 for loss and
+// gradients (few_lse 86, 55 where W stays in the caches; few_dx 55, few_dw 51); 64 rows 143 and 460, where the split operands
+// take 225 and 600 for 65 rows.  From 32 rows on the matrix instructions count (64 rows: 55 us of each product) and the
 // kernels are bound by the two together.
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
@@ -908,6 +924,8 @@ struct FewArgs {
     float* xs;                 // [slot][Kp], a copy of x for the backward call, zero behind the width and the counted rows
     float* z;                  // [slot][Vp], in units of log 2, -inf behind the vocabulary
     float2* part;              // [slot][Vp / 32]
+    const int* tgt;
+    float* zt;                 // [slot] the target's logit
 };
 // A wavefront makes the logits of 32 words, the four of a workgroup reading the same columns of x at about the same time; or,
 // where that would leave CUs idle, a workgroup has 32 words and its wavefronts share out the sum over the width (SHARE; taken
@@ -967,7 +985,7 @@ __global__ __launch_bounds__(256) void few_lse_kernel(FewArgs a) {
     }
     // lane (r, g) has words 4 g to 4 g + 3 of both groups for slot r of row group i
     auto finish = [&](int i, const f32x4 (&d)[2]) {
-        const int slot = 16 * i + r;
+        const int slot = 16 * i + r, t0 = slot < count ? a.tgt[slot] : -1;
         float v[2][4], m = -INFINITY;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -976,6 +994,7 @@ __global__ __launch_bounds__(256) void few_lse_kernel(FewArgs a) {
                 const int w = w0 + 16 * t + 4 * g + e;
                 const float b = a.bias ? a.bias[min(w, a.V - 1)] : 0.f;
                 v[t][e] = w < a.V ? fmaf(d[t][e], L2E, b * L2E) : -INFINITY;
+                if (w == t0) a.zt[slot] = v[t][e];
                 m = fmaxf(m, v[t][e]);
             }
             *reinterpret_cast<f32x4*>(a.z + (int64_t)slot * a.Vp + w0 + 16 * t + 4 * g) = f32x4{v[t][0], v[t][1], v[t][2], v[t][3]};
@@ -1270,13 +1289,13 @@ int capdec_vocab_ce_forward(const capdec_vocab_ce* a, void* saved, size_t saved_
         scan_kernel<<<1, 1024, 0, s>>>(sc);
         float2* part = (float2*)((char*)workspace + p.o_part);
         const FewArgs f{(const float*)a->x, a->ldx, (const float*)a->W, a->ldw, (const float*)a->bias, p.M, p.V, p.K, p.Vp, head,
-                        order, p.Kp, (float*)(sv + p.o_x), (float*)(sv + p.o_z), part};
+                        order, p.Kp, (float*)(sv + p.o_x), (float*)(sv + p.o_z), part, tgt, (float*)(sv + p.o_dlt)};
         const bool v4 = vec && p.K % 4 == 0;
         if (p.few_rows == 16) launch_few_lse<1>(f, v4, s);
         else if (p.few_rows == 32) launch_few_lse<2>(f, v4, s);
         else launch_few_lse<4>(f, v4, s);
-        nll_kernel<<<(p.M + 3) / 4, 256, 0, s>>>(part, p.Vp / 32, 1, p.Vp / 32, a->x, a->ldx, a->W, a->ldw, a->bias, a->dtype, p.M,
-                                                 p.K, slot, tgt, (float*)(sv + p.o_lse), (float*)(sv + p.o_dlt), nll);
+        nll_kernel<true><<<p.M, 1024, 0, s>>>(part, p.Vp / 32, 0, p.M, head, order, slot, tgt, (float*)(sv + p.o_lse),
+                                              (float*)(sv + p.o_dlt), nll);
         if (loss) loss_kernel<<<1, 1024, 0, s>>>(nll, p.M, head, loss);
         CAPDEC_LAUNCH_CHECK();
         return 0;
@@ -1303,14 +1322,15 @@ int capdec_vocab_ce_forward(const capdec_vocab_ce* a, void* saved, size_t saved_
     g.X = View{k.px, (int64_t)p.xs, p.Mp, 0};
     g.b2 = k.b2; g.head = head; g.kt = p.xs / 32; g.Mp = p.Mp;
     g.part = (float2*)((char*)workspace + p.o_part);
+    g.tgt = tgt; g.zt = (float*)(sv + p.o_dlt);
 #define LSE(E, S)                                                  \
     (p.few_z    ? launch_lse<Mid, E, S>(g, p.Vp, p.Mp, s)          \
      : p.wide_z ? launch_lse<Wide, E, S>(g, p.Vp, p.Mp, s)         \
                 : launch_lse<Big, E, S>(g, p.Vp, p.Mp, s))
     CAPDEC_TRY(BY_TYPE(p, LSE));
 #undef LSE
-    nll_kernel<<<(p.M + 3) / 4, 256, 0, s>>>(g.part, p.Vp / p.z_words, p.Mp, 1, a->x, a->ldx, a->W, a->ldw, a->bias, a->dtype,
-                                             p.M, p.K, slot, tgt, (float*)(sv + p.o_lse), (float*)(sv + p.o_dlt), nll);
+    nll_kernel<false><<<(p.M + 63) / 64, 1024, 0, s>>>(g.part, p.Vp / p.z_words, p.Mp, p.M, head, order, slot, tgt,
+                                                       (float*)(sv + p.o_lse), (float*)(sv + p.o_dlt), nll);
     if (loss) loss_kernel<<<1, 1024, 0, s>>>(nll, p.M, head, loss);
     CAPDEC_LAUNCH_CHECK();
     return 0;

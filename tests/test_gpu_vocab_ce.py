@@ -491,3 +491,29 @@ def test_few_rows_captured():
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(got, (want, dx, dW, db)))
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("M", [12, 150])
+def test_rows_sure_of_their_target(M, dt):
+    """Logits far above the others at the targets.  The target's logit and the sum have the same roundings, which cancel as
+    its probability goes to 1: the loss is off by 2 (1 - p) dz, by what up to 200 additions to a sum near 1 round off (half
+    a step of 2^-23 each, and no more than the 1 - p that is added) and by the roundings of the sum, its logarithm and one
+    product, 4 * 2^-23 - not by dz, here (K + 1) 2^-24 times some hundred.  No loss below -4 * 2^-23."""
+    K, V = 128, 700
+    g = torch.Generator("cuda").manual_seed(31)
+    W = torch.randn(V, K, device="cuda", generator=g).to(dt)
+    t = torch.randint(0, V, (M,), device="cuda", generator=g)
+    x = (W[t].float() * torch.linspace(0.02, 1.5, M, device="cuda")[:, None]).to(dt)
+    b = torch.randn(V, device="cuda", generator=g).to(dt)
+    w = torch.ones(M, device="cuda")
+    loss, _ = run(x, W, b, t, "none", w, -100)
+    z = x.double() @ W.double().T + b.double()
+    nll = torch.logsumexp(z, 1) - z.gather(1, t[:, None])[:, 0]
+    rest = -torch.expm1(-nll)                                 # 1 - p
+    S = x.double().abs() @ W.double().abs().T + b.double().abs()
+    dz = (3 * 2.0 ** -22 + (K + 1) * 2.0 ** -24) * S.max()
+    Z = z.abs().max() * 1.4427
+    tol = 2 * dz * rest + (3 * Z + 200) * 2.0 ** -23 * rest + rest.clamp(max=200 * 2.0 ** -24) + 4 * 2.0 ** -23
+    near(loss, nll, tol, "loss")
+    assert float(loss.min()) >= -4 * 2.0 ** -23 and float(nll.min()) < 1e-12 and float(nll.max()) > 1e-3
