@@ -1052,7 +1052,8 @@ def _vocab_ce_backward(st, row_grad, grad, mean, dx, lddx, dW, lddw, db):
 def vocab_ce_backward(state, grad=None, row_grad=None, mean=True, dx=None, dW=None, db=None, need=(True, True, True)):
     """Gradients of ``vocab_ce_forward``.  The upstream gradient is ``row_grad`` [M] fp32 (of nll) or ``grad``, a one-element
     fp32 tensor (of the mean, or with ``mean=False`` of the sum; None: 1).  Returns (dx, dW, db) in the operands' type,
-    written into the tensors given for them, or None where ``need`` says so."""
+    written into the tensors given for them (which share memory neither with W nor with one another; dx may be x), or None
+    where ``need`` says so."""
     if grad is not None and row_grad is not None:
         raise RuntimeError("capdec vocab_ce_backward: at most one of grad and row_grad")
     g = grad if grad is not None else row_grad
@@ -1071,6 +1072,7 @@ def vocab_ce_backward(state, grad=None, row_grad=None, mean=True, dx=None, dW=No
         outs.append(given)
     _same_device("vocab_ce_backward", [t for t in (g, state.saved, *outs) if t is not None])
     dx, dW, db = outs
+    _check_overlap("vocab_ce_backward", [t if t.dim() == 2 else t[None] for t in outs if t is not None], [state.W])
     _vocab_ce_backward(state, row_grad, grad, mean, dx, 0 if dx is None else _row_stride(dx, "dx"), dW,
                        0 if dW is None else _row_stride(dW, "dW"), db)
     return dx, dW, db

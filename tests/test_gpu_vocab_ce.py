@@ -517,3 +517,18 @@ def test_rows_sure_of_their_target(M, dt):
     tol = 2 * dz * rest + (3 * Z + 200) * 2.0 ** -23 * rest + rest.clamp(max=200 * 2.0 ** -24) + 4 * 2.0 ** -23
     near(loss, nll, tol, "loss")
     assert float(loss.min()) >= -4 * 2.0 ** -23 and float(nll.min()) < 1e-12 and float(nll.max()) > 1e-3
+
+
+def test_gradients_in_shared_memory():
+    """Gradients written over W or over one another are refused; dx in x's own memory is right."""
+    from capdec import ops
+    for M, dt in ((40, torch.float32), (100, torch.float32), (100, torch.bfloat16)):
+        x, W, b, t = make(M, 300, 64, dt, seed=41)
+        _, _, state = ops.vocab_ce_forward(x, W, b, t)
+        both = torch.empty(300 + M, 64, device="cuda", dtype=dt)
+        for bad in (dict(dW=W), dict(dx=W[:M]), dict(dx=both[:M], dW=both[M - 1:M + 299]), dict(db=W.view(-1)[64:364])):
+            with pytest.raises(RuntimeError, match="overlaps"):
+                ops.vocab_ce_backward(state, **bad)
+        want = ops.vocab_ce_backward(state)
+        got = ops.vocab_ce_backward(state, dx=x, dW=both[M:])
+        assert all(torch.equal(p, q) for p, q in zip(got, want)) and got[0] is x
