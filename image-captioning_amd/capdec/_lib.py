@@ -73,7 +73,7 @@ class SattModel(Structure):
 class VocabCE(Structure):
     _fields_ = [("x", c_void_p), ("W", c_void_p), ("bias", c_void_p), ("targets", c_void_p), ("ldx", c_int64),
                 ("ldw", c_int64), ("ignore_index", c_int64), ("M", c_int32), ("V", c_int32), ("K", c_int32),
-                ("dtype", c_int32)]
+                ("dtype", c_int32), ("loss_only", c_int32)]
 
 
 class Matrix(Structure):

@@ -69,8 +69,8 @@ def vocab_cross_entropy(x, weight, bias, targets, ignore_index=0, reduction="mea
     Rows whose target is ``ignore_index`` have loss 0 and gradient 0 and are not read; any other target outside [0, V)
     makes the loss NaN.  reduction: "mean" over the counted rows (NaN if there are none; the gradients are zero then),
     "sum", or "none" (a loss per target).  The loss is float32; gradients flow to x, weight and bias in their own type.
-    float32 operands above 64 rows are taken as pairs of float16 numbers scaled by the largest of each matrix: 22 bits, and
-    steps of 2^-39 of that largest number.  Likewise the rows' upstream gradients of float32 (above 64 rows) and float16
+    float32 operands above 64 rows are taken as pairs of float16 numbers scaled by the largest of each matrix (each row where
+    nothing asks for a gradient): 22 bits, and steps of 2^-39 of that largest number.  Likewise the rows' upstream gradients of float32 (above 64 rows) and float16
     operands: entries below 2^-38 of the largest are lost.
 
     A backward pass that is to be captured in a HIP graph must not run while an eager graph of the same leaves is alive:
@@ -88,6 +88,6 @@ def vocab_cross_entropy(x, weight, bias, targets, ignore_index=0, reduction="mea
         from . import autograd as AG
         loss = AG.vocab_cross_entropy(x2, weight, bias, t, ignore_index, reduction)
     else:
-        nll, loss, _ = ops.vocab_ce_forward(x2, weight, bias, t, ignore_index, want_loss=reduction != "none")
+        nll, loss, _ = ops.vocab_ce_forward(x2, weight, bias, t, ignore_index, want_loss=reduction != "none", loss_only=True)
         loss = nll if reduction == "none" else loss[0 if reduction == "mean" else 1]
     return loss.view(targets.shape) if reduction == "none" else loss

@@ -996,10 +996,11 @@ class VocabCEState:
     __slots__ = ("x", "W", "b", "targets", "args", "ref", "saved", "ws_bytes")
 
 
-def vocab_ce_forward(x, W, b, targets, ignore_index=0, want_loss=True):
+def vocab_ce_forward(x, W, b, targets, ignore_index=0, want_loss=True, loss_only=False):
     """Cross entropy of the projection x W^T + b, no logits kept: x [M,K], W [V,K], b [V] or None, all float32, bfloat16
     or float16 with unit column stride; targets [M] int64.  Returns (nll [M] fp32 with zeros for ignored rows,
-    loss [3] fp32 = (mean over the counted rows, sum, their number) or None, the state for ``vocab_ce_backward``)."""
+    loss [3] fp32 = (mean over the counted rows, sum, their number) or None, the state for ``vocab_ce_backward``).
+    ``loss_only``: no gradients will be asked for, and the state does not serve for them."""
     lib = _lib.load()
     ts = (x, W, targets) if b is None else (x, W, targets, b)
     for t in ts:
@@ -1022,7 +1023,7 @@ def vocab_ce_forward(x, W, b, targets, ignore_index=0, want_loss=True):
     st = VocabCEState()
     st.x, st.W, st.b, st.targets = x, W, b, targets
     st.args = a = _lib.VocabCE(x.data_ptr(), W.data_ptr(), _ptr(b), targets.data_ptr(), _row_stride(x, "x"),
-                               _row_stride(W, "W"), ignore_index, M, V, K, code)
+                               _row_stride(W, "W"), ignore_index, M, V, K, code, bool(loss_only))
     st.ref = r = byref(a)
     saved_bytes, ws_bytes = lib.capdec_vocab_ce_saved_bytes(r), lib.capdec_vocab_ce_forward_workspace_bytes(r)
     if not saved_bytes:
@@ -1056,6 +1057,8 @@ def vocab_ce_backward(state, grad=None, row_grad=None, mean=True, dx=None, dW=No
     where ``need`` says so."""
     if grad is not None and row_grad is not None:
         raise RuntimeError("capdec vocab_ce_backward: at most one of grad and row_grad")
+    if state.args.loss_only:
+        raise RuntimeError("capdec vocab_ce_backward: the forward call was for the loss alone")
     g = grad if grad is not None else row_grad
     if g is not None and (_chk(g, name="upstream gradient").numel() != (1 if grad is not None else state.args.M) or
                           not g.is_contiguous()):

@@ -641,6 +641,7 @@ typedef struct capdec_vocab_ce {
     int64_t ignore_index;
     int32_t M, V, K;
     int32_t dtype;                /* CAPDEC_F32 / CAPDEC_BF16 / CAPDEC_F16 */
+    int32_t loss_only;            /* != 0: no backward call follows (it would be refused) */
 } capdec_vocab_ce;
 size_t capdec_vocab_ce_saved_bytes(const capdec_vocab_ce* a /*host*/);
 size_t capdec_vocab_ce_forward_workspace_bytes(const capdec_vocab_ce* a /*host*/);

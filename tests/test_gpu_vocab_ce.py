@@ -532,3 +532,34 @@ def test_gradients_in_shared_memory():
         want = ops.vocab_ce_backward(state)
         got = ops.vocab_ce_backward(state, dx=x, dW=both[M:])
         assert all(torch.equal(p, q) for p, q in zip(got, want)) and got[0] is x
+
+
+@pytest.mark.parametrize("M,V,K", [(65, 500, 33), (70, 1000, 64), (200, 3000, 130), (700, 40000, 300), (600, 9000, 1540), (4200, 20000, 2048)])
+def test_loss_alone_of_float32_rows_of_any_size(M, V, K):
+    """Without gradients every row of x and W has a scale of its own: rows 1e-12 and 1e12 times the others keep their digits.
+    Bound of a row's logits from that row's own sums of magnitudes; no state that gradients could be taken from."""
+    from capdec import functional as F, ops
+    x, W, b, t = make(M, V, K, torch.float32, seed=51, ignored=0.2)
+    t[0] = V - 1
+    x[1:3] *= 1e-12
+    W[V // 2:V // 2 + 40] *= 1e-12
+    W[5] *= 1e12
+    x[:, :] = torch.where(torch.arange(K, device="cuda") < K // 2, x, -x.abs() * W[5].sign())      # (word 5 far below the others)
+    b[5] = -1e30
+    x[4] = 0
+    live = t != 0
+    z = x.double() @ W.double().T + b.double()
+    S = x.double().abs() @ W.double().abs().T + b.double().abs()
+    keep = [v for v in range(V) if v != 5]
+    z, S = z[:, keep], S[:, keep]
+    t2 = torch.where(t > 5, t - 1, t)
+    ok = live & (t != 5)
+    nll = torch.logsumexp(z, 1) - z.gather(1, t2[:, None])[:, 0]
+    dz = (3 * 2.0 ** -22 + (K + 1) * 2.0 ** -24) * S.max(1).values
+    tol = 2 * dz + (3 * z.abs().max(1).values * 1.4427 + 200) * 2.0 ** -23
+    got = F.vocab_cross_entropy(x, W, b, t, reduction="none")
+    assert bool((got[~live] == 0).all())
+    near(got[ok], nll[ok], tol[ok], "loss")
+    _, _, state = ops.vocab_ce_forward(x, W, b, t, loss_only=True)
+    with pytest.raises(RuntimeError, match="loss alone"):
+        ops.vocab_ce_backward(state)
