@@ -672,36 +672,44 @@ def _decoder_params(dec):
 
 
 class _VocabCrossEntropyFn(torch.autograd.Function):
-    """``ops.vocab_ce_forward`` / ``vocab_ce_backward`` as an autograd node; reduction "none", "sum" or "mean"."""
+    """``ops.vocab_ce_forward`` / ``vocab_ce_backward`` as an autograd node; reduction "none", "sum" or "mean".
+
+    W as it was in the forward call and the kernels' own buffer are saved tensors of the node: they are released with its
+    backward pass, go through saved-tensor hooks, and W stays what the forward call read where a parameter's ``data`` is
+    exchanged in between.  Of x, the bias and the targets the backward pass has all it needs in that buffer."""
 
     @staticmethod
     def forward(ctx, x, W, b, targets, ignore_index, reduction):
         ctx.reduction, ctx.state = reduction, None
-        ctx.save_for_backward(x, W, b)
+        ctx.shapes = x.shape, W.shape, None if b is None else b.shape
         if x.shape[0] == 0:                       # no rows: the mean over none is NaN, every gradient zero
+            ctx.save_for_backward(x.detach())     # (for the gradients' type and device)
             return {"none": x.new_zeros(0, dtype=torch.float32), "sum": x.new_zeros((), dtype=torch.float32),
                     "mean": x.new_full((), float("nan"), dtype=torch.float32)}[reduction]
         nll, loss, ctx.state = ops.vocab_ce_forward(x, W, b, targets, ignore_index, want_loss=reduction != "none")
+        ctx.save_for_backward(*ctx.state.release())
         return nll if reduction == "none" else loss[0 if reduction == "mean" else 1]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        x, W, b = ctx.saved_tensors               # raises where one was changed in place since
+        nx, nw, nb = ctx.needs_input_grad[:3]
         if ctx.state is None:
-            return tuple(torch.zeros_like(t) if t is not None and n else None
-                         for t, n in zip((x, W, b), ctx.needs_input_grad)) + (None, None, None)
+            like, = ctx.saved_tensors
+            return tuple(like.new_zeros(s) if s is not None and n else None
+                         for s, n in zip(ctx.shapes, (nx, nw, nb))) + (None, None, None)
+        W, saved = ctx.saved_tensors              # raises where W was changed in place since
         # (the gradient of an fp32 loss is fp32; a row's may come expanded)
         rows = ctx.reduction == "none"
         if rows:
             g = g.contiguous()
-        nx, nw, nb = ctx.needs_input_grad[:3]
-        st = ctx.state
-        K = x.shape[1]
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if nx else None
-        dW = torch.empty(W.shape, device=x.device, dtype=x.dtype) if nw else None
-        db = torch.empty(b.shape, device=x.device, dtype=x.dtype) if nb else None
-        ops._vocab_ce_backward(st, g if rows else None, None if rows else g, ctx.reduction == "mean", dx, K, dW, K, db)
+        sx, sw, sb = ctx.shapes
+        K = sx[1]
+        dx = torch.empty(sx, device=W.device, dtype=W.dtype) if nx else None
+        dW = torch.empty(sw, device=W.device, dtype=W.dtype) if nw else None
+        db = torch.empty(sb, device=W.device, dtype=W.dtype) if nb else None
+        ops._vocab_ce_backward(ctx.state, W, saved, g if rows else None, None if rows else g, ctx.reduction == "mean", dx, K, dW, K,
+                               db)
         return dx, dW, db, None, None, None
 
 

@@ -991,9 +991,17 @@ def _bytes(n, device):
 
 
 class VocabCEState:
-    """What ``vocab_ce_forward`` leaves for ``vocab_ce_backward``: the operands (neither of them may change in between), the
-    call's arguments, and the packed operands and row statistics in device memory."""
-    __slots__ = ("x", "W", "b", "targets", "args", "ref", "saved", "ws_bytes")
+    """What ``vocab_ce_forward`` leaves for ``vocab_ce_backward``: W (which may not change in between; the memory that the
+    forward call read, whatever becomes of a parameter's ``data``), the call's arguments, and the packed operands and row
+    statistics in device memory."""
+    __slots__ = ("x", "W", "b", "args", "ref", "saved", "ws_bytes")
+
+    def release(self):
+        """The two tensors of the state that the backward call reads, W and the packed operands, for someone else to hold:
+        the state keeps no tensor."""
+        held = self.W, self.saved
+        self.x = self.W = self.b = self.saved = None
+        return held
 
 
 def vocab_ce_forward(x, W, b, targets, ignore_index=0, want_loss=True, loss_only=False):
@@ -1021,7 +1029,7 @@ def vocab_ce_forward(x, W, b, targets, ignore_index=0, want_loss=True, loss_only
     if b is not None and (b.shape != (V,) or not b.is_contiguous()):
         raise RuntimeError(f"capdec vocab_ce: bias must hold {V} contiguous values, got {tuple(b.shape)}")
     st = VocabCEState()
-    st.x, st.W, st.b, st.targets = x, W, b, targets
+    st.x, st.W, st.b = x, W.detach(), b
     st.args = a = _lib.VocabCE(x.data_ptr(), W.data_ptr(), _ptr(b), targets.data_ptr(), _row_stride(x, "x"),
                                _row_stride(W, "W"), ignore_index, M, V, K, code, bool(loss_only))
     st.ref = r = byref(a)
@@ -1038,12 +1046,21 @@ def vocab_ce_forward(x, W, b, targets, ignore_index=0, want_loss=True, loss_only
     return out[:M], out[M:] if want_loss else None, st
 
 
-def _vocab_ce_backward(st, row_grad, grad, mean, dx, lddx, dW, lddw, db):
-    """The launch of ``vocab_ce_backward`` on checked tensors (None: not wanted, or no upstream gradient)."""
-    lib = _lib.load()
+def _vocab_ce_backward(st, W, saved, row_grad, grad, mean, dx, lddx, dW, lddw, db):
+    """The launch of ``vocab_ce_backward`` on checked tensors (None: not wanted, or no upstream gradient).  W holds the
+    values of the forward call, ``saved`` the buffer that it filled; both may have been elsewhere in between."""
+    lib, a = _lib.load(), st.args
+    if a.W != W.data_ptr() or a.ldw != _row_stride(W, "W"):
+        a.W, a.ldw, st.ws_bytes = W.data_ptr(), _row_stride(W, "W"), None
+        n = lib.capdec_vocab_ce_saved_bytes(st.ref)
+        if n != saved.numel():
+            # 16-bit rows are packed, or read in place where their alignment allows it; as the forward call had it
+            ld = a.K + (1 if n < saved.numel() else 0)
+            W = torch.empty(a.V, ld, device=W.device, dtype=W.dtype)[:, :a.K].copy_(W)
+            a.W, a.ldw = W.data_ptr(), ld
     if st.ws_bytes is None:
         st.ws_bytes = lib.capdec_vocab_ce_backward_workspace_bytes(st.ref)
-    n, saved = st.ws_bytes, st.saved
+    n = st.ws_bytes
     ws = _bytes(n, saved.device)
     _lib.check(lib.capdec_vocab_ce_backward(st.ref, saved.data_ptr(), saved.numel(), ws.data_ptr(), n, _ptr(row_grad),
                                             _ptr(grad), 1 if mean else 0, _ptr(dx), lddx, _ptr(dW), lddw, _ptr(db),
@@ -1076,7 +1093,7 @@ def vocab_ce_backward(state, grad=None, row_grad=None, mean=True, dx=None, dW=No
     _same_device("vocab_ce_backward", [t for t in (g, state.saved, *outs) if t is not None])
     dx, dW, db = outs
     _check_overlap("vocab_ce_backward", [t if t.dim() == 2 else t[None] for t in outs if t is not None], [state.W])
-    _vocab_ce_backward(state, row_grad, grad, mean, dx, 0 if dx is None else _row_stride(dx, "dx"), dW,
+    _vocab_ce_backward(state, state.W, state.saved, row_grad, grad, mean, dx, 0 if dx is None else _row_stride(dx, "dx"), dW,
                        0 if dW is None else _row_stride(dW, "dW"), db)
     return dx, dW, db
 

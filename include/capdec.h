@@ -623,8 +623,9 @@ int capdec_satt_greedy_decode(const capdec_satt_model* m, const float* enc, cons
  * one type.  Rows of x whose target is ignore_index are not read.  A counted target outside [0, V) makes its loss and
  * the gradients it enters NaN.  M, V <= 2^24, M V <= 2^42, K <= 2^20.
  * `saved` (capdec_vocab_ce_saved_bytes) carries packed operands (for up to 64 rows of fp32: x and the logits) and row
- * statistics from the forward call to the backward call, which reads W again: neither W nor `saved` may change in between.  `workspace` is scratch of one call.  Both are
- * 16-byte aligned.  Sums run in fixed orders: results repeat bit for bit.
+ * statistics from the forward call to the backward call, which reads W again, but neither x, bias nor targets: neither W
+ * nor `saved` may change in between, and W keeps its alignment.  `workspace` is scratch of one call.  Both are 16-byte
+ * aligned.  Sums run in fixed orders: results repeat bit for bit.
  * forward: nll [M] fp32; loss (nullable) [3] fp32 = (mean over the counted rows, NaN without any; sum; their number).
  * backward: the upstream gradient is row_grad [M] (fp32, d/d nll) or, where that is NULL, grad[0] (NULL: 1) for the sum of
  * nll (mean == 0) or for its mean (mean != 0); dx, dW, dbias are written (not added to), any of them may be NULL.
