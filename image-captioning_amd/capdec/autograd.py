@@ -688,7 +688,10 @@ class _VocabCrossEntropyFn(torch.autograd.Function):
                     "mean": x.new_full((), float("nan"), dtype=torch.float32)}[reduction]
         nll, loss, ctx.state = ops.vocab_ce_forward(x, W, b, targets, ignore_index, want_loss=reduction != "none")
         ctx.save_for_backward(*ctx.state.release())
-        return nll if reduction == "none" else loss[0 if reduction == "mean" else 1]
+        out = nll if reduction == "none" else loss[0 if reduction == "mean" else 1]
+        # a tensor of its own on that memory: autograd lets no caller change a view from in here in place (loss /= n)
+        return torch.empty(0, device=out.device, dtype=out.dtype).set_(out.untyped_storage(), out.storage_offset(), out.shape,
+                                                                       out.stride())
 
     @staticmethod
     @torch.autograd.function.once_differentiable

@@ -94,3 +94,19 @@ def test_saved_tensor_hooks(M, K, off, dt):
         loss = loss_of(x, view, b, t)
     got = torch.autograd.grad(loss, (x, view, b))
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("M", [0, 20, 100])
+def test_loss_changed_in_place(M, reduction):
+    """``loss /= n`` and the like, as on any other loss."""
+    x, W, b, t = make(max(M, 1), 300, 64, torch.float32)
+    x = x[:M]
+    one = loss_of(x, W, b, t[:M], reduction)
+    out = torch.ones_like(one)
+    want = torch.autograd.grad(one, (W, b), out * 0.25)
+    loss = loss_of(x, W, b, t[:M], reduction)
+    loss /= 4
+    got = torch.autograd.grad(loss, (W, b), out)
+    assert torch.equal(loss, one / 4) or M == 0
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
