@@ -73,6 +73,8 @@ def vocab_cross_entropy(x, weight, bias, targets, ignore_index=0, reduction="mea
     nothing asks for a gradient): 22 bits, and steps of 2^-39 of that largest number.  Likewise the rows' upstream gradients of float32 (above 64 rows) and float16
     operands: entries below 2^-38 of the largest are lost.
 
+    There is no forward-mode derivative: an input that carries a tangent is refused.
+
     A backward pass that is to be captured in a HIP graph must not run while an eager graph of the same leaves is alive:
     drop the losses of earlier eager passes first."""
     if reduction not in ("mean", "sum", "none"):
@@ -83,8 +85,10 @@ def vocab_cross_entropy(x, weight, bias, targets, ignore_index=0, reduction="mea
     if (x2.stride(1) != 1 and x2.shape[1] > 1) or (x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]):
         x2 = x2.contiguous()                       # columns apart, or rows that share memory (a broadcast x)
     t = t.contiguous()
-    if x2.shape[0] == 0 or (torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad or
-                                                          (bias is not None and bias.requires_grad))):
+    ins = (x2, weight) if bias is None else (x2, weight, bias)
+    # (a tangent of forward-mode differentiation goes to the node as well, which refuses it rather than lose it)
+    if x2.shape[0] == 0 or (torch.is_grad_enabled() and any(v.requires_grad for v in ins)) or \
+            any(torch.autograd.forward_ad.unpack_dual(v).tangent is not None for v in ins):
         from . import autograd as AG
         loss = AG.vocab_cross_entropy(x2, weight, bias, t, ignore_index, reduction)
     else:

@@ -110,3 +110,20 @@ def test_loss_changed_in_place(M, reduction):
     got = torch.autograd.grad(loss, (W, b), out)
     assert torch.equal(loss, one / 4) or M == 0
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("M", [20, 100])
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_tangents_are_refused(which, M):
+    """Forward-mode differentiation is not offered: an input's tangent is refused, not dropped, with and without gradients."""
+    from torch.autograd import forward_ad as fw
+    x, W, b, t = make(M, 300, 64, torch.float32)
+    for grads in (False, True):
+        ins = [v.detach().requires_grad_(grads) for v in (x, W, b)]
+        with fw.dual_level():
+            ins[which] = fw.make_dual(ins[which], torch.ones_like(ins[which]))
+            with pytest.raises(RuntimeError, match="jvp|forward"):
+                loss_of(*ins, t)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="jvp|forward"):
+                loss_of(*ins, t)
+    assert bool(loss_of(*(v.detach() for v in (x, W, b)), t).isfinite())
