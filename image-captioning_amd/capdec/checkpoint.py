@@ -7,6 +7,8 @@ trainable decoder + feature head, whose keys are a subset of the reference's, so
 
 Files are read with ``torch.load(..., weights_only=True)``: nothing in the file is executed.
 """
+import warnings
+
 import torch
 
 _BUFFER_SUFFIXES = ("running_mean", "running_var", "num_batches_tracked", "positional_encoding.pe")
@@ -24,7 +26,11 @@ def load_reference_checkpoint(path_or_dict, model, trainer=None):
     ``optimizer="muon"`` steps (entry ``"muon"`` of a checkpoint that such a trainer wrote, by parameter name).  The reference's optimizer state is keyed by parameter
     index in ``model.parameters()`` order of ITS model (backbone first); the index of a name is recovered as its rank
     among the state_dict keys that are not buffers (``running_*``, ``num_batches_tracked``, ``positional_encoding.pe``).
-    Parameters without a stored state (the frozen backbone never gets one) are skipped."""
+    Parameters without a stored state (the frozen backbone never gets one) are skipped.
+
+    Matrices that the checkpoint's trainer stepped by momentum and ``trainer`` steps with Adam have no moments to restore.
+    Zero moments under the stored step count would make their first updates three to six times the learning rate, and
+    there is one step count for all: Adam starts afresh then (all moments and the count zero), with a warning."""
     ckpt = path_or_dict if isinstance(path_or_dict, dict) else torch.load(path_or_dict, map_location="cpu",
                                                                           weights_only=True)
     ref_sd = ckpt["state_dict"]
@@ -41,6 +47,10 @@ def load_reference_checkpoint(path_or_dict, model, trainer=None):
         prefix = "decoderRNN." if core is not None else ""
         steps = set()
         momenta = ckpt.get("muon", {})
+        fresh = [n for n in trainer.grads if prefix + n in momenta and n not in trainer.muon_names]
+        if fresh:
+            warnings.warn(f"capdec: the checkpoint holds orthogonalised updates' momenta for {len(fresh)} matrices that this trainer "
+                          f"steps with Adam ({fresh[0]}, ...): Adam's moments and step count start afresh")
         for name, grad_view in trainer.grads.items():
             if name in trainer.muon_names:                 # a checkpoint written with Adam has no momentum for it: zero
                 a = (grad_view.data_ptr() - trainer.flat_g.data_ptr()) // 4
@@ -51,7 +61,7 @@ def load_reference_checkpoint(path_or_dict, model, trainer=None):
                     mom.zero_()
                 continue
             st = state.get(index_of.get(prefix + name, -1))
-            if st is None:
+            if fresh or st is None:
                 continue
             off = grad_view.data_ptr() - trainer.flat_g.data_ptr()
             a = off // 4
@@ -59,6 +69,11 @@ def load_reference_checkpoint(path_or_dict, model, trainer=None):
             trainer.m[a:a + n].copy_(st["exp_avg"].reshape(-1))
             trainer.v[a:a + n].copy_(st["exp_avg_sq"].reshape(-1))
             steps.add(int(st["step"]))
+        if fresh:
+            for a, b in trainer.adam_runs:
+                trainer.m[a:b].zero_()
+                trainer.v[a:b].zero_()
+            steps = {0}
         if steps:
             trainer.t = max(steps)
         groups = ckpt["optimizer"].get("param_groups")
