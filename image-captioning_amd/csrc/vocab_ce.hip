@@ -84,11 +84,13 @@ bool wide_pays(int64_t wide_tiles, int kt) { return kt >= 48 && wide_tiles >= 25
 bool make_plan(const capdec_vocab_ce* a, Plan& p) {
     if (!a || a->M < 1 || a->V < 1 || a->K < 1 || a->dtype < 0 || a->dtype > 2) return false;
     if (a->M > (1 << 24) || a->V > (1 << 24) || a->K > (1 << 20)) return false;
-    if ((int64_t)a->M * a->V > (int64_t)1 << 42) return false;          // tiles are counted in 32 bits
     p = Plan{};
     p.M = a->M; p.V = a->V; p.K = a->K;
     p.Mp = (a->M + 255) / 256 * 256;
     p.Vp = (a->V + 255) / 256 * 256;
+    // a launch has less than 2^32 work-items; the logits take one for 128 of them, in workgroups of up to 512, eight of which
+    // may be added to make their number a multiple of 8
+    if ((int64_t)p.Mp * p.Vp > ((int64_t)1 << 39) - ((int64_t)1 << 19)) return false;
     p.Kp = (a->K + 31) / 32 * 32;
     p.split = a->dtype == CAPDEC_F32;
     p.elt = a->dtype == CAPDEC_BF16 ? BF16 : F16;

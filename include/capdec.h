@@ -621,7 +621,8 @@ int capdec_satt_greedy_decode(const capdec_satt_model* m, const float* enc, cons
  *   z = x W^T + bias;  nll[r] = log(sum_v exp z[r,v]) - z[r, targets[r]], 0 where targets[r] == ignore_index
  * x [M,K] and W [V,K] have unit column stride and row strides ldx, ldw (elements); x, W, bias and their gradients share
  * one type.  Rows of x whose target is ignore_index are not read.  A counted target outside [0, V) makes its loss and
- * the gradients it enters NaN.  M, V <= 2^24, M V <= 2^42, K <= 2^20.
+ * the gradients it enters NaN.  M, V <= 2^24, K <= 2^20 and, with
+ * M and V rounded up to multiples of 256, M V <= 2^39 - 2^19.
  * `saved` (capdec_vocab_ce_saved_bytes) carries packed operands (for up to 64 rows of fp32: x and the logits) and row
  * statistics from the forward call to the backward call, which reads W again, but neither x, bias nor targets: neither W
  * nor `saved` may change in between, and W keeps its alignment.  `workspace` is scratch of one call.  Both are 16-byte
