@@ -183,7 +183,7 @@ bool make_plan(const capdec_vocab_ce* a, Plan& p) {
 
 struct Head {               // first 256 bytes of the saved buffer
     int count;              // rows with a counted target
-    unsigned amax_x, amax_w;   // bits of the largest finite magnitude (split operands)
+    int ex, ew;             // split operands: x and W are packed times 2^ex and 2^ew
 };
 struct BwdHead {            // first 256 bytes of the backward workspace (upstream gradients of the rows)
     float factor;           // what dx, dW and db are to be multiplied by
@@ -199,11 +199,10 @@ __device__ __forceinline__ float factor_of(const Upstream& u, const Head* head) 
     return ldexpf((u.grad ? u.grad[0] : 1.f) / (u.mean ? (float)head->count : 1.f), -G_EXP);
 }
 
-// power of two that brings amax to [2^14, 2^15); the operands' scales are undone in fp32
-__device__ __forceinline__ int scale_exp(unsigned amax_bits) {
-    const int e = (int)(amax_bits >> 23) - 127;        // floor(log2), denormals count as 2^-127
-    if (amax_bits == 0) return 0;
-    return min(14 - e, 60);
+// power of two that brings amax to [2^14, 2^15), denormal numbers below it (-113 .. 141, more than one fp32 number holds)
+__device__ __forceinline__ int scale_exp(float amax) {
+    const unsigned bits = __float_as_uint(amax);
+    return bits == 0 ? 0 : 14 - ((int)(bits >> 23) - 127);
 }
 __device__ __forceinline__ float pow2(int e) { return ldexpf(1.f, e); }
 
@@ -272,7 +271,7 @@ __device__ void compact(const ScanArgs& a) {
     }
     if (threadIdx.x == 0) {
         a.head->count = done;
-        a.head->amax_x = a.head->amax_w = 0;
+        a.head->ex = a.head->ew = 0;
     }
 }
 
@@ -347,7 +346,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     const int64_t total = a.nx + a.nw + a.Vp;
     const int cpr = a.Kp / 8;
     const int count = a.head->count;
-    float scale[2] = {1.f, 1.f};
+    int scale[2] = {0, 0};
     if (a.split) {                                  // every block joins the partial maxima for itself; the first notes them
         __shared__ float wm[2][4];
         float m[2] = {0.f, 0.f};
@@ -364,11 +363,11 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             m[k] = fmaxf(fmaxf(wm[k][0], wm[k][1]), fmaxf(wm[k][2], wm[k][3]));
-            scale[k] = pow2(scale_exp(__float_as_uint(m[k])));
+            scale[k] = scale_exp(m[k]);
         }
         if (blockIdx.x == 0 && threadIdx.x == 0) {
-            a.head->amax_x = __float_as_uint(m[0]);
-            a.head->amax_w = __float_as_uint(m[1]);
+            a.head->ex = scale[0];
+            a.head->ew = scale[1];
         }
     }
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
@@ -395,7 +394,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
             }
             *reinterpret_cast<s16x8*>(dst + c) = o;
         } else {
-            const float s = scale[isw];
+            const int s = scale[isw];
             float v[8];
             if (!zero && a.vec && c + 8 <= a.K) {
                 const f32x4* q = reinterpret_cast<const f32x4*>((const float*)src + base + c);
@@ -410,7 +409,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 short h, l;
-                split16(v[e] * s, h, l);
+                split16(ldexpf(v[e], s), h, l);
                 hi[e] = h;
                 lo[e] = l;
             }
@@ -453,9 +452,8 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a, RowScales f)
             for (int c = lane; c < a.K; c += 64) see(src[c]);
         }
         m = wave_max(m);
-        const int e2 = scale_exp(__float_as_uint(m));
-        const float s = pow2(e2);
-        if (lane == 0) (isw ? f.w : f.x)[row] = pow2(-e2);
+        const int s = scale_exp(m);
+        if (lane == 0) (isw ? f.w : f.x)[row] = pow2(-s);
         for (int c = lane * 4; c < a.Kp; c += 256) {                   // four columns: halves of a group's hi and lo
             f32x4 v = {0.f, 0.f, 0.f, 0.f};
             if (VEC) {
@@ -469,7 +467,7 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a, RowScales f)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 short h, l;
-                split16(v[e] * s, h, l);
+                split16(ldexpf(v[e], s), h, l);
                 hi[e] = h;
                 lo[e] = l;
             }
@@ -505,7 +503,7 @@ struct LogitArgs {
 
 template <bool SPLIT>
 __device__ __forceinline__ float logit_scale(const Head* head) {
-    return SPLIT ? pow2(-scale_exp(head->amax_x)) * pow2(-scale_exp(head->amax_w)) * L2E : L2E;
+    return SPLIT ? ldexpf(L2E, -(head->ex + head->ew)) : L2E;
 }
 
 template <class C, int ELT, bool SPLIT, bool BY_ROW>
@@ -525,12 +523,12 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void lse_kernel(LogitArgs a) {
     }
     f32x16 acc[C::TI][C::TJ];
     contract<C, ELT, false, false, SPLIT>(a.W, a.X, i0, j0, 0, a.kt, lds, acc);
-    const float c0 = BY_ROW ? L2E : logit_scale<SPLIT>(a.head);
+    const float c0 = logit_scale<SPLIT>(a.head);
     float2* red = reinterpret_cast<float2*>(lds);
 #pragma unroll
     for (int tj = 0; tj < C::TJ; ++tj) {
         float m = -INFINITY;
-        const float c1 = BY_ROW ? c0 * a.f.x[j0 + (wj * C::TJ + tj) * 32 + (lane & 31)] : c0;
+        const float c1 = BY_ROW ? a.f.x[j0 + (wj * C::TJ + tj) * 32 + (lane & 31)] : c0;
 #pragma unroll
         for (int ti = 0; ti < C::TI; ++ti)
 #pragma unroll
@@ -538,7 +536,8 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void lse_kernel(LogitArgs a) {
                 const int word = i0 + (wi * C::TI + ti) * 32 + 8 * q + 4 * h;
                 const f32x4 b = *reinterpret_cast<const f32x4*>(a.b2 + word);
                 f32x4 c = {c1, c1, c1, c1};
-                if (BY_ROW) c *= *reinterpret_cast<const f32x4*>(a.f.w + word);
+                // (the two powers first: one alone may be denormal, which would round its product with L2E)
+                if (BY_ROW) c = c * *reinterpret_cast<const f32x4*>(a.f.w + word) * L2E;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float v = fmaf(acc[ti][tj][4 * q + e], c[e], b[e]);
@@ -849,11 +848,8 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void grad_kernel(GradArgs a) {
             }
         }
     }
-    float f = 1.f;
-    if (OUT == 1) {
-        f = factor_of(a.up, a.head);
-        if (SPLIT) f *= pow2(-scale_exp(a.head->amax_x));
-    }
+    const float f = OUT == 1 ? factor_of(a.up, a.head) : 1.f;
+    const int ex = OUT == 1 && SPLIT ? -a.head->ex : 0;
     if (OUT == 1 && !SPLIT && a.vec) {
         // 16-bit results go through LDS, 32 rows of the wavefront at a time: stores of 16 bytes a lane instead of 2
         constexpr int COLS = 32 * C::TJ, LD = COLS + 8, CH = COLS / 8;
@@ -898,7 +894,7 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void grad_kernel(GradArgs a) {
                 const int i = ib + acc_row(e, h);
                 if (i >= nI) continue;
                 if (OUT == 0) d[(int64_t)i * a.ldp] = acc[ti][tj][e];
-                else store_as(a.out, (int64_t)i * a.ldo + j, acc[ti][tj][e] * f, a.dtype);
+                else store_as(a.out, (int64_t)i * a.ldo + j, SPLIT ? ldexpf(acc[ti][tj][e] * f, ex) : acc[ti][tj][e] * f, a.dtype);
             }
         }
     }
@@ -911,7 +907,8 @@ __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part,
                                                  const float* __restrict__ rest, const void* W, int64_t ldw,
                                                  const Head* __restrict__ head, Upstream up, int split, void* out,
                                                  int64_t ldo, int dtype) {
-    const float f = factor_of(up, head) * (split ? pow2(-scale_exp(head->amax_w)) : 1.f);
+    const float f = factor_of(up, head);
+    const int ew = split ? -head->ew : 0;
     const int tiles = (head->count + 255) / 256, nsplit = splits_of(splits, tiles);
     const int64_t plane = (int64_t)(rows ? rows : tiles * 256) * Kp;
     const int cpr = (K + 3) / 4;
@@ -930,7 +927,7 @@ __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part,
                     if (c + e < K) v[e] = fmaf(q, load_as_f32(W, (int64_t)w * ldw + c + e, dtype), v[e]);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] *= f;
+            for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e] * f, ew);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -942,8 +939,8 @@ __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ part,
 __global__ __launch_bounds__(256) void dw_kernel(const float* __restrict__ part, int64_t plane, int nsplit, int Kp, int rows,
                                                  int K, const Head* __restrict__ head, Upstream up, int split, void* dW,
                                                  int64_t ldw, int dtype, const float* __restrict__ dbp, int piece, int row_tile, void* db, int v0) {
-    const float fb = factor_of(up, head);
-    const float f = fb * (split ? pow2(-scale_exp(head->amax_x)) : 1.f);
+    const float f = factor_of(up, head);
+    const int ex = split ? -head->ex : 0;
     const int cpr = (K + 3) / 4;
     const int64_t nw = nsplit > 1 ? (int64_t)rows * cpr : 0;
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < nw + (dbp ? rows : 0); t += (int64_t)gridDim.x * 256) {
@@ -951,7 +948,7 @@ __global__ __launch_bounds__(256) void dw_kernel(const float* __restrict__ part,
             const int v = (int)(t - nw), tiles = (head->count + row_tile - 1) / row_tile;
             float s = 0.f;
             for (int k = 0; k < tiles; ++k) s += dbp[(int64_t)k * piece + v];
-            store_as(db, v0 + v, s * fb, dtype);
+            store_as(db, v0 + v, s * f, dtype);
             continue;
         }
         const int r = (int)(t / cpr), c = (int)(t - (int64_t)r * cpr) * 4;
@@ -960,7 +957,7 @@ __global__ __launch_bounds__(256) void dw_kernel(const float* __restrict__ part,
         for (int k = 0; k < nsplit; ++k) v += *reinterpret_cast<const f32x4*>(part + k * plane + (int64_t)r * Kp + c);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (c + e < K) store_as(dW, (int64_t)(v0 + r) * ldw + c + e, v[e] * f, dtype);
+            if (c + e < K) store_as(dW, (int64_t)(v0 + r) * ldw + c + e, ldexpf(v[e] * f, ex), dtype);
     }
 }
 
