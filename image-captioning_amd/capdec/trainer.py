@@ -112,8 +112,9 @@ class CaptionTrainer:
         get_loader.py:184, so the shape changes from batch to batch: pad or bucket the captions to few lengths, or the
         step mostly runs launch by launch); the least recently used one is dropped.
         vocab_loss: "logits" materialises the [rows, vocabulary] logits and turns them into their gradient in place; "pieces"
-        keeps no logits and forms the gradient for a piece of the vocabulary at a time (same loss and gradients to fp32's
-        rounding; less memory, and faster from a few thousand rows on).
+        keeps no logits and forms the gradient for a piece of the vocabulary at a time (``functional.vocab_cross_entropy``, which
+        says what it keeps of float32: loss and gradients to about fp32's rounding; less memory, and faster from a few
+        thousand rows on).
         optimizer: "adam" for every parameter; "muon" steps the matrices of the decoder layers and of the LSTM along their
         orthogonalised momentum (``ops.muon_step`` with ``muon_momentum``, ``muon_nesterov``, ``muon_weight_decay``) and
         everything else -- embedding, vocabulary projection, feature head, biases, norms -- with Adam.  Both share the

@@ -309,6 +309,79 @@ __device__ __forceinline__ void contract(const View& P, const View& Q, int i0, i
     }
 }
 
+// The same tile sum from fp32 operands on the fp32 matrix instruction (v_mfma_f32_32x32x2_f32, the same accumulators), for
+// operands whose entries are too far apart for pairs.  Elements past an operand's k limit count as zero, rows past its end
+// are copies of its last.  k-tiles of 32 in LDS, rows 33 apart, so that reads and both orders of writes meet no bank twice;
+// loads are neither ahead nor wide, and nothing is assumed of their alignment.
+struct View32 {             // one fp32 operand
+    const float* p;
+    int64_t ld;             // elements between rows of the stored matrix
+    const int* order;       // N: where row x is stored; nullable
+    int n;                  // extent of the i or j axis
+};
+template <int NX, int THREADS, bool T>
+__device__ __forceinline__ void stage32(const View32& v, int x0, int k0, int klim, float* img) {
+    constexpr int BATCH = 16, STEP = T ? THREADS / NX : THREADS / 32;      // loads in flight; rows between a thread's elements
+    static_assert(NX * 32 % (THREADS * BATCH) == 0 && (!T || THREADS % NX == 0), "elements do not divide over the threads");
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));        // addresses are made here each time: kept over the k-tiles they cost other code its registers
+    const int fix = T ? tid % NX : tid % 32, var = T ? tid / NX : tid / 32;
+    const int at = T ? min(x0 + fix, v.n - 1) : min(k0 + fix, klim - 1);   // always inside; zeros are put in afterwards
+#pragma unroll 1
+    for (int i = 0; i < NX * 32 / THREADS; i += BATCH) {
+        float q[BATCH];
+#pragma unroll
+        for (int e = 0; e < BATCH; ++e) {
+            const int r = var + (i + e) * STEP;
+            const int row = T ? min(k0 + r, klim - 1) : min(x0 + r, v.n - 1);
+            q[e] = v.p[(int64_t)(!T && v.order ? v.order[row] : row) * v.ld + at];
+        }
+#pragma unroll
+        for (int e = 0; e < BATCH; ++e) {
+            const int r = var + (i + e) * STEP, k = T ? r : fix;
+            img[(T ? fix : r) * 33 + k] = k0 + k < klim ? q[e] : 0.f;
+        }
+    }
+}
+// k in [k0, k1); elements from klim on are zero.  Ends behind a barrier.
+template <class C, bool TP, bool TQ>
+__device__ __forceinline__ void contract32(const View32& P, const View32& Q, int i0, int j0, int k0, int k1, int klim, short* lds,
+                                           f32x16 (&acc)[C::TI][C::TJ]) {
+    static_assert(C::KG == 1 && (C::BI + C::BJ) * 33 * 4 <= C::LDS_BYTES, "the tile does not fit");
+    float* const ip = reinterpret_cast<float*>(lds);
+    float* const iq = ip + C::BI * 33;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave / C::WJ, wj = wave % C::WJ, h = lane >> 5;
+#pragma unroll
+    for (int ti = 0; ti < C::TI; ++ti)
+#pragma unroll
+        for (int tj = 0; tj < C::TJ; ++tj)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[ti][tj][e] = 0.f;
+    klim = min(klim, k1);
+    for (int k = k0; k < klim; k += 32) {
+        stage32<C::BI, C::THREADS, TP>(P, i0, k, klim, ip);
+        stage32<C::BJ, C::THREADS, TQ>(Q, j0, k, klim, iq);
+        __syncthreads();
+        const float* a = ip + (wi * C::TI * 32 + (lane & 31)) * 33 + h;
+        const float* b = iq + (wj * C::TJ * 32 + (lane & 31)) * 33 + h;
+#pragma unroll 2
+        for (int kk = 0; kk < 32; kk += 2) {
+            float av[C::TI], bv[C::TJ];
+#pragma unroll
+            for (int ti = 0; ti < C::TI; ++ti) av[ti] = a[ti * 32 * 33 + kk];
+#pragma unroll
+            for (int tj = 0; tj < C::TJ; ++tj) bv[tj] = b[tj * 32 * 33 + kk];
+#pragma unroll
+            for (int ti = 0; ti < C::TI; ++ti)
+#pragma unroll
+                for (int tj = 0; tj < C::TJ; ++tj)
+                    acc[ti][tj] = __builtin_amdgcn_mfma_f32_32x32x2f32(av[ti], bv[tj], acc[ti][tj], 0, 0, 0);
+        }
+        __syncthreads();
+    }
+    __syncthreads();
+}
+
 // Workgroup -> tile.  Workgroup ids go round-robin to the 8 XCDs, each with an L2 of its own: XCD x takes the x-th
 // eighth of the tile sequence, and the sequence walks blocks of eight i-tiles by all j, so that the workgroups that run
 // on one XCD at a time share operand rows.  A performance assumption only.

@@ -8,7 +8,7 @@
 // rows' log-sum-exp, and contracted with W and x while it is in the caches.  Four products of 2 M V K flops in all for
 // loss and gradients, bound by the matrix cores at large sizes and by reading W at few rows.
 // fp32 operands are split into two fp16 numbers (mma16.h), but for batches of at most 64 rows, which have kernels of their
-// own that read W as it is; 16-bit operands are multiplied as they are.  Sums, softmax
+// own that read W as it is, and for rows too far apart (FAR below); 16-bit operands are multiplied as they are.  Sums, softmax
 // statistics and the partial sums of the gradients are fp32.  G takes the operands' 16-bit type (scaled by 2^14, so
 // that probabilities down to 2^-28 stay normal in fp16).  That rounding averages out in sums over rows or words, except
 // at the targets, whose entries are near -g_r: what it takes off them is carried beside G and added to dx, and to dW up to
@@ -16,6 +16,7 @@
 // Every sum has a fixed order: results repeat bit for bit.
 #include "mma16.h"
 #include <math.h>
+#include <type_traits>
 
 using namespace mma16;
 
@@ -27,6 +28,13 @@ constexpr size_t PIECE_BYTES = (size_t)512 << 20;
 constexpr int FEW = 64;                          // rows of fp32 up to which W is read as it is
 constexpr int FEW_WAVES = 1024;                  // from so many words / 32 on, no sum is shared by wavefronts
 constexpr int AMAX_BLOCKS = 256;
+// Pairs of fp16 numbers carry a matrix with one power of two, which brings its largest entry to [2^14, 2^15): a value is
+// off by 2^-23 of itself or, since fp16 ends in steps of 2^-24, by 2^-39 of that largest entry.  A row whose own largest
+// entry is at least 2^-16 of it thus keeps 2^-23 of its largest entry, as it would with a power of two of its own.  Where
+// a row that is not zero lies below that (a word far larger than the others but masked, say), x, W and G stay in fp32 and
+// the products take the fp32 matrix instruction (10240 x 10000 x 512, loss and gradients: 1.4 -> 7.7 ms).  Found on the
+// device, in the pass that takes the maxima; the kernels hold both forms.
+constexpr float FAR = 65536.f;
 
 // dx has as many row tiles as there are counted rows, which only the device knows: the number of parts for each possible
 // number of row tiles goes along (one part beyond 64 of them, 16384 rows, where there are tiles enough).
@@ -140,7 +148,7 @@ bool make_plan(const capdec_vocab_ce* a, Plan& p) {
     p.z_words = p.few_z ? Mid::BI : p.wide_z ? Wide::BI : Big::BI;
     p.z_rows = p.few_z ? Mid::BJ : p.wide_z ? Wide::BJ : Big::BJ;
     p.o_part = take(at, (size_t)(p.Vp / p.z_words) * p.Mp * 8);
-    p.o_amax = take(at, 2 * AMAX_BLOCKS * 4);
+    p.o_amax = take(at, 2 * AMAX_BLOCKS * 8);
     p.fwd = at;
 
     const int es = p.split ? 4 : 2;
@@ -184,6 +192,7 @@ bool make_plan(const capdec_vocab_ce* a, Plan& p) {
 struct Head {               // first 256 bytes of the saved buffer
     int count;              // rows with a counted target
     int ex, ew;             // split operands: x and W are packed times 2^ex and 2^ew
+    int far;                // fp32 operands that are multiplied as they are; the packed x is fp32 then, W is not packed
 };
 struct BwdHead {            // first 256 bytes of the backward workspace (upstream gradients of the rows)
     float factor;           // what dx, dW and db are to be multiplied by
@@ -222,7 +231,7 @@ struct ScanArgs {
     const float* x; int64_t ldx;          // split operands: also the largest finite magnitudes of x (counted rows) and W
     const float* W; int64_t ldw;
     int nparts, vec;
-    float* part;                          // [2][AMAX_BLOCKS]
+    float2* part;                         // [2][AMAX_BLOCKS]: largest magnitude; that of the row where it is least
 };
 
 // The first workgroup compacts the rows: stable, 4096 targets per round.
@@ -271,20 +280,17 @@ __device__ void compact(const ScanArgs& a) {
     }
     if (threadIdx.x == 0) {
         a.head->count = done;
-        a.head->ex = a.head->ew = 0;
+        a.head->ex = a.head->ew = a.head->far = 0;
     }
 }
 
-// The others take the maxima, one partial each: a wavefront reads four rows at a time.
+// The others take the maxima, one partial each: a wavefront reads four rows at a time.  Beside the largest magnitude the
+// least of the rows' own (of rows that are not zero).
 __device__ void partial_max(const ScanArgs& a, int block) {
     const bool isw = block >= a.nparts;
     const int rows = isw ? a.V : a.M, nw = a.nparts * 16;
-    float m = 0.f;
+    float top = 0.f, least = INFINITY;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    auto see = [&](float v) {
-        v = fabsf(v);
-        if (v < INFINITY) m = fmaxf(m, v);
-    };
     for (int r = (block - (isw ? a.nparts : 0)) * 16 + wave; r < rows; r += 4 * nw) {
         const float* row[4];
         bool use[4];
@@ -294,6 +300,11 @@ __device__ void partial_max(const ScanArgs& a, int block) {
             use[k] = isw || a.targets[q] != a.ignore;
             row[k] = isw ? a.W + (int64_t)q * a.ldw : a.x + (int64_t)q * a.ldx;
         }
+        float m[4] = {0.f, 0.f, 0.f, 0.f};
+        auto see = [&](int k, float v) {
+            v = fabsf(v);
+            if (v < INFINITY) m[k] = fmaxf(m[k], v);
+        };
         if (a.vec) {
             for (int c = lane * 4; c < a.K; c += 256) {
                 f32x4 v[4] = {};
@@ -303,23 +314,31 @@ __device__ void partial_max(const ScanArgs& a, int block) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) see(v[k][e]);
+                    for (int e = 0; e < 4; ++e) see(k, v[k][e]);
             }
         } else {
             for (int c = lane; c < a.K; c += 64) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (use[k]) see(row[k][c]);
+                    if (use[k]) see(k, row[k][c]);
             }
         }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            m[k] = wave_max(m[k]);
+            top = fmaxf(top, m[k]);
+            if (m[k] > 0.f) least = fminf(least, m[k]);
+        }
     }
-    m = wave_max(m);
-    __shared__ float wm[16];
-    if (lane == 0) wm[wave] = m;
+    __shared__ float2 wm[16];
+    if (lane == 0) wm[wave] = make_float2(top, least);
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) m = fmaxf(m, wm[w]);
-        a.part[(isw ? AMAX_BLOCKS - a.nparts : 0) + block] = m;
+        for (int w = 1; w < 16; ++w) {
+            top = fmaxf(top, wm[w].x);
+            least = fminf(least, wm[w].y);
+        }
+        a.part[(isw ? AMAX_BLOCKS - a.nparts : 0) + block] = make_float2(top, least);
     }
 }
 
@@ -339,7 +358,7 @@ struct PackArgs {
     const int* order;
     short* px; short* pw; float* b2;
     int64_t nx, nw;           // 8-column chunks of x and W
-    const float* part;        // split operands: the partial maxima
+    const float2* part;       // split operands: the partial maxima
     int nparts;
 };
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
@@ -347,27 +366,34 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     const int cpr = a.Kp / 8;
     const int count = a.head->count;
     int scale[2] = {0, 0};
+    bool far = false;
     if (a.split) {                                  // every block joins the partial maxima for itself; the first notes them
-        __shared__ float wm[2][4];
-        float m[2] = {0.f, 0.f};
+        __shared__ float wm[4][4];
+        float m[4] = {0.f, 0.f, INFINITY, INFINITY};
         for (int k = threadIdx.x; k < a.nparts; k += 256) {
-            m[0] = fmaxf(m[0], a.part[k]);
-            m[1] = fmaxf(m[1], a.part[AMAX_BLOCKS + k]);
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+                const float2 v = a.part[o * AMAX_BLOCKS + k];
+                m[o] = fmaxf(m[o], v.x);
+                m[2 + o] = fminf(m[2 + o], v.y);
+            }
         }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            m[k] = wave_max(m[k]);
+        for (int k = 0; k < 4; ++k) {
+            m[k] = k < 2 ? wave_max(m[k]) : -wave_max(-m[k]);
             if ((threadIdx.x & 63) == 0) wm[k][threadIdx.x >> 6] = m[k];
         }
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            m[k] = fmaxf(fmaxf(wm[k][0], wm[k][1]), fmaxf(wm[k][2], wm[k][3]));
-            scale[k] = scale_exp(m[k]);
-        }
+        for (int k = 0; k < 4; ++k)
+            m[k] = k < 2 ? fmaxf(fmaxf(wm[k][0], wm[k][1]), fmaxf(wm[k][2], wm[k][3]))
+                         : fminf(fminf(wm[k][0], wm[k][1]), fminf(wm[k][2], wm[k][3]));
+        far = m[2] * FAR < m[0] || m[3] * FAR < m[1];
+        if (!far) scale[0] = scale_exp(m[0]), scale[1] = scale_exp(m[1]);
         if (blockIdx.x == 0 && threadIdx.x == 0) {
             a.head->ex = scale[0];
             a.head->ew = scale[1];
+            a.head->far = far;
         }
     }
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
@@ -377,6 +403,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
             continue;
         }
         const bool isw = t >= a.nx;
+        if (isw && far) continue;
         const int64_t u = isw ? t - a.nx : t;
         const int row = (int)(u / cpr), c = (int)(u - (int64_t)row * cpr) * 8;
         if (!isw && row >= ((count + 31) & ~31)) continue;
@@ -394,7 +421,6 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
             }
             *reinterpret_cast<s16x8*>(dst + c) = o;
         } else {
-            const int s = scale[isw];
             float v[8];
             if (!zero && a.vec && c + 8 <= a.K) {
                 const f32x4* q = reinterpret_cast<const f32x4*>((const float*)src + base + c);
@@ -405,6 +431,13 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = (!zero && c + e < a.K) ? ((const float*)src)[base + c + e] : 0.f;
             }
+            if (far) {
+                f32x4* d = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(dst) + c);
+                d[0] = f32x4{v[0], v[1], v[2], v[3]};
+                d[1] = f32x4{v[4], v[5], v[6], v[7]};
+                continue;
+            }
+            const int s = scale[isw];
             s16x8 hi, lo;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -485,6 +518,8 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a, RowScales f)
 // ---- (max, sum of exp) of every row over each tile of 256 words; values in units of log 2 ---------------------------
 struct LogitArgs {
     View W, X;
+    View32 W32, X32;                             // split operands: the fp32 ones
+    int K;
     const float* b2;
     const Head* head;
     int kt, Mp;
@@ -506,6 +541,15 @@ __device__ __forceinline__ float logit_scale(const Head* head) {
     return SPLIT ? ldexpf(L2E, -(head->ex + head->ew)) : L2E;
 }
 
+// the logits of a tile times logit_scale() (or the rows' scales)
+template <class C, int ELT, bool SPLIT>
+__device__ __forceinline__ void logits(const LogitArgs& a, bool far, int i0, int j0, short* lds, f32x16 (&acc)[C::TI][C::TJ]) {
+    if (SPLIT && far) {
+        const View32 x{a.X32.p, a.X32.ld, a.X32.order, a.head->count};
+        contract32<C, false, false>(a.W32, x, i0, j0, 0, a.K, a.K, lds, acc);
+    } else contract<C, ELT, false, false, SPLIT>(a.W, a.X, i0, j0, 0, a.kt, lds, acc);
+}
+
 template <class C, int ELT, bool SPLIT, bool BY_ROW>
 __global__ __launch_bounds__(C::THREADS, C::EU) void lse_kernel(LogitArgs a) {
     extern __shared__ __attribute__((aligned(16))) short lds[];
@@ -522,13 +566,15 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void lse_kernel(LogitArgs a) {
         at[tj] = slot < count ? a.tgt[slot] - i0 - wi * C::TI * 32 : -1;
     }
     f32x16 acc[C::TI][C::TJ];
-    contract<C, ELT, false, false, SPLIT>(a.W, a.X, i0, j0, 0, a.kt, lds, acc);
+    const bool far = SPLIT && a.head->far;
+    logits<C, ELT, SPLIT>(a, far, i0, j0, lds, acc);
     const float c0 = logit_scale<SPLIT>(a.head);
     float2* red = reinterpret_cast<float2*>(lds);
 #pragma unroll
     for (int tj = 0; tj < C::TJ; ++tj) {
         float m = -INFINITY;
-        const float c1 = BY_ROW ? a.f.x[j0 + (wj * C::TJ + tj) * 32 + (lane & 31)] : c0;
+        float c1 = c0;
+        if (BY_ROW) c1 = far ? 1.f : a.f.x[j0 + (wj * C::TJ + tj) * 32 + (lane & 31)];
 #pragma unroll
         for (int ti = 0; ti < C::TI; ++ti)
 #pragma unroll
@@ -536,8 +582,11 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void lse_kernel(LogitArgs a) {
                 const int word = i0 + (wi * C::TI + ti) * 32 + 8 * q + 4 * h;
                 const f32x4 b = *reinterpret_cast<const f32x4*>(a.b2 + word);
                 f32x4 c = {c1, c1, c1, c1};
-                // (the two powers first: one alone may be denormal, which would round its product with L2E)
-                if (BY_ROW) c = c * *reinterpret_cast<const f32x4*>(a.f.w + word) * L2E;
+                if (BY_ROW) {          // (the two powers first: one alone may be denormal, which would round its product with L2E)
+                    const f32x4 f = *reinterpret_cast<const f32x4*>(a.f.w + word);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c[e] = c[e] * (far ? 1.f : f[e]) * L2E;
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float v = fmaf(acc[ti][tj][4 * q + e], c[e], b[e]);
@@ -675,7 +724,8 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void dlogits_kernel(LogitArgs a)
     const int i0 = a.v0 + ti_ * C::BI, j0 = tj_ * C::BJ;
     if (j0 >= count) return;
     f32x16 acc[C::TI][C::TJ];
-    contract<C, ELT, false, false, SPLIT>(a.W, a.X, i0, j0, 0, a.kt, lds, acc);
+    const bool far = SPLIT && a.head->far;
+    logits<C, ELT, SPLIT>(a, far, i0, j0, lds, acc);
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));       // the addresses below are made here, not ahead of the contraction (72 spills)
     const int lane = tid & 63, wave = tid >> 6, wi = wave / C::WJ, wj = wave % C::WJ, h = lane >> 5;
@@ -684,107 +734,121 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void dlogits_kernel(LogitArgs a)
     constexpr int PL = SPLIT ? 2 : 1;
     constexpr int LOW = SPLIT ? 16 : WORDS;               // from a value to its low part
     constexpr int LD = WORDS * 2 + 8;                     // 16-bit elements per row of the turned tile: G, and its low parts
-    // one 32-row block of the wavefront at a time
-    short* tile = lds + wave * 32 * LD;
-    float* colsum = reinterpret_cast<float*>(lds + C::WAVES * 32 * LD);      // [WJ][BI]
-    float sums[2] = {0.f, 0.f};
+    auto finish = [&](auto as_fp32) {        // G in fp32, or in pairs or 16 bits: two copies of the code, no branches within
+        constexpr bool AS32 = decltype(as_fp32)::value;
+        // one 32-row block of the wavefront at a time
+        short* tile = lds + wave * 32 * LD;
+        float* colsum = reinterpret_cast<float*>(lds + C::WAVES * 32 * LD);      // [WJ][BI]
+        float sums[2] = {0.f, 0.f};
 #pragma unroll
-    for (int tj = 0; tj < C::TJ; ++tj) {
-        const int s = j0 + (wj * C::TJ + tj) * 32 + (lane & 31);
-        const bool live = s < count;
-        const float l2 = live ? a.lse[s] : 0.f;
-        const float w = live ? (a.rw ? a.rw[s] : pow2(G_EXP)) : 0.f;
-        const float* b2 = a.b2 + i0 + wi * WORDS;
+        for (int tj = 0; tj < C::TJ; ++tj) {
+            const int s = j0 + (wj * C::TJ + tj) * 32 + (lane & 31);
+            const bool live = s < count;
+            const float l2 = live ? a.lse[s] : 0.f;
+            const float w = live ? (a.rw ? a.rw[s] : pow2(G_EXP)) : 0.f;
+            const float* b2 = a.b2 + i0 + wi * WORDS;
 #pragma unroll
-        for (int ti = 0; ti < C::TI; ++ti) {
+            for (int ti = 0; ti < C::TI; ++ti) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int wd = ti * 32 + 8 * q + 4 * h;       // word inside the wavefront's range
-                const f32x4 b = *reinterpret_cast<const f32x4*>(b2 + wd);
-                s16x4 hi, lo;
+                for (int q = 0; q < 4; ++q) {
+                    const int wd = ti * 32 + 8 * q + 4 * h;       // word inside the wavefront's range
+                    const f32x4 b = *reinterpret_cast<const f32x4*>(b2 + wd);
+                    s16x4 hi, lo;
+                    f32x4 full;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v = __builtin_amdgcn_exp2f(fmaf(acc[ti][tj][4 * q + e], c1, b[e]) - l2) * w;
-                    if (!live) v = 0.f;
-                    if (SPLIT) {
+                    for (int e = 0; e < 4; ++e) {
+                        float v = __builtin_amdgcn_exp2f(fmaf(acc[ti][tj][4 * q + e], c1, b[e]) - l2) * w;
+                        if (!live) v = 0.f;
+                        full[e] = v;
+                        if (SPLIT) {
+                            short p, r;
+                            split16(v, p, r);
+                            hi[e] = p;
+                            lo[e] = r;
+                        } else {
+                            asm("" : "+v"(v));
+                            hi[e] = to_bits<ELT>(v);
+                            lo[e] = to_bits<ELT>(v - from_bits<ELT>(hi[e]));
+                        }
+                    }
+                    if (AS32) {
+                        *reinterpret_cast<f32x4*>(tile + (lane & 31) * LD + 2 * wd) = full;
+                        continue;
+                    }
+                    short* d = tile + (lane & 31) * LD + (SPLIT ? (int)split_col(wd) : wd);
+                    *reinterpret_cast<s16x4*>(d) = hi;
+                    if (SPLIT || a.dbp) *reinterpret_cast<s16x4*>(d + LOW) = lo;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // (the tile belongs to this wavefront alone: LDS operations of a wavefront complete in order)
+            // What rounding takes off a target's entry, usually its row's largest by far, is kept: dx gets it back, and dW of
+            // a batch too small for such errors to average out.
+            if (h == 0 && live) {
+                const int t = a.tgt[s] - (i0 + wi * WORDS);
+                if (t >= 0 && t < WORDS) {
+                    float v = expm1f(a.dlt[s]) * w;
+                    asm("" : "+v"(v));
+                    short* d = tile + lane * LD + (SPLIT ? (int)split_col(t) : t);
+                    if (AS32) {
+                        *reinterpret_cast<float*>(tile + lane * LD + 2 * t) = v;
+                    } else if (SPLIT) {
                         short p, r;
                         split16(v, p, r);
-                        hi[e] = p;
-                        lo[e] = r;
+                        d[0] = p;
+                        d[16] = r;
                     } else {
-                        asm("" : "+v"(v));
-                        hi[e] = to_bits<ELT>(v);
-                        lo[e] = to_bits<ELT>(v - from_bits<ELT>(hi[e]));
+                        const short q = to_bits<ELT>(v);
+                        const float rest = v - from_bits<ELT>(q);
+                        d[0] = q;
+                        d[LOW] = to_bits<ELT>(rest);
+                        a.rest[s] = rest;
                     }
                 }
-                short* d = tile + (lane & 31) * LD + (SPLIT ? (int)split_col(wd) : wd);
-                *reinterpret_cast<s16x4*>(d) = hi;
-                if (SPLIT || a.dbp) *reinterpret_cast<s16x4*>(d + LOW) = lo;
             }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        // (the tile belongs to this wavefront alone: LDS operations of a wavefront complete in order)
-        // What rounding takes off a target's entry, usually its row's largest by far, is kept: dx gets it back, and dW of
-        // a batch too small for such errors to average out.
-        if (h == 0 && live) {
-            const int t = a.tgt[s] - (i0 + wi * WORDS);
-            if (t >= 0 && t < WORDS) {
-                float v = expm1f(a.dlt[s]) * w;
-                asm("" : "+v"(v));
-                short* d = tile + lane * LD + (SPLIT ? (int)split_col(t) : t);
-                if (SPLIT) {
-                    short p, r;
-                    split16(v, p, r);
-                    d[0] = p;
-                    d[16] = r;
-                } else {
-                    const short q = to_bits<ELT>(v);
-                    const float rest = v - from_bits<ELT>(q);
-                    d[0] = q;
-                    d[LOW] = to_bits<ELT>(rest);
-                    a.rest[s] = rest;
+            __builtin_amdgcn_wave_barrier();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            constexpr int CH = WORDS * PL / 8;                     // 16-byte chunks per row
+            constexpr int RPP = 64 / CH;                           // rows per pass
+            static_assert(64 % CH == 0, "row does not divide over the wavefront");
+            const int row0 = j0 + (wj * C::TJ + tj) * 32;
+            short* gp = a.g + (int64_t)(ti_ * C::BI + wi * WORDS) * PL;
+#pragma unroll 4
+            for (int r = lane / CH; r < 32; r += RPP) {
+                const s16x8 v = *reinterpret_cast<const s16x8*>(tile + r * LD + (lane % CH) * 8);
+                *reinterpret_cast<s16x8*>(gp + (int64_t)(row0 + r) * a.ldg + (lane % CH) * 8) = v;
+            }
+            if (a.dbp) {
+#pragma unroll
+                for (int k = 0; k < WORDS / 64; ++k) {
+                    const int wd = lane + 64 * k;
+                    const short* d = tile + (SPLIT ? (int)split_col(wd) : wd);
+                    float sum = 0.f;
+#pragma unroll 8
+                    for (int r = 0; r < 32; ++r) {
+                        sum += AS32 ? *reinterpret_cast<const float*>(tile + r * LD + 2 * wd)
+                                            : from_bits<ELT>(d[r * LD]) + from_bits<ELT>(d[r * LD + LOW]);
+                    }
+                    sums[k] += sum;
                 }
             }
-        }
-        __builtin_amdgcn_wave_barrier();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        constexpr int CH = WORDS * PL / 8;                     // 16-byte chunks per row
-        constexpr int RPP = 64 / CH;                           // rows per pass
-        static_assert(64 % CH == 0, "row does not divide over the wavefront");
-        const int row0 = j0 + (wj * C::TJ + tj) * 32;
-        short* gp = a.g + (int64_t)(ti_ * C::BI + wi * WORDS) * PL;
-#pragma unroll 4
-        for (int r = lane / CH; r < 32; r += RPP) {
-            const s16x8 v = *reinterpret_cast<const s16x8*>(tile + r * LD + (lane % CH) * 8);
-            *reinterpret_cast<s16x8*>(gp + (int64_t)(row0 + r) * a.ldg + (lane % CH) * 8) = v;
+            __builtin_amdgcn_wave_barrier();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
         if (a.dbp) {
 #pragma unroll
-            for (int k = 0; k < WORDS / 64; ++k) {
-                const int wd = lane + 64 * k;
-                const short* d = tile + (SPLIT ? (int)split_col(wd) : wd);
+            for (int k = 0; k < WORDS / 64; ++k) colsum[wj * C::BI + wi * WORDS + lane + 64 * k] = sums[k];
+            __syncthreads();
+            for (int i = threadIdx.x; i < C::BI; i += C::THREADS) {
                 float sum = 0.f;
-#pragma unroll 8
-                for (int r = 0; r < 32; ++r) {
-                    sum += from_bits<ELT>(d[r * LD]) + from_bits<ELT>(d[r * LD + LOW]);
-                }
-                sums[k] += sum;
+#pragma unroll
+                for (int w = 0; w < C::WJ; ++w) sum += colsum[w * C::BI + i];
+                a.dbp[(int64_t)tj_ * a.piece + ti_ * C::BI + i] = sum;
             }
         }
-        __builtin_amdgcn_wave_barrier();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
-    if (a.dbp) {
-#pragma unroll
-        for (int k = 0; k < WORDS / 64; ++k) colsum[wj * C::BI + wi * WORDS + lane + 64 * k] = sums[k];
-        __syncthreads();
-        for (int i = threadIdx.x; i < C::BI; i += C::THREADS) {
-            float sum = 0.f;
-#pragma unroll
-            for (int w = 0; w < C::WJ; ++w) sum += colsum[w * C::BI + i];
-            a.dbp[(int64_t)tj_ * a.piece + ti_ * C::BI + i] = sum;
-        }
-    }
+    };
+    if (SPLIT && far) finish(std::integral_constant<bool, SPLIT>{});
+    else finish(std::false_type{});
 }
 
 // dx and dW of one piece.  OUT 0: fp32 partial sums [split][i][j], added onto what earlier pieces left when `add`;
@@ -792,6 +856,8 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void dlogits_kernel(LogitArgs a)
 constexpr int REST_ROWS = 64;
 struct GradArgs {
     View P, Q;
+    View32 P32, Q32;               // split operands: the fp32 ones
+    int k32;                       // dx: words of the piece that exist
     const Head* head;
     Upstream up;
     int I, J;                      // rows and columns stored
@@ -828,7 +894,9 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void grad_kernel(GradArgs a) {
     const int kt = a.k_live ? (count + KT - 1) / KT : a.kt;
     const int per = (kt + a.nsplit - 1) / a.nsplit;
     f32x16 acc[C::TI][C::TJ];
-    contract<C, ELT, TP, true, SPLIT>(a.P, a.Q, i0, j0, z * per, min(kt, (z + 1) * per), lds, acc);
+    const int kt1 = min(kt, (z + 1) * per);
+    if (SPLIT && a.head->far) contract32<C, TP, true>(a.P32, a.Q32, i0, j0, z * per * KT, kt1 * KT, a.k_live ? count : a.k32, lds, acc);
+    else contract<C, ELT, TP, true, SPLIT>(a.P, a.Q, i0, j0, z * per, kt1, lds, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave / C::WJ, wj = wave % C::WJ, h = lane >> 5;
     if (TP && !SPLIT && z == 0 && count <= REST_ROWS) {
         // row m adds rest[m] x[m] to its target's row of dW
@@ -1375,7 +1443,7 @@ int capdec_vocab_ce_forward(const capdec_vocab_ce* a, void* saved, size_t saved_
     }
     PackArgs k{};
     ScanArgs sc{a->targets, p.M, p.V, p.K, a->ignore_index, head, order, slot, tgt, (const float*)a->x, a->ldx, (const float*)a->W,
-                a->ldw, 0, vec && p.K % 4 == 0, (float*)((char*)workspace + p.o_amax)};
+                a->ldw, 0, vec && p.K % 4 == 0, (float2*)((char*)workspace + p.o_amax)};
     if (p.split && !p.by_row) sc.nparts = (int)blocks_for((int64_t)(p.V > p.M ? p.V : p.M), 16, AMAX_BLOCKS);
     scan_kernel<<<1 + 2 * sc.nparts, 1024, 0, s>>>(sc);
     k.nparts = sc.nparts;
@@ -1399,6 +1467,11 @@ int capdec_vocab_ce_forward(const capdec_vocab_ce* a, void* saved, size_t saved_
     LogitArgs g{};
     g.W = View{p.pack_w ? k.pw : (const short*)a->W, p.pack_w ? (int64_t)p.xs : a->ldw, p.V, 0};
     g.X = View{k.px, (int64_t)p.xs, p.Mp, 0};
+    if (p.split) {
+        g.W32 = View32{(const float*)a->W, a->ldw, nullptr, p.V};
+        g.X32 = View32{(const float*)a->x, a->ldx, order, 0};              // (as many rows as are counted)
+        g.K = p.K;
+    }
     g.b2 = k.b2; g.head = head; g.kt = p.xs / 32; g.Mp = p.Mp;
     g.part = (float2*)((char*)workspace + p.o_part);
     g.tgt = tgt; g.zt = (float*)(sv + p.o_dlt);
@@ -1467,6 +1540,11 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
         LogitArgs g{};
         g.W = View{W, ldw, p.V, 0};
         g.X = View{px, (int64_t)p.xs, p.Mp, 0};
+        if (p.split) {
+            g.W32 = View32{(const float*)a->W, a->ldw, nullptr, p.V};
+            g.X32 = View32{(const float*)px, p.Kp, nullptr, 0};
+            g.K = p.K;
+        }
         g.b2 = (const float*)(sv + p.o_b2); g.head = head; g.kt = p.xs / 32; g.Mp = p.Mp;
         g.lse = (const float*)(sv + p.o_lse); g.dlt = (const float*)(sv + p.o_dlt); g.rw = rw; g.tgt = (const int*)(sv + p.o_tgt);
         g.g = G; g.ldg = (int64_t)p.piece * pl; g.rest = rest; g.dbp = dbias ? (float*)(ws + p.o_db) : nullptr; g.v0 = v0; g.piece = p.piece;
@@ -1480,6 +1558,11 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
             GradArgs d{};
             d.P = View{G, g.ldg, p.Mp, 0};
             d.Q = View{W + (int64_t)v0 * ldw, ldw, p.Kp, real};
+            if (p.split) {
+                d.P32 = View32{(const float*)G, p.piece, nullptr, p.Mp};
+                d.Q32 = View32{(const float*)a->W + (int64_t)v0 * a->ldw, a->ldw, nullptr, p.K};
+                d.k32 = real;
+            }
             d.head = head; d.up = up; d.I = p.Mp; d.J = p.Kp; d.rows_live = 1; d.kt = words / kt; d.splits = p.sx;
             d.part = dxp; d.ldp = p.Kp; d.add = v0 > 0;
 #define DX(E, S) (p.wide_dx ? launch_grad<Wide, E, false, S, 0>(d, p.Mp, p.Kp, p.dx_tiles, s) : launch_grad<Big, E, false, S, 0>(d, p.Mp, p.Kp, p.dx_tiles, s))
@@ -1490,6 +1573,10 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
             GradArgs d{};
             d.P = View{G, g.ldg, words, p.Mp};
             d.Q = View{px, (int64_t)p.xs, p.Kp, p.Mp};
+            if (p.split) {
+                d.P32 = View32{(const float*)G, p.piece, nullptr, words};
+                d.Q32 = View32{(const float*)px, p.Kp, nullptr, p.Kp};
+            }
             d.head = head; d.up = up; d.k_live = 1; d.nsplit = p.sw;
             d.tgt = g.tgt; d.rest = rest; d.v0 = v0;
             if (p.sw == 1) {

@@ -1,10 +1,16 @@
-"""The vocabulary cross entropy of float32 operands over fp32's range."""
+"""The vocabulary cross entropy of float32 operands over fp32's range: rows far apart, very small and large ones.
+
+Bounds are those of test_gpu_vocab_ce.definition, taken of the rows and words that count: a word whose bias is -inf, or a row
+whose upstream gradient is zero, is left out of the definition, since it enters nothing."""
 import pytest
 import torch
 
 from test_gpu_vocab_ce import definition, make, near, run
 
 pytestmark = pytest.mark.gpu
+
+# rows, words, width: with 128 x 128, 256 x 128 and 256 x 256 tiles of the logits, odd sizes, parts of the contractions
+SIZES = [(70, 1000, 64), (100, 500, 33), (200, 3000, 130), (700, 40000, 96), (1024, 13000, 1024), (1700, 16500, 768)]
 
 
 @pytest.mark.parametrize("scale", [(1e-30, 1), (1, 1e-30), (1e-30, 1e30), (1e30, 1e-30)])
@@ -22,3 +28,86 @@ def test_very_small_and_large_operands(M, scale):
         near(got, ref, bound, name, 2.0 ** -149)
     from capdec import functional as F
     near(F.vocab_cross_entropy(x, W, b, t, reduction="none"), nll, torch.full_like(nll, tn), "loss alone")
+
+
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("far", [1e6, 1e9, 1e30])
+def test_a_masked_word_far_larger_than_the_others(size, far):
+    """It may not cost the other words digits, with gradients as without."""
+    from capdec import functional as F
+    M, V, K = size
+    x, W, b, t = make(M, V, K, torch.float32, seed=61)
+    W[5] *= far
+    b[5] = float("-inf")
+    t[t == 5] = 6
+    keep = torch.arange(V, device="cuda") != 5
+    w = torch.rand(M, device="cuda") + 0.1
+    loss, (dx, dW, db) = run(x, W, b, t, "none", w)
+    (nll, *want), (tn, *tol) = definition(x, W[keep], b[keep], torch.where(t > 5, t - 1, t), w)
+    for got, ref, bound, name in zip((dx, dW[keep], db[keep]), want, tol, ("dx", "dW", "db")):
+        near(got, ref, bound, name)
+    assert int(dW[5].count_nonzero()) == 0 and float(db[5]) == 0.0
+    near(loss, nll, torch.full_like(nll, tn), "loss")
+    near(F.vocab_cross_entropy(x, W, b, t, reduction="none"), nll, torch.full_like(nll, tn), "loss alone")
+
+
+@pytest.mark.parametrize("size", SIZES)
+def test_rows_far_apart(size):
+    """Rows 1e-12 times the others, and one 1e9 times the others without an upstream gradient."""
+    M, V, K = size
+    x, W, b, t = make(M, V, K, torch.float32, seed=62)
+    x[1:4] *= 1e-12
+    t[1:4] = V - 1
+    x[7] *= 1e9
+    t[7] = 1
+    w = torch.rand(M, device="cuda") + 0.1
+    w[7] = 0.0
+    loss, (dx, dW, db) = run(x, W, b, t, "none", w)
+    keep = torch.arange(M, device="cuda") != 7
+    (nll, ref, *want), (tn, bound, *tol) = definition(x[keep], W, b, t[keep], w[keep])
+    near(loss[keep], nll, torch.full_like(nll, tn), "loss")
+    near(dx[keep], ref, bound, "dx")
+    assert int(dx[7].count_nonzero()) == 0
+    for got, r, bd, name in zip((dW, db), want, tol, ("dW", "db")):
+        near(got, r, bd, name)
+    # the small rows by their own sums of magnitudes: their logits are the bias
+    (nll, *_), (tn, *_) = definition(x[1:4], W, b, t[1:4], w[1:4])
+    near(loss[1:4], nll, torch.full_like(nll, tn), "loss of the small rows")
+
+
+def test_rows_far_apart_captured():
+    """One graph, replayed with operands that are far apart and with ones that are not."""
+    from capdec import ops
+    x, W, b, t = make(150, 900, 96, torch.float32, seed=63)
+    ins = [v.clone() for v in (x, W, b)]
+
+    def step():
+        _, loss, state = ops.vocab_ce_forward(*ins, t)
+        return (loss,) + ops.vocab_ce_backward(state)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for k in range(5):
+        for dst, src in zip(ins, make(150, 900, 96, torch.float32, seed=64 + k)):
+            dst.copy_(src)
+        if k % 2:
+            ins[1][17] *= 1e8
+            ins[2][17] = float("-inf")
+            t[t == 17] = 18
+        graph.replay()
+        got = [o.clone() for o in outs]
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, step())) and all(bool(p.isfinite().all()) for p in got)
+
+
+def test_zero_rows_are_not_far_apart():
+    """Rows of zeros (a padding word) leave the operands as pairs: the same bits as without them."""
+    x, W, b, t = make(100, 600, 64, torch.float32, seed=65, ignored=0.0, ignore=-1)
+    t[t >= 590] = 3
+    W[590:] = 0
+    b[590:] = float("-inf")
+    want = run(x, W[:590], b[:590], t, "sum", None, -1)
+    got = run(x, W, b, t, "sum", None, -1)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1][1][:590], want[1][1])
