@@ -70,12 +70,12 @@ def vocab_cross_entropy(x, weight, bias, targets, ignore_index=0, reduction="mea
     makes the loss NaN.  reduction: "mean" over the counted rows (NaN if there are none; the gradients are zero then),
     "sum", or "none" (a loss per target).  The loss is float32; gradients flow to x, weight and bias in their own type.
     float32 operands above 64 rows are taken as pairs of float16 numbers scaled by the largest of each matrix (each row where
-    nothing asks for a gradient): 22 bits, and steps of 2^-39 of that largest number.  Where the largest numbers of two rows
-    of x or of W (zeros aside) are more than 2^16 apart and a gradient is asked for, they are multiplied as they are, which
-    takes four to six times as long.
-    The gradient of the logits (a probability times a row's upstream gradient) is kept in the operands' own numbers: rounded to 16 bits for bfloat16 and
-    float16, as a pair for float32 above 64 rows; in float16 and pairs what lies below 2^-38 of the largest upstream
-    gradient is lost.
+    nothing asks for a gradient): 22 bits, and steps of 2^-39 of that largest number.  They are multiplied as they are, which
+    takes four to six times as long, where weight holds infinities and, if a gradient is asked for, where the largest numbers
+    of two rows of x or of weight (zeros aside) are more than 2^16 apart.
+    The gradient of the logits (a probability times a row's upstream gradient) is kept in the operands' own numbers: rounded
+    to 16 bits for bfloat16 and float16, as a pair for float32 above 64 rows; in float16 and pairs what lies below 2^-38 of
+    the largest upstream gradient is lost.
 
     There is no forward-mode derivative: an input that carries a tangent is refused.
 

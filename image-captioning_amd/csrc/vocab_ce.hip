@@ -31,9 +31,10 @@ constexpr int AMAX_BLOCKS = 256;
 // Pairs of fp16 numbers carry a matrix with one power of two, which brings its largest entry to [2^14, 2^15): a value is
 // off by 2^-23 of itself or, since fp16 ends in steps of 2^-24, by 2^-39 of that largest entry.  A row whose own largest
 // entry is at least 2^-16 of it thus keeps 2^-23 of its largest entry, as it would with a power of two of its own.  Where
-// a row that is not zero lies below that (a word far larger than the others but masked, say), x, W and G stay in fp32 and
-// the products take the fp32 matrix instruction (10240 x 10000 x 512, loss and gradients: 1.4 -> 7.7 ms).  Found on the
-// device, in the pass that takes the maxima; the kernels hold both forms.
+// a row that is not zero lies below that (a word far larger than the others but masked, say), or W holds infinities, whose
+// low part would be NaN (a logit of -inf is a number), x, W and G stay in fp32 and the products take the fp32 matrix
+// instruction (10240 x 10000 x 512, loss and gradients: 1.4 -> 7.7 ms).  Found on the device, in the pass that takes the
+// maxima; the kernels hold both forms.
 constexpr float FAR = 65536.f;
 
 // dx has as many row tiles as there are counted rows, which only the device knows: the number of parts for each possible
@@ -231,7 +232,7 @@ struct ScanArgs {
     const float* x; int64_t ldx;          // split operands: also the largest finite magnitudes of x (counted rows) and W
     const float* W; int64_t ldw;
     int nparts, vec;
-    float2* part;                         // [2][AMAX_BLOCKS]: largest magnitude; that of the row where it is least
+    float2* part;                         // [2][AMAX_BLOCKS]: largest magnitude; that of the row where it is least, or 0
 };
 
 // The first workgroup compacts the rows: stable, 4096 targets per round.
@@ -285,11 +286,13 @@ __device__ void compact(const ScanArgs& a) {
 }
 
 // The others take the maxima, one partial each: a wavefront reads four rows at a time.  Beside the largest magnitude the
-// least of the rows' own (of rows that are not zero).
+// least of the rows' own (of rows that are not zero), 0 once W has shown an infinity.  (An infinity of x needs no exact
+// products: its row's loss is not finite either way.)
 __device__ void partial_max(const ScanArgs& a, int block) {
     const bool isw = block >= a.nparts;
     const int rows = isw ? a.V : a.M, nw = a.nparts * 16;
     float top = 0.f, least = INFINITY;
+    bool inf = false;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int r = (block - (isw ? a.nparts : 0)) * 16 + wave; r < rows; r += 4 * nw) {
         const float* row[4];
@@ -304,6 +307,7 @@ __device__ void partial_max(const ScanArgs& a, int block) {
         auto see = [&](int k, float v) {
             v = fabsf(v);
             if (v < INFINITY) m[k] = fmaxf(m[k], v);
+            inf |= v == INFINITY;
         };
         if (a.vec) {
             for (int c = lane * 4; c < a.K; c += 256) {
@@ -330,6 +334,7 @@ __device__ void partial_max(const ScanArgs& a, int block) {
             if (m[k] > 0.f) least = fminf(least, m[k]);
         }
     }
+    if (isw && __any(inf)) least = 0.f;
     __shared__ float2 wm[16];
     if (lane == 0) wm[wave] = make_float2(top, least);
     __syncthreads();
@@ -469,9 +474,11 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a, RowScales f)
         const float* src = isw ? (const float*)a.W + (int64_t)row * a.ldw : (const float*)a.x + (int64_t)a.order[row] * a.ldx;
         short* dst = (isw ? a.pw : a.px) + (int64_t)row * a.xs;
         float m = 0.f;
+        bool inf = false;
         auto see = [&](float v) {
             v = fabsf(v);
             if (v < INFINITY) m = fmaxf(m, v);
+            inf |= v == INFINITY;
         };
         if (VEC) {
 #pragma unroll 2
@@ -487,6 +494,7 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a, RowScales f)
         m = wave_max(m);
         const int s = scale_exp(m);
         if (lane == 0) (isw ? f.w : f.x)[row] = pow2(-s);
+        if (isw && inf) a.head->far = 1;                               // (whoever says so says the same)
         for (int c = lane * 4; c < a.Kp; c += 256) {                   // four columns: halves of a group's hi and lo
             f32x4 v = {0.f, 0.f, 0.f, 0.f};
             if (VEC) {

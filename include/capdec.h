@@ -625,8 +625,8 @@ int capdec_satt_greedy_decode(const capdec_satt_model* m, const float* enc, cons
  * M and V rounded up to multiples of 256, M V <= 2^39 - 2^19.
  * 16-bit operands are multiplied as they are, the gradient of the logits is rounded to their type.  fp32 operands: M <= 64
  * as they are.  Above, as pairs of fp16 numbers with one power of two for x and one for W (loss_only: one for each row): 22
- * bits, in steps of 2^-39 of the largest magnitude of the matrix (row); without loss_only, where the largest magnitudes of
- * two rows of x or of W, zeros aside, are more than 2^16 apart, as they are.  The gradient of the logits is a pair then.  fp16
+ * bits, in steps of 2^-39 of the largest magnitude of the matrix (row); as they are where W holds infinities and, without
+ * loss_only, where the largest magnitudes of two rows of x or of W, zeros aside, are more than 2^16 apart.  The gradient of the logits is a pair then.  fp16
  * and pairs lose of it what is below 2^-38 of the largest upstream gradient.
  * `saved` (capdec_vocab_ce_saved_bytes) carries packed operands (for up to 64 rows of fp32: x and the logits) and row
  * statistics from the forward call to the backward call, which reads W again, but neither x, bias nor targets: neither W

@@ -111,3 +111,28 @@ def test_zero_rows_are_not_far_apart():
     want = run(x, W[:590], b[:590], t, "sum", None, -1)
     got = run(x, W, b, t, "sum", None, -1)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1][1][:590], want[1][1])
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,V,K", [(20, 700, 64), (100, 700, 64), (300, 9000, 800)])
+def test_a_word_of_infinite_distance(M, V, K, dt):
+    """A weight of -inf against positive entries of x: the word's logits are -inf, the others as if it were not there.  In
+    dx its column is 0 * inf."""
+    from capdec import functional as F
+    x, W, b, t = make(M, V, K, dt, seed=66)
+    x[:, 3] = x[:, 3].abs() + 0.5
+    W[5, 3] = float("-inf")
+    t[t == 5] = 6
+    keep = torch.arange(V, device="cuda") != 5
+    w = torch.rand(M, device="cuda") + 0.1
+    loss, (dx, dW, db) = run(x, W, b, t, "none", w)
+    (nll, ref, *want), (tn, bound, *tol) = definition(x, W[keep], b[keep], torch.where(t > 5, t - 1, t), w)
+    sub = 2.0 ** -25 if dt == torch.float16 else 0.0
+    near(loss, nll, torch.full_like(nll, tn), "loss")
+    cols = torch.arange(K, device="cuda") != 3
+    near(dx[:, cols], ref[:, cols], bound[:, cols], "dx", sub)
+    assert bool(dx[t != 0, 3].isnan().all())
+    for got, r, bd, name in zip((dW, db), want, tol, ("dW", "db")):
+        near(got[keep], r, bd, name, sub)
+    assert int(dW[5].count_nonzero()) == 0
+    near(F.vocab_cross_entropy(x, W, b, t, reduction="none"), nll, torch.full_like(nll, tn), "loss alone")
