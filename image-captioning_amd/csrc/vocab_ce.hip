@@ -9,8 +9,8 @@
 // loss and gradients, bound by the matrix cores at large sizes and by reading W at few rows.
 // fp32 operands are split into two fp16 numbers (mma16.h), but for batches of at most 64 rows, which have kernels of their
 // own that read W as it is, and for rows too far apart (FAR below); 16-bit operands are multiplied as they are.  Sums, softmax
-// statistics and the partial sums of the gradients are fp32.  G takes the operands' 16-bit type (scaled by 2^14, so
-// that probabilities down to 2^-28 stay normal in fp16).  That rounding averages out in sums over rows or words, except
+// statistics and the partial sums of the gradients are fp32.  G takes the operands' 16-bit type (fp16 scaled by 2^14,
+// so that probabilities down to 2^-28 stay normal).  That rounding averages out in sums over rows or words, except
 // at the targets, whose entries are near -g_r: what it takes off them is carried beside G and added to dx, and to dW up to
 // 64 rows, and db sums the unrounded values.  Against rounding of the results alone: dx and db 1.0, dW 1.0 - 1.3 times.
 // Every sum has a fixed order: results repeat bit for bit.
@@ -23,7 +23,7 @@ using namespace mma16;
 namespace {
 
 constexpr float L2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-constexpr int G_EXP = 14;                        // G is stored times 2^14
+constexpr int G_EXP = 14;                        // G is stored times 2^14 where it is fp16 numbers, and as it is in fp32 and bf16
 constexpr size_t PIECE_BYTES = (size_t)512 << 20;
 constexpr int FEW = 64;                          // rows of fp32 up to which W is read as it is
 constexpr int FEW_WAVES = 1024;                  // from so many words / 32 on, no sum is shared by wavefronts
@@ -202,11 +202,12 @@ struct Upstream {           // where that factor comes from: a BwdHead, or one s
     const BwdHead* bh;
     const float* grad;
     int mean;
+    int gexp;               // G_EXP, or 0 where G is not fp16 numbers
 };
 __device__ __forceinline__ float factor_of(const Upstream& u, const Head* head) {
     if (u.bh) return u.bh->factor;
     if (head->count == 0) return 0.f;
-    return ldexpf((u.grad ? u.grad[0] : 1.f) / (u.mean ? (float)head->count : 1.f), -G_EXP);
+    return ldexpf((u.grad ? u.grad[0] : 1.f) / (u.mean ? (float)head->count : 1.f), head->far ? 0 : -u.gexp);
 }
 
 // power of two that brings amax to [2^14, 2^15), denormal numbers below it (-113 .. 141, more than one fp32 number holds)
@@ -542,6 +543,7 @@ struct LogitArgs {
     float* dbp;                                  // [row tile][word of the piece], nullable
     float* rest;                                 // [slot] what rounding took off the target's entry (16-bit operands)
     int v0, piece;
+    int gexp;
 };
 
 template <bool SPLIT>
@@ -696,11 +698,11 @@ __global__ __launch_bounds__(1024) void loss_kernel(const float* __restrict__ nl
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------
-// The rows' own upstream gradients, brought to [2^13, 2^14] at most by a power of two, and the factor that undoes it.  (One
-// scalar for all rows needs no kernel: G is stored times 2^14, and factor_of() has the rest.)
+// The rows' own upstream gradients, brought to [2^(gexp - 1), 2^gexp] at most by a power of two, and the factor that undoes
+// it.  (One scalar for all rows needs no kernel: G is stored times 2^gexp, and factor_of() has the rest.)
 __global__ __launch_bounds__(1024) void weights_kernel(const float* __restrict__ row_grad, const Head* __restrict__ head,
-                                                       const int* __restrict__ order, int Mp, float* __restrict__ rw,
-                                                       BwdHead* __restrict__ bh) {
+                                                       const int* __restrict__ order, int Mp, int gexp,
+                                                       float* __restrict__ rw, BwdHead* __restrict__ bh) {
     const int count = head->count;
     __shared__ float wm[16];
     float m = 0.f;
@@ -713,9 +715,10 @@ __global__ __launch_bounds__(1024) void weights_kernel(const float* __restrict__
     __syncthreads();
     m = 0.f;
     for (int w = 0; w < 16; ++w) m = fmaxf(m, wm[w]);
-    // m * scale in [2^13, 2^14)
+    // m * scale in [2^(gexp - 1), 2^gexp)
+    if (head->far) gexp = 0;
     const int e = (int)(__float_as_uint(m) >> 23) - 127;
-    const float scale = m > 0.f ? pow2(min(G_EXP - 1 - e, 126)) : 1.f;
+    const float scale = m > 0.f ? pow2(min(gexp - 1 - e, 126)) : 1.f;
     for (int s = threadIdx.x; s < Mp; s += 1024) rw[s] = s < count ? row_grad[order[s]] * scale : 0.f;
     if (threadIdx.x == 0) bh->factor = count > 0 ? 1.f / scale : 0.f;
 }
@@ -753,7 +756,7 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void dlogits_kernel(LogitArgs a)
             const int s = j0 + (wj * C::TJ + tj) * 32 + (lane & 31);
             const bool live = s < count;
             const float l2 = live ? a.lse[s] : 0.f;
-            const float w = live ? (a.rw ? a.rw[s] : pow2(G_EXP)) : 0.f;
+            const float w = live ? (a.rw ? a.rw[s] : pow2(AS32 ? 0 : a.gexp)) : 0.f;
             const float* b2 = a.b2 + i0 + wi * WORDS;
 #pragma unroll
             for (int ti = 0; ti < C::TI; ++ti) {
@@ -1215,7 +1218,7 @@ __global__ __launch_bounds__(256) void few_g_kernel(FewGrad a) {
     for (int s = wave; s < a.rows; s += 4) {
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
         if (s < count) {
-            const float l2 = a.lse[s], f = a.rw ? a.rw[s] : pow2(G_EXP);
+            const float l2 = a.lse[s], f = a.rw ? a.rw[s] : 1.f;
             const int t = a.tgt[s] - w;
             const f32x4 z = *reinterpret_cast<const f32x4*>(a.z + (int64_t)s * a.Vp + w);
 #pragma unroll
@@ -1521,10 +1524,11 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
     const int* order = (const int*)(sv + p.o_order);
     const int* slot = (const int*)(sv + p.o_slot);
     float* rw = row_grad ? (float*)(ws + p.o_rw) : nullptr;
-    const Upstream up{row_grad ? (const BwdHead*)ws : nullptr, grad, mean};
+    const int gexp = p.few || (!p.split && p.elt == BF16) ? 0 : G_EXP;
+    const Upstream up{row_grad ? (const BwdHead*)ws : nullptr, grad, mean, gexp};
     float* rest = (float*)(ws + p.o_rest);
     if (row_grad) {
-        weights_kernel<<<1, 1024, 0, s>>>(row_grad, head, order, p.Mp, rw, (BwdHead*)ws);
+        weights_kernel<<<1, 1024, 0, s>>>(row_grad, head, order, p.Mp, gexp, rw, (BwdHead*)ws);
         CAPDEC_LAUNCH_CHECK();
     }
     if (p.few) {
@@ -1555,7 +1559,7 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a, const void* saved, size_t
         }
         g.b2 = (const float*)(sv + p.o_b2); g.head = head; g.kt = p.xs / 32; g.Mp = p.Mp;
         g.lse = (const float*)(sv + p.o_lse); g.dlt = (const float*)(sv + p.o_dlt); g.rw = rw; g.tgt = (const int*)(sv + p.o_tgt);
-        g.g = G; g.ldg = (int64_t)p.piece * pl; g.rest = rest; g.dbp = dbias ? (float*)(ws + p.o_db) : nullptr; g.v0 = v0; g.piece = p.piece;
+        g.g = G; g.ldg = (int64_t)p.piece * pl; g.rest = rest; g.dbp = dbias ? (float*)(ws + p.o_db) : nullptr; g.v0 = v0; g.piece = p.piece; g.gexp = gexp;
 #define DL(E, S)                                                   \
     (p.few_z    ? launch_dlogits<Mid, E, S>(g, words, p.Mp, s)     \
      : p.wide_z ? launch_dlogits<Wide, E, S>(g, words, p.Mp, s)    \

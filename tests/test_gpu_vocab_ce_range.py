@@ -136,3 +136,23 @@ def test_a_word_of_infinite_distance(M, V, K, dt):
         near(got[keep], r, bd, name, sub)
     assert int(dW[5].count_nonzero()) == 0
     near(F.vocab_cross_entropy(x, W, b, t, reduction="none"), nll, torch.full_like(nll, tn), "loss alone")
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("M,dt,far", [(40, torch.float32, False), (100, torch.float32, False), (100, torch.float32, True),
+                                      (100, torch.bfloat16, False)])
+def test_weights_near_the_end_of_the_range(M, dt, far, reduction):
+    """W up to 1e36 and more against an x of 1e-36: the gradient of the logits carries no factor that its products could overflow by
+    before it is undone."""
+    x, W, b, t = make(M, 300, 64, dt, seed=67)
+    x, W = (x.float() * 1e-36).to(dt), (W.float() * 1e36).to(dt)
+    if far:
+        W[7] = W[7] * 1e-30
+    w = torch.rand(M, device="cuda") + 0.1 if reduction == "none" else torch.full((M,), 1 / int((t != 0).sum()), device="cuda")
+    loss, grads = run(x, W, b, t, reduction, w if reduction == "none" else None)
+    (_, *want), (_, *tol) = definition(x, W, b, t, w)
+    assert bool(loss.isfinite().all())
+    near(grads[0], want[0], tol[0], "dx")
+    # x has fewer digits at its small end, and its products with G may leave the range: steps of 2^-149 each
+    near(grads[1], want[1], tol[1] + M * 2.0 ** -149, "dW", 2.0 ** -134 if dt == torch.bfloat16 else 0.0)
+    near(grads[2], want[2], tol[2], "db")
