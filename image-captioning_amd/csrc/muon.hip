@@ -7,8 +7,10 @@
 // from about 1000 x 1000 on, by launch and pipeline latency below.
 // The iterate, A and B are kept as pairs of fp16 numbers times a power of two (SPLIT in mma16.h) with fp32 sums: an error
 // made while r steps remain grows by up to a^r (3.4^r for the usual coefficients) in the directions whose singular
-// values are still small, so the early steps need all of fp32's digits whatever the matrices' type.  The powers of two
-// come from the exact maxima of the polynomials on the interval that the singular values can be in.
+// values are still small, so the steps need fp32's digits whatever the matrices' type.  (Single fp16 numbers in the last
+// two steps towards a bfloat16 result, a third of their products, made 1530 us of 1900 for 2048 x 8192, but left it up to
+// 3.2e-3 off in norm, depending on the spectrum, where rounding alone is 1.7e-3; in the last step alone, 2.2e-3.)  The
+// powers of two come from the exact maxima of the polynomials on the interval that the singular values can be in.
 #include "mma16.h"
 #include <math.h>
 
@@ -85,12 +87,11 @@ bool make_dims(int count, int rows, int cols, Dims& d) {
     d.norm = (size_t)d.batch * NORM_BLOCKS * 8;
     d.slab = 0;                           // the most that a product of this batch, or of the rest of the matrices, may take
     const int n = d.tall ? d.rp : d.cp, rest = count % d.batch ? count % d.batch : d.batch;
-    for (int kdiv = 16; kdiv <= 32; kdiv += 16)
-        for (int nz : {d.batch, rest})
-            for (int k : {n, d.m}) {
-                const size_t b = symmetric_plan(d.m, k / kdiv, nz).slab;
-                if (b > d.slab) d.slab = b;
-            }
+    for (int nz : {d.batch, rest})
+        for (int k : {n, d.m}) {
+            const size_t b = symmetric_plan(d.m, k / 16, nz).slab;
+            if (b > d.slab) d.slab = b;
+        }
     return true;
 }
 
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(256) void norm_kernel(Batch b, int rows, int cols, 
 // X_0 2^sx = U 2^sx / (|U| + eps) into the padded layout
 __global__ __launch_bounds__(256) void normalise_kernel(Batch b, int rows, int cols, int rp, int cp, int dtype, Momentum mo,
                                                         int vec, const double* __restrict__ part, int nparts, float eps,
-                                                        float scale, int split, short* __restrict__ X, int64_t x_elems) {
+                                                        float scale, short* __restrict__ X, int64_t x_elems) {
     const Item& it = b.it[blockIdx.y];
     double s = 0.0;
     for (int k = threadIdx.x & 63; k < nparts; k += 64) s += part[blockIdx.y * NORM_BLOCKS + k];
@@ -218,9 +219,9 @@ __global__ __launch_bounds__(256) void normalise_kernel(Batch b, int rows, int c
             hi[e] = h;
             lo[e] = l;
         }
-        short* d = x + (split ? (int64_t)r * cp * 2 + split_col(c) : (int64_t)r * cp + c);
+        short* d = x + (int64_t)r * cp * 2 + split_col(c);
         *reinterpret_cast<s16x8*>(d) = hi;
-        if (split) *reinterpret_cast<s16x8*>(d + 16) = lo;
+        *reinterpret_cast<s16x8*>(d + 16) = lo;
     }
 }
 
@@ -235,7 +236,7 @@ struct StepArgs {
     int tri;                       // symmetric result: only the tiles on and above the diagonal, mirrored as they are stored
     int nsplit; float* slab;       // contraction in parts: partial sums [matrix][part][tile][accumulator][thread]
     Map map;
-    short* out; int64_t ldo; int out_split;       // inner products
+    short* out; int64_t ldo;       // inner products
     // last product of the last step
     Batch b; int dtype;
     float lr, decay, scale;        // update: p <- p (1 - lr decay) - lr scale out
@@ -247,7 +248,7 @@ enum { INNER = 0, RESULT = 1, UPDATE = 2 };
 // sums added in order, then the epilogue; a workgroup per accumulator of a tile (blockIdx.y).
 enum { WHOLE = 0, PART = 1, JOIN = 2 };
 
-template <class C, bool TP, bool TQ, bool SPLIT, int OUT, int PHASE>
+template <class C, bool TP, bool TQ, int OUT, int PHASE>
 __global__ __launch_bounds__(C::THREADS, C::EU) void step_kernel(StepArgs a) {
     extern __shared__ __attribute__((aligned(16))) short lds[];
     int ti_, tj_, z;
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void step_kernel(StepArgs a) {
         P.p += mat * a.strideP;
         Q.p += mat * a.strideQ;
         const int part = z - mat * (PHASE == PART ? a.nsplit : 1), per = PHASE == PART ? (a.kt + a.nsplit - 1) / a.nsplit : a.kt;
-        contract<C, F16, TP, TQ, SPLIT>(P, Q, i0, j0, part * per, min(a.kt, (part + 1) * per), lds, acc);
+        contract<C, F16, TP, TQ, true>(P, Q, i0, j0, part * per, min(a.kt, (part + 1) * per), lds, acc);
         if (threadIdx.x >= C::GROUP) return;
     }
     int tid = threadIdx.x;
@@ -286,8 +287,7 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void step_kernel(StepArgs a) {
     auto finish = [&](int ti, int tj, const f32x16& sum) {
         const int j = j0 + (wj * C::TJ + tj) * 32 + (lane & 31), ib = i0 + (wi * C::TI + ti) * 32;
         if (j >= a.J) return;
-        const int64_t js = SPLIT ? split_col(j) : j;
-        const int64_t jo = a.out_split ? split_col(j) : j;
+        const int64_t js = split_col(j);
         float v[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = a.alpha * sum[e];
@@ -297,11 +297,11 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void step_kernel(StepArgs a) {
             for (int e = 0; e < 16; ++e) {
                 const short* q = R + (int64_t)min(ib + acc_row(e, h), a.I - 1) * a.ldr + js;
                 hi[e] = q[0];
-                lo[e] = SPLIT ? q[16] : (short)0;
+                lo[e] = q[16];
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-                v[e] = fmaf(a.beta, from_bits<F16>(hi[e]) + (SPLIT ? from_bits<F16>(lo[e]) : 0.f), v[e]);
+                v[e] = fmaf(a.beta, from_bits<F16>(hi[e]) + from_bits<F16>(lo[e]), v[e]);
         }
         if (OUT == INNER) {
             short* out = a.out + mat * a.strideO;
@@ -314,9 +314,9 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void step_kernel(StepArgs a) {
                 lo[e / 4][e % 4] = r;
                 const int i = ib + acc_row(e, h);
                 if (i >= a.I) continue;
-                short* d = out + (int64_t)i * a.ldo + jo;
+                short* d = out + (int64_t)i * a.ldo + js;
                 d[0] = p;
-                if (a.out_split) d[16] = r;
+                d[16] = r;
             }
             if (a.tri && ti_ != tj_) {
                 // row j of the mirrored tile: four neighbours at a time (I is a multiple of 32)
@@ -324,9 +324,9 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void step_kernel(StepArgs a) {
                 for (int q = 0; q < 4; ++q) {
                     const int i = ib + 8 * q + 4 * h;
                     if (i >= a.I) continue;
-                    short* d = out + (int64_t)j * a.ldo + (a.out_split ? split_col(i) : i);
+                    short* d = out + (int64_t)j * a.ldo + split_col(i);
                     *reinterpret_cast<s16x4*>(d) = hi[q];
-                    if (a.out_split) *reinterpret_cast<s16x4*>(d + 16) = lo[q];
+                    *reinterpret_cast<s16x4*>(d + 16) = lo[q];
                 }
             }
             return;
@@ -366,7 +366,7 @@ __global__ __launch_bounds__(C::THREADS, C::EU) void step_kernel(StepArgs a) {
     }
 }
 
-template <class C, bool TP, bool TQ, bool SPLIT, int OUT, int PHASE>
+template <class C, bool TP, bool TQ, int OUT, int PHASE>
 int launch(const StepArgs& a0, int nz, hipStream_t s) {
     StepArgs a = a0;
     int ni = (a.I + C::BI - 1) / C::BI, nj = (a.J + C::BJ - 1) / C::BJ;
@@ -377,44 +377,33 @@ int launch(const StepArgs& a0, int nz, hipStream_t s) {
     const unsigned grid = make_map(a.map, ni, nj, PHASE == PART ? nz * a.nsplit : nz);
     constexpr int bytes = PHASE == JOIN ? 0 : C::LDS_BYTES;
     if (bytes > 64 * 1024)
-        CAPDEC_TRY((int)hipFuncSetAttribute(reinterpret_cast<const void*>(step_kernel<C, TP, TQ, SPLIT, OUT, PHASE>),
+        CAPDEC_TRY((int)hipFuncSetAttribute(reinterpret_cast<const void*>(step_kernel<C, TP, TQ, OUT, PHASE>),
                                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    step_kernel<C, TP, TQ, SPLIT, OUT, PHASE><<<dim3(grid, PHASE == JOIN ? C::TI * C::TJ : 1), PHASE == JOIN ? C::GROUP : C::THREADS, bytes, s>>>(a);
+    step_kernel<C, TP, TQ, OUT, PHASE><<<dim3(grid, PHASE == JOIN ? C::TI * C::TJ : 1), PHASE == JOIN ? C::GROUP : C::THREADS, bytes, s>>>(a);
     CAPDEC_LAUNCH_CHECK();
     return 0;
 }
 
 // the largest tiles that give every CU one, from 256x256 to 64x64; fewer than two of those for each: four groups to a tile
-template <bool TP, bool TQ, bool SPLIT, int OUT>
+template <bool TP, bool TQ, int OUT>
 int launch_sized(const StepArgs& a, int nz, hipStream_t s) {
     auto tiles = [&](int bi, int bj) { return (int64_t)((a.I + bi - 1) / bi) * ((a.J + bj - 1) / bj) * nz; };
-    if (tiles(256, 256) >= 256) return launch<Wide, TP, TQ, SPLIT, OUT, WHOLE>(a, nz, s);
-    if (tiles(256, 128) >= 256) return launch<Big, TP, TQ, SPLIT, OUT, WHOLE>(a, nz, s);
-    if (tiles(128, 128) >= 256) return launch<Mid, TP, TQ, SPLIT, OUT, WHOLE>(a, nz, s);
-    if (tiles(64, 64) >= 512) return launch<Small, TP, TQ, SPLIT, OUT, WHOLE>(a, nz, s);
-    return launch<Deep, TP, TQ, SPLIT, OUT, WHOLE>(a, nz, s);
-}
-template <bool TP, bool TQ, int OUT>
-int launch_split(const StepArgs& a, bool split, int nz, hipStream_t s) {
-    return split ? launch_sized<TP, TQ, true, OUT>(a, nz, s) : launch_sized<TP, TQ, false, OUT>(a, nz, s);
+    if (tiles(256, 256) >= 256) return launch<Wide, TP, TQ, OUT, WHOLE>(a, nz, s);
+    if (tiles(256, 128) >= 256) return launch<Big, TP, TQ, OUT, WHOLE>(a, nz, s);
+    if (tiles(128, 128) >= 256) return launch<Mid, TP, TQ, OUT, WHOLE>(a, nz, s);
+    if (tiles(64, 64) >= 512) return launch<Small, TP, TQ, OUT, WHOLE>(a, nz, s);
+    return launch<Deep, TP, TQ, OUT, WHOLE>(a, nz, s);
 }
 
 // A symmetric product of a batch, into planes of the operands' layout.
 template <bool T>
-int launch_symmetric(StepArgs a, bool split, int nz, float* slab, hipStream_t s) {
+int launch_symmetric(StepArgs a, int nz, float* slab, hipStream_t s) {
     const Symmetric p = symmetric_plan(a.I, a.kt, nz);
     a.tri = p.on; a.nsplit = p.nsplit; a.slab = slab;
-#define SYM(S)                                                                                   \
-    if (!p.on) return launch_sized<T, T, S, INNER>(a, nz, s);                                    \
-    if (p.nsplit == 1)                                                                           \
-        return p.wide ? launch<Wide, T, T, S, INNER, WHOLE>(a, nz, s) : launch<Mid, T, T, S, INNER, WHOLE>(a, nz, s); \
-    CAPDEC_TRY((p.wide ? launch<Wide, T, T, S, INNER, PART>(a, nz, s) : launch<Mid, T, T, S, INNER, PART>(a, nz, s))); \
-    return p.wide ? launch<Wide, T, T, S, INNER, JOIN>(a, nz, s) : launch<Mid, T, T, S, INNER, JOIN>(a, nz, s);
-    if (split) {
-        SYM(true)
-    }
-    SYM(false)
-#undef SYM
+    if (!p.on) return launch_sized<T, T, INNER>(a, nz, s);
+    if (p.nsplit == 1) return p.wide ? launch<Wide, T, T, INNER, WHOLE>(a, nz, s) : launch<Mid, T, T, INNER, WHOLE>(a, nz, s);
+    CAPDEC_TRY((p.wide ? launch<Wide, T, T, INNER, PART>(a, nz, s) : launch<Mid, T, T, INNER, PART>(a, nz, s)));
+    return p.wide ? launch<Wide, T, T, INNER, JOIN>(a, nz, s) : launch<Mid, T, T, INNER, JOIN>(a, nz, s);
 }
 
 // Largest |p(x)| on [0, top] of a x + b x^3 + c x^5 (odd) or b x + c x^2: ends and stationary points.
@@ -452,7 +441,7 @@ int exponent_for(double top) {
 }
 
 struct Iteration {
-    int steps, exact_steps;                       // the first exact_steps keep two numbers per value
+    int steps;
     float a, b, c, eps;
 };
 
@@ -467,7 +456,6 @@ int run_batch(const Batch& b, int nz, const Dims& d, const Iteration& n, int dty
     float* slab = (float*)(B + (size_t)d.batch * d.a_elems);
     double sigma = 1.0;                           // bound of the iterate's singular values
     int sx = exponent_for(sigma);
-    bool split = n.exact_steps > 0;
     int vec = d.cols % 4 == 0;                    // every row of every matrix starts on four elements
     for (int z = 0; z < nz && vec; ++z) {
         const Item& it = b.it[z];
@@ -480,35 +468,33 @@ int run_batch(const Batch& b, int nz, const Dims& d, const Iteration& n, int dty
     const int64_t items = (int64_t)d.rp * (d.cp / 8);
     const unsigned blocks = (unsigned)(items / 256 + 1 < 1024 ? items / 256 + 1 : 1024);
     normalise_kernel<<<dim3(blocks, nz), 256, 0, s>>>(b, d.rows, d.cols, d.rp, d.cp, dtype, mo, vec, part, nparts, n.eps,
-                                                      ldexpf(1.f, sx), split, X[0], (int64_t)d.x_elems);
+                                                      ldexpf(1.f, sx), X[0], (int64_t)d.x_elems);
     CAPDEC_LAUNCH_CHECK();
     for (int k = 0; k < n.steps; ++k) {
-        const int pl = split ? 2 : 1, kdiv = split ? 16 : 32;
         const double lambda = sigma * sigma;
         const int sa = exponent_for(lambda), sb = exponent_for(top_of_poly(n.b, n.c, lambda));
-        const int64_t ldx = (int64_t)d.cp * pl, lda = (int64_t)d.m * pl;
+        const int64_t ldx = (int64_t)d.cp * 2, lda = (int64_t)d.m * 2;
         StepArgs g{};
         g.strideP = g.strideQ = (int64_t)d.x_elems;
         g.P = g.Q = View{X[k & 1], ldx, d.m, d.rp};
         g.alpha = ldexpf(1.f, sa - 2 * sx);
-        g.I = g.J = d.m; g.kt = (d.tall ? d.rp : d.cp) / kdiv;
-        g.out = A; g.ldo = lda; g.out_split = split; g.strideO = (int64_t)d.a_elems;
-        if (d.tall) CAPDEC_TRY(launch_symmetric<true>(g, split, nz, slab, s));
-        else CAPDEC_TRY(launch_symmetric<false>(g, split, nz, slab, s));
+        g.I = g.J = d.m; g.kt = (d.tall ? d.rp : d.cp) / 16;
+        g.out = A; g.ldo = lda; g.strideO = (int64_t)d.a_elems;
+        if (d.tall) CAPDEC_TRY(launch_symmetric<true>(g, nz, slab, s));
+        else CAPDEC_TRY(launch_symmetric<false>(g, nz, slab, s));
 
         g.strideP = g.strideQ = g.strideR = (int64_t)d.a_elems;
         g.P = g.Q = View{A, lda, d.m, d.m};
         g.R = A; g.ldr = lda;
         g.alpha = (float)ldexp((double)n.c, sb - 2 * sa);
         g.beta = (float)ldexp((double)n.b, sb - sa);
-        g.kt = d.m / kdiv;
+        g.kt = d.m / 16;
         g.out = B;
-        CAPDEC_TRY(launch_symmetric<false>(g, split, nz, slab, s));
+        CAPDEC_TRY(launch_symmetric<false>(g, nz, slab, s));
 
         const bool end = k + 1 == n.steps;
         const double next = top_of_step(n.a, n.b, n.c, sigma);
         const int sn = end ? 0 : exponent_for(next);
-        const bool next_split = k + 1 < n.exact_steps;
         StepArgs h = end ? last : StepArgs{};
         h.b = b;
         const View vx{X[k & 1], ldx, d.cp, d.rp}, vb{B, lda, d.m, d.m};
@@ -517,32 +503,26 @@ int run_batch(const Batch& b, int nz, const Dims& d, const Iteration& n, int dty
         h.R = X[k & 1]; h.ldr = ldx; h.strideR = (int64_t)d.x_elems;
         h.I = end ? d.rows : d.rp;
         h.J = end ? d.cols : d.cp;
-        h.kt = d.m / kdiv;
-        h.out = X[~k & 1]; h.ldo = (int64_t)d.cp * (next_split ? 2 : 1); h.out_split = next_split; h.strideO = (int64_t)d.x_elems;
+        h.kt = d.m / 16;
+        h.out = X[~k & 1]; h.ldo = ldx; h.strideO = (int64_t)d.x_elems;
         if (d.tall) {
             h.P = View{X[k & 1], ldx, d.rp, d.rp}; h.strideP = (int64_t)d.x_elems;
             h.Q = vb; h.strideQ = (int64_t)d.a_elems;
-            if (!end) CAPDEC_TRY((launch_split<false, false, INNER>(h, split, nz, s)));
-            else if (mo.on) CAPDEC_TRY((launch_split<false, false, UPDATE>(h, split, nz, s)));
-            else CAPDEC_TRY((launch_split<false, false, RESULT>(h, split, nz, s)));
+            if (!end) CAPDEC_TRY((launch_sized<false, false, INNER>(h, nz, s)));
+            else if (mo.on) CAPDEC_TRY((launch_sized<false, false, UPDATE>(h, nz, s)));
+            else CAPDEC_TRY((launch_sized<false, false, RESULT>(h, nz, s)));
         } else {
             h.P = vb; h.strideP = (int64_t)d.a_elems;
             h.Q = vx; h.strideQ = (int64_t)d.x_elems;
-            if (!end) CAPDEC_TRY((launch_split<false, true, INNER>(h, split, nz, s)));
-            else if (mo.on) CAPDEC_TRY((launch_split<false, true, UPDATE>(h, split, nz, s)));
-            else CAPDEC_TRY((launch_split<false, true, RESULT>(h, split, nz, s)));
+            if (!end) CAPDEC_TRY((launch_sized<false, true, INNER>(h, nz, s)));
+            else if (mo.on) CAPDEC_TRY((launch_sized<false, true, UPDATE>(h, nz, s)));
+            else CAPDEC_TRY((launch_sized<false, true, RESULT>(h, nz, s)));
         }
         sigma = next;
         sx = sn;
-        split = next_split;
     }
     return 0;
 }
-
-// A bfloat16 result is rounded by up to 2^-8: its last two steps take one fp16 number per value, a third of the products.  Their
-// error, about 2^-12 a value and grown once by a, stays below that rounding (6.5e-4 against 1.7e-3 in norm for gradients
-// of a few strong directions over noise; 2.5e-3 where all but 16 of 512 directions are a thousandth of those).
-int exact_steps(int steps, int dtype) { return dtype == CAPDEC_BF16 ? (steps > 2 ? steps - 2 : 0) : steps; }
 
 // the iterate's bound must leave the powers of two in fp32's and fp16's range
 bool iteration_fits(const float* coeffs, int steps) {
@@ -576,7 +556,7 @@ int capdec_orthogonalize(const capdec_matrix* mats, int count, int rows, int col
         CAPDEC_REQUIRE(mats[k].src && mats[k].dst && (rows == 1 || (mats[k].ld_src >= cols && mats[k].ld_dst >= cols)));
     if (!capdec_aligned16(workspace)) return CAPDEC_EALIGN;
     if (workspace_bytes < capdec_orthogonalize_workspace_bytes(count, rows, cols)) return CAPDEC_ENOMEM;
-    const Iteration n{steps, exact_steps(steps, dtype), coeffs[0], coeffs[1], coeffs[2], eps};
+    const Iteration n{steps, coeffs[0], coeffs[1], coeffs[2], eps};
     for (int k = 0; k < count; k += d.batch) {
         const int nz = count - k < d.batch ? count - k : d.batch;
         Batch b{};
@@ -601,7 +581,7 @@ int capdec_muon_step(const capdec_muon_param* params, int count, int rows, int c
     }
     if (!capdec_aligned16(workspace)) return CAPDEC_EALIGN;
     if (workspace_bytes < capdec_orthogonalize_workspace_bytes(count, rows, cols)) return CAPDEC_ENOMEM;
-    const Iteration n{steps, steps, coeffs[0], coeffs[1], coeffs[2], eps};
+    const Iteration n{steps, coeffs[0], coeffs[1], coeffs[2], eps};
     const Momentum mo{1, nesterov, momentum, grad_scale};
     for (int k = 0; k < count; k += d.batch) {
         const int nz = count - k < d.batch ? count - k : d.batch;

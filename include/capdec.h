@@ -663,8 +663,8 @@ int capdec_vocab_ce_backward(const capdec_vocab_ce* a /*host*/, const void* save
  * Orthogonalised updates of weight matrices (no counterpart in the reference, whose optimizer is Adam, train.py:217).
  *   X = U / (|U|_F + eps);  steps times:  A = X X^T, X <- a X + (b A + c A^2) X      (coeffs = {a, b, c}, host)
  * which drives the singular values of U towards 1.  `count` matrices of one shape per call, rows x cols with unit column
- * stride, rows * cols <= 2^31, any of 16 bits or fp32.  Sums are fp32, intermediate values pairs of fp16 numbers (22 bits),
- * in the last two steps towards a bfloat16 result single fp16 numbers.  Coefficients under which singular values in
+ * stride, rows * cols <= 2^31, any of 16 bits or fp32.  Sums are fp32, intermediate values pairs of fp16 numbers (22 bits).
+ * Coefficients under which singular values in
  * [0, 1] could grow beyond 64 within the steps are refused (CAPDEC_EINVAL), as are more than 32 steps.  A zero matrix stays
  * zero.  Sums run in fixed orders: results repeat bit for bit.
  * capdec_orthogonalize: dst = the last X; dst may be src.
