@@ -69,8 +69,8 @@ __device__ __forceinline__ int acc_row(int e, int h) { return (e & 3) + 8 * (e >
 
 // 16 bytes per lane from `src` to 1 KiB of LDS at `dst` (wave-uniform), asynchronously.  Written as assembly because the
 // compiler, where it knows of such loads, waits for all of them before every transposing LDS read; it has no output
-// registers, and contract() waits for it by count.  m0 has no other user: a kernel's tiles all come this way, or all through
-// the builtin.
+// registers, and contract() waits for it by count.  m0 is reserved, so that no clobber list takes it: it has no other
+// user, since a kernel's tiles all come this way, or all through the builtin (the generated code has no kernel with both).
 __device__ __forceinline__ void dma16(const short* src, short* dst) {
     const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) short*)dst);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src) : "memory");
@@ -395,10 +395,11 @@ inline unsigned make_map(Map& m, int ni, int nj, int nz) {
     return (unsigned)m.per * 8u;
 }
 __device__ __forceinline__ bool tile_of(const Map& m, unsigned block, int& ti, int& tj, int& z) {
+    if ((int)(block >> 3) >= m.per) return false;            // (no tiles at all: per is 0)
     const int t = (int)(block & 7) * m.per + (int)(block >> 3);
     const int plane = m.ni * m.nj;
     z = t / plane;
-    if ((int)(block >> 3) >= m.per || z >= m.nz) return false;
+    if (z >= m.nz) return false;
     int u = t - z * plane;
     const int band = u / (8 * m.nj);
     u -= band * 8 * m.nj;
