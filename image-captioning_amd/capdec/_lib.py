@@ -190,6 +190,7 @@ _SIGNATURES = {
     "capdec_vocab_ce_saved_bytes": (c_size_t, [POINTER(VocabCE)]),
     "capdec_vocab_ce_forward_workspace_bytes": (c_size_t, [POINTER(VocabCE)]),
     "capdec_vocab_ce_backward_workspace_bytes": (c_size_t, [POINTER(VocabCE)]),
+    "capdec_vocab_ce_tiles": (c_int, [POINTER(VocabCE), POINTER(c_int32)]),
     "capdec_vocab_ce_forward": (c_int, [POINTER(VocabCE), _P, c_size_t, _P, c_size_t, _P, _P, _P]),
     "capdec_vocab_ce_backward": (c_int, [POINTER(VocabCE), _P, c_size_t, _P, c_size_t, _P, _P, c_int, _P, c_int64, _P,
                                          c_int64, _P, _P]),

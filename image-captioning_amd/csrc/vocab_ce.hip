@@ -1422,6 +1422,16 @@ size_t capdec_vocab_ce_backward_workspace_bytes(const capdec_vocab_ce* a) {
     return make_plan(a, p) ? p.bwd : 0;
 }
 
+int capdec_vocab_ce_tiles(const capdec_vocab_ce* a, int32_t* tiles) {
+    Plan p;
+    CAPDEC_REQUIRE(tiles && make_plan(a, p));
+    const int wide = Wide::BI * Wide::BJ, big = Big::BI * Big::BJ, mid = Mid::BI * Mid::BJ;
+    tiles[0] = p.few ? 0 : p.few_z ? mid : p.wide_z ? wide : big;
+    tiles[1] = p.few || a->loss_only ? 0 : p.wide_dx ? wide : big;
+    tiles[2] = p.few || a->loss_only ? 0 : p.wide_dw ? wide : big;
+    return 0;
+}
+
 int capdec_vocab_ce_forward(const capdec_vocab_ce* a, void* saved, size_t saved_bytes, void* workspace,
                             size_t workspace_bytes, float* nll, float* loss, void* stream) {
     Plan p;

@@ -653,6 +653,9 @@ typedef struct capdec_vocab_ce {
 size_t capdec_vocab_ce_saved_bytes(const capdec_vocab_ce* a /*host*/);
 size_t capdec_vocab_ce_forward_workspace_bytes(const capdec_vocab_ce* a /*host*/);
 size_t capdec_vocab_ce_backward_workspace_bytes(const capdec_vocab_ce* a /*host*/);
+/* tiles[3] (host): elements of the output tiles that these sizes take for the logits, dx and dW (128 x 128, 256 x 128 or
+ * 256 x 256; 0 where there are none), so that tests and benchmarks know what they run. */
+int capdec_vocab_ce_tiles(const capdec_vocab_ce* a /*host*/, int32_t* tiles /*host*/);
 int capdec_vocab_ce_forward(const capdec_vocab_ce* a /*host*/, void* saved, size_t saved_bytes, void* workspace,
                             size_t workspace_bytes, float* nll, float* loss, void* stream);
 int capdec_vocab_ce_backward(const capdec_vocab_ce* a /*host*/, const void* saved, size_t saved_bytes, void* workspace,

@@ -1,8 +1,50 @@
 """The vocabulary cross entropy at the sizes that select each of its tiles, against the definition in 64 bits."""
+import ctypes
+
 import pytest
 import torch
 
+from test_gpu_vocab_ce import check, make
+
 pytestmark = pytest.mark.gpu
+
+MID, BIG, WIDE = 128 * 128, 256 * 128, 256 * 256
+
+
+def tiles_of(M, V, K, dt, loss_only=False):
+    from capdec import _lib
+    at = 1 << 20
+    code = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}[dt]
+    t = (ctypes.c_int32 * 3)()
+    assert _lib.load().capdec_vocab_ce_tiles(_lib.VocabCE(at, at, at, at, K, K, 0, M, V, K, code, loss_only), t) == 0
+    return tuple(t)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,V,K,want", [
+    (300, 2000, 96, (MID, BIG, BIG)),
+    (2000, 9000, 64, (BIG, BIG, BIG)),              # parts of dx and of dW, joined afterwards
+    (2000, 16500, 2048, (WIDE, WIDE, WIDE)),        # dx in parts
+    (8100, 2000, 2048, (WIDE, WIDE, WIDE)),         # dW in parts
+    (1700, 16500, 1536, (WIDE, BIG, WIDE))])
+def test_gradients_with_every_tile(M, V, K, want, dt):
+    """With a bias and ignored rows; a retuned rule that leaves a tile without a test shows here."""
+    assert tiles_of(M, V, K, dt) == want
+    x, W, b, t = make(M, V, K, dt, seed=70)
+    t[-1] = V - 1
+    check(x, W, b, t, "mean")
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,V,K,want", [(300, 2000, 96, MID), (2000, 9000, 64, BIG), (2000, 16500, 2048, WIDE)])
+def test_loss_alone_with_every_tile(M, V, K, want, dt):
+    from capdec import functional as F
+    from test_gpu_vocab_ce import definition, near
+    assert tiles_of(M, V, K, dt, True) == (want, 0, 0)
+    x, W, b, t = make(M, V, K, dt, seed=71)
+    t[-1] = V - 1
+    (nll, *_), (tol, *_) = definition(x, W, b, t, torch.zeros(M, device="cuda"))
+    near(F.vocab_cross_entropy(x, W, b, t, reduction="none"), nll, torch.full_like(nll, tol), "loss")
 
 
 def test_largest_number_of_logits():
