@@ -35,7 +35,10 @@ struct Batch {
 
 // A and A^2 are symmetric: from 768 on, the upper triangle of 256 x 256 or 128 x 128 tiles, its contraction in parts where
 // that fills the CUs better.  Times in us from measurements of split operands (a k-tile takes a CU 1.36 with one 256 x 256
-// tile; 0.45, 0.80, 1.15 with one to three 128 x 128 tiles); the parts' sums go to memory and back at 4 TB/s.
+// tile; 0.58, 0.80, 1.15 with one to three 128 x 128 tiles); the parts' sums go to memory and back at 4 TB/s.  (With 0.45 for
+// one tile A^2 of 2048 stayed a whole square: 2048 x 2048 910 instead of 770 us, 2560 x 2560 1226 instead of 1263.)
+// From 768 on: 16 matrices of 768 x 768 take 817 us as triangles and 987 whole, 768 x 4096 358 and 398; one square matrix would
+// be faster whole up to 1024 (768: 249 and 187, 1024: 279 and 233), batches of 640 slower (16 of them: 568, as triangles 498).
 struct Symmetric {
     bool on, wide;
     int nsplit;
@@ -46,7 +49,7 @@ Symmetric symmetric_plan(int m, int kt, int nz) {
     if (m < 768) return best;
     auto mids = [](int64_t n) {
         const int64_t per = (n + 255) / 256, left = per % 3;
-        return (double)(per / 3) * 1.15 + (left == 2 ? 0.80 : left == 1 ? 0.45 : 0.0);
+        return (double)(per / 3) * 1.15 + (left == 2 ? 0.80 : left == 1 ? 0.58 : 0.0);
     };
     const int64_t w = (m + 255) / 256, h = (m + 127) / 128;
     // the whole square, by the rule of launch_sized
