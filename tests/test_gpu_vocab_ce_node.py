@@ -127,3 +127,14 @@ def test_tangents_are_refused(which, M):
             with torch.no_grad(), pytest.raises(RuntimeError, match="jvp|forward"):
                 loss_of(*ins, t)
     assert bool(loss_of(*(v.detach() for v in (x, W, b)), t).isfinite())
+
+
+def test_recomputed_in_the_backward_pass():
+    """Under torch's activation checkpointing, which runs the forward pass again."""
+    from torch.utils.checkpoint import checkpoint
+    x, W, b, t = make(100, 500, 64, torch.bfloat16)
+    want = torch.autograd.grad(loss_of(x, W, b, t), (x, W, b))
+    for reentrant in (False, True):
+        ins = [v.detach().requires_grad_() for v in (x, W, b)]
+        checkpoint(loss_of, *ins, t, use_reentrant=reentrant).backward()
+        assert all(torch.equal(p.grad, q) for p, q in zip(ins, want))

@@ -156,3 +156,28 @@ def test_weights_near_the_end_of_the_range(M, dt, far, reduction):
     # x has fewer digits at its small end, and its products with G may leave the range: steps of 2^-149 each
     near(grads[1], want[1], tol[1] + M * 2.0 ** -149, "dW", 2.0 ** -134 if dt == torch.bfloat16 else 0.0)
     near(grads[2], want[2], tol[2], "db")
+
+
+def test_far_rows_in_pieces_and_at_odd_strides():
+    """More than one piece of the vocabulary, operands and gradients inside wider matrices at odd offsets."""
+    from capdec import ops
+    M, V, K = 30000, 10007, 37
+    x, W, b, t = make(M, V, K, torch.float32, seed=68)
+    W[5] *= 1e8
+    b[5] = float("-inf")
+    t[t == 5] = 6
+    xs, ws, gx, gw = (torch.full((r, K + 6), 7.0, device="cuda") for r in (M, V, M, V))
+    xv, wv, dx, dW = (v[:, 1:1 + K] for v in (xs, ws, gx, gw))
+    xv.copy_(x), wv.copy_(W)
+    _, loss, state = ops.vocab_ce_forward(xv, wv, b, t)
+    xs.fill_(float("nan"))
+    _, _, db = ops.vocab_ce_backward(state, dx=dx, dW=dW)
+    keep = torch.arange(V, device="cuda") != 5
+    w = torch.full((M,), 1 / int((t != 0).sum()), device="cuda")
+    (nll, *want), (tn, *tol) = definition(x, W[keep], b[keep], torch.where(t > 5, t - 1, t), w)
+    near(loss[0], nll.sum() * float(w[0]), tn + 2.0 ** -22 * nll.sum() * float(w[0]), "loss")
+    for got, ref, bound, name in zip((dx, dW[keep], db[keep]), want, tol, ("dx", "dW", "db")):
+        near(got, ref, bound, name)
+    assert int(dW[5].count_nonzero()) == 0
+    for wide in (gx, gw):
+        assert bool((wide[:, 0] == 7).all()) and bool((wide[:, 1 + K:] == 7).all())
