@@ -38,3 +38,20 @@ def test_forward_refuses_what_cannot_be_launched():
     n = 1 << 40
     assert lib.capdec_vocab_ce_forward(a, BASE, n, BASE, n, BASE, None, None) == -22
     assert lib.capdec_vocab_ce_backward(a, BASE, n, BASE, n, None, None, 1, BASE, 64, BASE, 64, None, None) == -22
+
+
+def test_tiles_of_sizes():
+    import ctypes
+
+    from capdec import _lib
+    lib = _lib.load()
+    t = (ctypes.c_int32 * 3)(7, 7, 7)
+
+    def a(M, dtype=0, loss_only=0, V=1000):
+        return _lib.VocabCE(BASE, BASE, None, BASE, 64, 64, 0, M, V, 64, dtype, loss_only)
+    assert lib.capdec_vocab_ce_tiles(None, t) == -22 and lib.capdec_vocab_ce_tiles(a(100), None) == -22
+    assert lib.capdec_vocab_ce_tiles(a(0), t) == -22 and tuple(t) == (7, 7, 7)
+    assert lib.capdec_vocab_ce_tiles(a(64), t) == 0 and tuple(t) == (0, 0, 0)            # float32: kernels without tiles
+    for dtype in (0, 1, 2):
+        assert lib.capdec_vocab_ce_tiles(a(65, dtype), t) == 0 and tuple(t) == (128 * 128, 256 * 128, 256 * 128)
+        assert lib.capdec_vocab_ce_tiles(a(65, dtype, 1), t) == 0 and tuple(t) == (128 * 128, 0, 0)
