@@ -1115,7 +1115,10 @@ def _matrices(what, ts, dtypes):
     if isinstance(ts, torch.Tensor):
         if ts.dim() < 2:
             raise RuntimeError(f"capdec {what}: a matrix or a batch of matrices expected, got shape {tuple(ts.shape)}")
-        ts = list(ts.unbind(0)) if ts.dim() == 3 else [ts] if ts.dim() == 2 else list(ts.flatten(0, -3).unbind(0))
+        batch = [ts]
+        while batch and batch[0].dim() > 2:            # views, whatever the batch's strides: what is written must arrive in ts
+            batch = [m for t in batch for m in t.unbind(0)]
+        ts = batch
     ts = list(ts)
     for t in ts:
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
