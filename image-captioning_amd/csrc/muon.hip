@@ -187,7 +187,8 @@ __global__ __launch_bounds__(256) void normalise_kernel(Batch b, int rows, int c
     for (int k = threadIdx.x & 63; k < nparts; k += 64) s += part[blockIdx.y * NORM_BLOCKS + k];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    const float inv = s == 0.0 ? 0.f : (float)((double)scale / (sqrt(s) + (double)eps));
+    int e2 = 0;                        // 1 / (|U| + eps) may be more than an fp32 number holds
+    const float inv = s == 0.0 ? 0.f : (float)frexp((double)scale / (sqrt(s) + (double)eps), &e2);
     short* x = X + blockIdx.y * x_elems;
     const int cpr = cp / 8;
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < (int64_t)rp * cpr; t += (int64_t)gridDim.x * 256) {
@@ -218,7 +219,7 @@ __global__ __launch_bounds__(256) void normalise_kernel(Batch b, int rows, int c
         for (int e = 0; e < 8; ++e) {
             if (mo.on) u[e] = mo.nesterov ? fmaf(mo.mu, m[e], u[e] * mo.grad_scale) : m[e];
             short h, l;
-            split16(u[e] * inv, h, l);
+            split16(ldexpf(u[e], e2) * inv, h, l);
             hi[e] = h;
             lo[e] = l;
         }

@@ -40,3 +40,16 @@ def test_empty_batches():
         assert ops.orthogonalize(torch.empty(shape, device="cuda")).shape == shape
     assert ops.orthogonalize([]) == []
     ops.muon_step([], [], [], lr=0.1)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale", [1e-33, 1e-36, 1e36])
+def test_norms_at_the_ends_of_the_range(scale, dt):
+    """Without eps: matrices whose norm has no reciprocal in fp32, and large ones; on their own (rounded) values."""
+    from capdec import ops
+    from test_gpu_muon import definition, near
+    G = (gradient_like((60, 90)) * scale).to(dt)
+    near(ops.orthogonalize(G, eps=0.0), definition(G, eps=0.0), dt)
+    m, p = torch.zeros(60, 90, device="cuda"), torch.zeros(60, 90, device="cuda")
+    ops.muon_step([p], [G.float()], [m], lr=1.0, momentum=0.0, nesterov=False, eps=0.0, update_scale=1.0)
+    near(-p, definition(G, eps=0.0), torch.float32)
